@@ -134,11 +134,11 @@ def _qkv(case, seed, tokens):
 
 
 def _block_scale(amax):
-    """The least power of two s with amax <= 448 s, as fp32 (1 for a block of zeros)."""
+    """The least power of two s with amax <= 448 s, as fp32 (the least of all for a block of zeros)."""
     mantissa, exponent = torch.frexp(amax)  # amax = mantissa * 2^exponent, mantissa in [1/2, 1); 448 = 7/8 * 2^9
     exponent = exponent - 9 + (mantissa > 0.875).to(exponent.dtype)
-    scale = torch.ldexp(torch.ones_like(amax), exponent.clamp(MIN_EXPONENT, MAX_EXPONENT))
-    return torch.where(amax > 0, scale, torch.ones_like(scale))
+    exponent = torch.where(amax > 0, exponent, MIN_EXPONENT).clamp(MIN_EXPONENT, MAX_EXPONENT)
+    return torch.ldexp(torch.ones_like(amax), exponent)
 
 
 def _random_blocks(case, seed, blocks, factor):
@@ -324,7 +324,7 @@ def _append_rows(codes, scales, x, slots, blocks, inverse, first):
     amax.index_reduce_(0, inverse, x.abs().amax(-1), "amax")
     before = scales[blocks]
     scale = _block_scale(amax)
-    scale = torch.where((first > 0)[:, None] & ((before >= scale) | (amax == 0)), before, scale)
+    scale = torch.where((first > 0)[:, None], torch.maximum(before, scale), scale)
     raw = codes.view(torch.uint8)
     held = raw[blocks]
     moved = (held.view(E4M3).float() * (before / scale)[..., None, None]).to(E4M3).view(torch.uint8)
@@ -437,11 +437,11 @@ def exact(case, seed):
                 x = rows[at[r] + a - first:at[r] + b - first].double().transpose(0, 1)  # [H, b - a, D]
                 block = first_slots[at[r] + a - first] // bs
                 top = x.abs().amax((1, 2))
-                scale = torch.where(top > 0, torch.exp2(torch.ceil(torch.log2(top / E4M3_MAX))), 1.0)
+                scale = torch.exp2(torch.ceil(torch.log2(top / E4M3_MAX)).clamp_min(MIN_EXPONENT))
                 held = a - j * bs
                 if held:
                     old = scales[block].clone()
-                    scale = torch.where((old >= scale) | (top == 0), old, scale)
+                    scale = torch.maximum(old, scale)
                     moved = values[block, :, :held] * (old / scale)[:, None, None]
                     values[block, :, :held] = moved.to(E4M3).double()
                 values[block, :, held:held + b - a] = (x / scale[:, None, None]).to(E4M3).double()
