@@ -6,6 +6,7 @@ points raise if the library is missing or a tensor is not on a ROCm device.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -26,7 +27,7 @@ KEY_DENSE, KEY_UNIFORM, KEY_MIXED = 0, 1, 2
 VALUE_DENSE, VALUE_UNIFORM = 0, 1
 SELECT_MAGNITUDE, SELECT_VARIANCE, SELECT_GIVEN = 0, 1, 2
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}
 # element types the kernels read and write (sources, outputs, metadata)
@@ -148,13 +149,48 @@ class CopyBlock(ctypes.Structure):
 
 COPY_MAX_BLOCKS = 8
 
+
+def _fields(pointers: str, integers: str, more=()) -> list:
+    return [(n, ctypes.c_void_p) for n in pointers.split()] + [(n, ctypes.c_int64) for n in integers.split()] + list(more)
+
+
+class PromptAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("query keys values out", "q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh o_sb o_st o_sh"),
+        *_fields("q_starts k_starts", "requests Hq Hkv D q_tokens k_tokens dtype"),
+        ("scale", ctypes.c_double), ("causal", ctypes.c_int64), ("fill", ctypes.c_int64),
+    ]
+
+
+class BlockTablesArgs(ctypes.Structure):
+    _fields_ = _fields("table lengths free state tokens slots starts", "total requests max_blocks blocks block_size")
+
+
+class AppendBlocksArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("keys values", "dtype k_st k_sh v_st v_sh"),
+        *_fields("slots", "tokens H D blocks block_size"),
+        *_fields("key_codes value_codes key_scale value_scale nonfinite", ""),
+    ]
+
+
+class BlockAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("query out", "dtype q_st q_sh o_st o_sh tokens"),
+        *_fields("starts table lengths", "requests max_blocks blocks block_size"),
+        *_fields("key_codes value_codes key_scale value_scale", "Hq Hkv D"),
+        ("scale", ctypes.c_double), ("max_tokens", ctypes.c_int64), ("fill", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
 EXPORTED = (
     "dkv_last_error", "dkv_abi_version", "dkv_quantize_rows", "dkv_quantize_row_blocks", "dkv_quantize_value_rows",
     "dkv_quantize_key_pages",
     "dkv_dequantize_rows",
     "dkv_dequantize_mixed", "dkv_decode_workspace_bytes", "dkv_decode_attention", "dkv_decode_attention_noalloc",
     "dkv_decode_scratch_bytes", "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize",
-    "dkv_decode_route",
+    "dkv_decode_route", "dkv_prompt_attention", "dkv_reserve_blocks", "dkv_release_blocks", "dkv_append_blocks",
+    "dkv_block_attention", "dkv_block_attention_workspace_bytes",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -193,10 +229,19 @@ def load() -> ctypes.CDLL:
         lib.dkv_decode_route.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(DecodeKernels)]
         lib.dkv_materialize.argtypes = [ctypes.POINTER(MaterializeArgs), vp]
         lib.dkv_copy_token_blocks.argtypes = [ctypes.POINTER(CopyBlock), i64, vp]
+        lib.dkv_prompt_attention.argtypes = [ctypes.POINTER(PromptAttentionArgs), vp]
+        lib.dkv_reserve_blocks.argtypes = [ctypes.POINTER(BlockTablesArgs), vp]
+        lib.dkv_release_blocks.argtypes = [ctypes.POINTER(BlockTablesArgs), vp]
+        lib.dkv_append_blocks.argtypes = [ctypes.POINTER(AppendBlocksArgs), vp]
+        lib.dkv_block_attention.argtypes = [ctypes.POINTER(BlockAttentionArgs), vp]
+        lib.dkv_block_attention_workspace_bytes.argtypes = [i64, i64, i64, i64]
+        lib.dkv_block_attention_workspace_bytes.restype = i64
         for name in ("dkv_quantize_rows", "dkv_quantize_row_blocks", "dkv_quantize_value_rows", "dkv_quantize_key_pages",
                      "dkv_dequantize_rows",
                      "dkv_dequantize_mixed", "dkv_decode_attention", "dkv_decode_attention_noalloc",
-                     "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize", "dkv_decode_route"):
+                     "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize", "dkv_decode_route",
+                     "dkv_prompt_attention", "dkv_reserve_blocks", "dkv_release_blocks", "dkv_append_blocks",
+                     "dkv_block_attention"):
             getattr(lib, name).restype = ctypes.c_int
         if lib.dkv_abi_version() != ABI_VERSION:
             raise RuntimeError("libdartkv_hip.so ABI version mismatch; rebuild it")
@@ -242,6 +287,16 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(index)
     return torch.cuda.current_stream(index).cuda_stream
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one (HIP launches go to the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE_ALREADY
+    return torch.cuda.device(device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def ptr(t: Optional[torch.Tensor]) -> int:

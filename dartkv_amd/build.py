@@ -21,7 +21,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdartkv_hip.so")
 SOURCES = ["capi.hip", "quantize.hip", "decode.hip", "decode_fast.hip", "decode_uniform.hip", "decode_tiles.hip",
-           "materialize.hip", "prep.hip", "copy.hip"]
+           "materialize.hip", "prep.hip", "copy.hip", "prompt.hip", "block_tables.hip", "block_append.hip",
+           "block_attention.hip", "block_chunks.hip"]
 ARCH = os.environ.get("DKV_OFFLOAD_ARCH", "gfx950")
 
 
@@ -48,7 +49,8 @@ def command(output: str = LIB) -> list[str]:
 
 # Sources whose kernels must keep every value in registers: a spill to scratch
 # (private memory in HBM) would add memory traffic to the page and tile kernels' loops.
-NO_SCRATCH = {"decode_fast.hip", "decode_uniform.hip", "decode_tiles.hip"}
+NO_SCRATCH = {"decode_fast.hip", "decode_uniform.hip", "decode_tiles.hip", "prompt.hip", "block_attention.hip",
+              "block_chunks.hip"}
 
 
 def _run(cmd: list[str], verbose: bool) -> str:

@@ -1,0 +1,484 @@
+// Attention of a tile of query rows over a request's keys (gfx950, wave64): the kernel of prompt_attention
+// (16-bit keys and values, prompt.hip) and of block_attention's long chunks (e4m3 blocks, blocks_chunk.hip).
+//
+// Rows.  The query heads of a KV head are rows of one problem: row t * G + g is token t of head h * G + g, so a
+// tile of BM rows reads its keys once for all G heads, and a causal tile of 128 rows masks no more than 128 / G
+// tokens' diagonal.  Row t * G + g sees the first t + 1 + (nk - nq) keys (all nk without the causal mask).
+//
+// One pass over the keys, 64 at a time, with a running maximum m and sum l (fp32) per row:
+//   s = c q.k (c = scale log2 e), p = 2^(s - m), l += p, o += p v, and o, l times 2^(m - m') when m grows.
+// m is only raised when a row's maximum exceeds it by more than 8 (2^8: p stays within bf16 and fp16, and l and
+// o are sums of the same p), so most tiles scale nothing.
+//
+// Matrix layout.  Both products are v_mfma_f32_32x32x16 with the query row in the column of the result:
+// S^T = K Q^T puts keys 8 (i / 4) + 4 half + i % 4 (i < 16) of 32 in lane (row, half)'s accumulators, and
+// O^T = V^T P^T takes P^T's 16 keys of a step from the same lane: step ks, slot j is key 16 ks + 8 (j / 4) +
+// 4 half + j % 4, accumulator 8 (ks % 2) + j.  So P never leaves its lane, a row's maximum takes one exchange
+// between the wave's halves, and its scale one value per lane.  V^T's operand has four keys of one channel per
+// ds_read_b64_tr_b16: V stays in token order in LDS.
+//
+// LDS.  Rows of 2 DP bytes in chunks of 16, chunk c of row r at c ^ swizzle(r): sixteen consecutive rows' reads
+// of one chunk (K) and four consecutive rows' reads of four chunks (V) fall in different banks.  Two buffers of
+// 64 keys; the next tile's copies are in flight while a tile is computed (one barrier per tile).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dkv_device.h"
+
+namespace dkv {
+
+struct PromptParams {
+  const void *q, *k, *v;
+  void* o;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh;  // strides in elements
+  const int32_t *q_starts, *k_starts;  // [R + 1], or NULL: every request has q_tokens (k_tokens)
+  int32_t R, H, G, D;
+  int64_t q_tokens, k_tokens;  // rows of the packed tensors, or of each request
+  float c;                     // scale * log2(e)
+  int32_t causal, fill;        // fill: rows behind the last request become 0
+  // e4m3 blocks
+  const uint8_t *kc, *vc;       // [blocks][H][bs][D]
+  const float *kscale, *vscale;  // [blocks][H]
+  const int32_t *table, *lengths;
+  int64_t blocks;
+  int32_t max_blocks, bs_shift;
+  int32_t skip_rows;  // requests of at most this many rows are another kernel's
+};
+
+namespace prompt {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kKeys = 64;  // keys of a tile
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0,
+                                                  0);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, half2v));
+}
+
+// The other half's value of the same row.
+__device__ __forceinline__ float other_half(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <int DP>
+__device__ __forceinline__ int swizzle(int row) {
+  if constexpr (DP == 64)
+    return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  else
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+// 64 x 16 bytes, lane l's from byte `offset` of the buffer to LDS address lds + 16 l; zeros outside the buffer.
+// From inline assembly, so that the compiler does not wait for it before the other buffer's reads.
+__device__ __forceinline__ void buffer_to_lds(u32x4 rsrc, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(offset), "s"(lds),
+               "s"(rsrc)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A buffer descriptor of `bytes` bytes at `base` (both wave-uniform).
+__device__ __forceinline__ u32x4 buffer(const void* base, uint32_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)base;
+  return (u32x4){uniform((uint32_t)a), uniform((uint32_t)(a >> 32)) & 0xffffu, uniform(bytes), 0x00027000u};
+}
+
+// Which request and row tile a workgroup has: the requests' tiles in order, found by a wave's scan over them.
+struct Tile {
+  int request;  // -1: none
+  int tile, rows;
+  int64_t q0;   // first token
+  int nq;
+};
+
+template <int BM>
+__device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) {
+  Tile t = {-1, 0, 0, 0, 0};
+  const int lane = threadIdx.x & 63;
+  if (!p.q_starts) {
+    const int rows = (int)p.q_tokens * p.G, tiles = (rows + BM - 1) / BM;
+    const int r = (int)(index / tiles);
+    if (r >= p.R) return t;
+    t = {r, (int)(index - (int64_t)r * tiles), rows, 0, (int)p.q_tokens};
+    return t;
+  }
+  int64_t before = 0;
+  const int total = p.R + (p.fill ? 1 : 0);
+  for (int base = 0; base < total; base += 64) {
+    const int r = base + lane;
+    int64_t a = 0, b = 0;
+    if (r < total) {
+      a = p.q_starts[r];
+      b = r < p.R ? p.q_starts[r + 1] : p.q_tokens;
+      a = a < 0 ? 0 : a > p.q_tokens ? p.q_tokens : a;  // (never outside the tensor, whatever the starts say)
+      b = b < a ? a : b > p.q_tokens ? p.q_tokens : b;
+    }
+    int rows = (int)(b - a) * p.G;
+    if (rows <= p.skip_rows && r < p.R) rows = 0;
+    const int tiles = (rows + BM - 1) / BM;
+    int sum = tiles;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int up = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += up;
+    }
+    const uint64_t hit = __ballot(before + sum > index);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      t.request = base + l;
+      t.rows = __shfl(rows, l, 64);
+      t.tile = (int)(index - before) - (__shfl(sum, l, 64) - __shfl(tiles, l, 64));
+      t.q0 = __shfl((int)a, l, 64);
+      t.nq = (int)(__shfl((int)b, l, 64) - t.q0);
+      return t;
+    }
+    before += __shfl(sum, 63, 64);
+  }
+  return t;
+}
+
+// Copies of 16-bit keys and values: straight from memory to LDS.
+template <int DP, int WAVES>
+struct DenseSource {
+  const char *k, *v;
+  int64_t kst, vst;  // bytes
+  int nk, valid;     // valid: bytes of a row
+  uint32_t koff[kKeys * DP / 512 / WAVES], voff[kKeys * DP / 512 / WAVES];
+  static constexpr int kCopies = kKeys * DP / 512 / WAVES;  // of a wave, for keys and for values
+  static constexpr int kRowBytes = 2 * DP;
+
+  __device__ __forceinline__ void init(const PromptParams& p, const Tile& t, int h, int64_t k0, int nk_) {
+    const int64_t b = p.k_starts ? 0 : t.request;
+    k = (const char*)p.k + 2 * (b * p.k_sb + k0 * p.k_st + h * p.k_sh);
+    v = (const char*)p.v + 2 * (b * p.v_sb + k0 * p.v_st + h * p.v_sh);
+    kst = 2 * p.k_st, vst = 2 * p.v_st, nk = nk_, valid = 2 * p.D;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int at = (i * WAVES + wave) * 1024 + lane * 16;  // LDS byte of the tile
+      const int row = at / kRowBytes, chunk = ((at % kRowBytes) >> 4) ^ swizzle<DP>(row);
+      const bool in = chunk * 16 < valid;
+      koff[i] = in ? (uint32_t)(row * kst) + chunk * 16 : 0x80000000u;
+      voff[i] = in ? (uint32_t)(row * vst) + chunk * 16 : 0x80000000u;
+    }
+  }
+  // Start the copies of keys [j, j + 64) to the LDS tiles at lk and lv.
+  __device__ __forceinline__ void issue(int j, uint32_t lk, uint32_t lv) {
+    const int left = nk - j < kKeys ? nk - j : kKeys;
+    const u32x4 rk = buffer(k + j * kst, (uint32_t)((left - 1) * kst) + valid);
+    const u32x4 rv = buffer(v + j * vst, (uint32_t)((left - 1) * vst) + valid);
+    const int wave = uniform(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) buffer_to_lds(rk, koff[i], lk + (i * WAVES + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) buffer_to_lds(rv, voff[i], lv + (i * WAVES + wave) * 1024);
+  }
+};
+
+// Keys and values held in e4m3 blocks: read into registers while the tile before is computed, then converted into
+// LDS.  bf16 queries: codes times their scale (exact), fp16 queries: keys as bare fp16 codes (a scaled value may
+// leave fp16's range), whose scale goes to the logits, and values as scaled bf16.
+template <int DP, bool BF, int WAVES>
+struct BlockSource {
+  static constexpr int kChunks = 4 * DP / (64 * WAVES);  // 16 codes each, of a thread
+  static constexpr int kRowBytes = 2 * DP;
+  const PromptParams& p;
+  const int32_t* table;
+  int h, nk;
+  int id[kChunks];
+  u32x4 k[kChunks], v[kChunks];
+  float ks[kChunks], vs[kChunks];
+
+  __device__ __forceinline__ BlockSource(const PromptParams& p_, int request, int h_, int nk_)
+      : p(p_), table(p_.table + (int64_t)request * p_.max_blocks), h(h_), nk(nk_) {}
+  __device__ __forceinline__ static int row_of(int i) { return (threadIdx.x + i * 64 * WAVES) / (DP / 16); }
+  __device__ __forceinline__ static int chunk_of(int i) { return (threadIdx.x + i * 64 * WAVES) % (DP / 16); }
+  // The blocks of keys [j, j + 64), asked for a tile ahead.
+  __device__ __forceinline__ void blocks(int j) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int at = (j + row_of(i)) >> p.bs_shift;
+      id[i] = table[at < p.max_blocks ? at : p.max_blocks - 1];
+    }
+  }
+  __device__ __forceinline__ void issue(int j) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int key = j + row_of(i), ch = 16 * chunk_of(i);
+      const bool in = key < nk && ch < p.D, good = (uint32_t)id[i] < (uint64_t)p.blocks;
+      const int64_t bh = (int64_t)(good ? id[i] : 0) * p.H + h;
+      const int64_t off = ((bh << p.bs_shift) + (key & ((1 << p.bs_shift) - 1))) * p.D + (in ? ch : 0);
+      k[i] = *(const u32x4*)(p.kc + off), v[i] = *(const u32x4*)(p.vc + off);
+      ks[i] = p.kscale[bh], vs[i] = p.vscale[bh];
+      if (!in || !good) v[i] = (u32x4){0, 0, 0, 0};
+      if (!in) k[i] = (u32x4){0, 0, 0, 0};
+      else if (!good) k[i] = (u32x4){0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};  // NaN: a bad entry shows
+    }
+  }
+  template <bool AS_BF>
+  __device__ __forceinline__ static void convert(u32x4 w, float scale, u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t lo, hi;
+      if constexpr (AS_BF) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w[i], scale, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w[i], scale, true));
+      } else {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[i], 1.0f, true));
+      }
+      if (i < 2)
+        a[2 * i] = lo, a[2 * i + 1] = hi;
+      else
+        b[2 * i - 4] = lo, b[2 * i - 3] = hi;
+    }
+  }
+  // The tile read last to LDS: keys, values and (fp16) the scale of every 16 keys.
+  __device__ __forceinline__ void finish(char* lk, char* lv, float* lscale) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int row = row_of(i), chunk = chunk_of(i);
+      const int a = row * kRowBytes + (((2 * chunk) ^ swizzle<DP>(row)) << 4);
+      const int b = row * kRowBytes + (((2 * chunk + 1) ^ swizzle<DP>(row)) << 4);
+      u32x4 x, y;
+      convert<BF>(k[i], ks[i], x, y);
+      *(u32x4*)(lk + a) = x, *(u32x4*)(lk + b) = y;
+      convert<true>(v[i], vs[i], x, y);
+      *(u32x4*)(lv + a) = x, *(u32x4*)(lv + b) = y;
+      if (!BF && chunk == 0 && row % 16 == 0) lscale[row / 16] = ks[i];
+    }
+  }
+};
+
+template <int DP, bool BF, int WAVES, bool BLOCKS>
+__global__ void __launch_bounds__(64 * WAVES) prompt_tiles(PromptParams p) {
+  constexpr int BM = 32 * WAVES, KS = DP / 16, CB = DP / 32;
+  constexpr int kRowBytes = 2 * DP, kTileBytes = kKeys * kRowBytes;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+
+  const int h = (int)(blockIdx.x % p.H);
+  Tile t = find_tile<BM>(p, blockIdx.x / p.H);
+  if (t.request < 0) return;
+  t.request = uniform(t.request), t.tile = uniform(t.tile), t.rows = uniform(t.rows), t.nq = uniform(t.nq);
+  t.q0 = (int64_t)uniform((uint32_t)t.q0);
+  t.tile = (t.rows + BM - 1) / BM - 1 - t.tile;  // the longest tiles first
+  int64_t k0 = 0;
+  int nk = (int)p.k_tokens;
+  if (t.request >= p.R) {
+    nk = 0;
+  } else if constexpr (BLOCKS) {
+    const int64_t most = (int64_t)p.max_blocks << p.bs_shift, length = p.lengths[t.request];
+    nk = uniform((int)(length < 0 ? 0 : length > most ? most : length));
+  } else if (p.k_starts) {
+    int64_t a = p.k_starts[t.request], b = p.k_starts[t.request + 1];
+    a = a < 0 ? 0 : a > p.k_tokens ? p.k_tokens : a;
+    b = b < a ? a : b > p.k_tokens ? p.k_tokens : b;
+    k0 = (int64_t)uniform((uint32_t)a), nk = uniform((int)(b - a));
+  }
+
+  // this lane's row, how many keys it sees, and its query in the products' operand layout
+  const int row = t.tile * BM + wave * 32 + (lane & 31);
+  const bool real = row < t.rows;
+  const int token = row / p.G, head = h * p.G + row % p.G;
+  const int64_t qb = p.q_starts ? 0 : t.request;
+  auto limit_of = [&](int tok) {
+    int n = p.causal ? tok + 1 + nk - t.nq : nk;
+    return n < 0 ? 0 : n > nk ? nk : n;
+  };
+  const int limit = real ? limit_of(token) : 0;
+  const int last_row = min(t.tile * BM + BM, t.rows) - 1;
+  const int tile_limit = uniform(limit_of(last_row / p.G));
+  const int wave_first = min(t.tile * BM + wave * 32, t.rows - 1), wave_last = min(wave_first + 31, t.rows - 1);
+  const bool wave_real = t.tile * BM + wave * 32 < t.rows;
+  const int wave_min = uniform(limit_of(wave_first / p.G));
+  const int wave_max = wave_real ? uniform(limit_of(wave_last / p.G)) : 0;
+
+  u32x4 q[KS];
+  {
+    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + (t.q0 + token) * p.q_st + head * p.q_sh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int ch = 16 * ks + 8 * half;
+      q[ks] = (u32x4){0, 0, 0, 0};
+      if (real && ch < p.D) q[ks] = *(const u32x4*)(src + 2 * ch);
+    }
+  }
+
+  f32x16 o[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[cb][i] = 0.f;
+  float m = -3.402823466e38f, l = 0.f;
+
+  // LDS bytes of this lane's operand chunks within a tile
+  int kaddr[KS], vaddr[CB][2];
+  {
+    const int key = lane & 31;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kaddr[ks] = key * kRowBytes + (((2 * ks + half) ^ swizzle<DP>(key)) << 4);
+    const int L = lane & 15;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int r = 8 * s + 4 * half + (L >> 2);
+        const int chunk = 4 * cb + 2 * ((lane >> 4) & 1) + ((L & 3) >> 1);
+        vaddr[cb][s] = r * kRowBytes + ((chunk ^ swizzle<DP>(r)) << 4) + 8 * (L & 1);
+      }
+  }
+  const uint32_t lds0 = uniform((uint32_t)(uintptr_t)(lds_void*)lds);
+
+  DenseSource<DP, WAVES> dense;
+  BlockSource<DP, BF, WAVES> blocks(p, t.request, h, nk);
+  float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][4]
+  if (tile_limit > 0) {
+    if constexpr (BLOCKS) {
+      blocks.blocks(0);
+      blocks.issue(0);
+      blocks.blocks(kKeys);
+      blocks.finish(lds, lds + kTileBytes, lscale);
+    } else {
+      dense.init(p, t, h, k0, nk);
+      dense.issue(0, lds0, lds0 + kTileBytes);
+    }
+  }
+  int buf = 0;
+  for (int j = 0; j < tile_limit; j += kKeys) {
+    // this wave's copies are done, then everybody's; and everybody has read the other buffer
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int at = buf * 2 * kTileBytes;
+    const float* ls = lscale + 4 * buf;
+    buf ^= 1;
+    const int next = buf * 2 * kTileBytes;
+    const bool more = j + kKeys < tile_limit;
+    if (more) {
+      if constexpr (BLOCKS) {
+        blocks.issue(j + kKeys);
+        blocks.blocks(j + 2 * kKeys);
+      } else {
+        dense.issue(j + kKeys, lds0 + next, lds0 + next + kTileBytes);
+      }
+    }
+    if (j < wave_max) {
+    const char* lk = lds + at;
+    const char* lv = lds + at + kTileBytes;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t2][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[t2] = mfma32<BF>(*(const u32x4*)(lk + kaddr[ks] + t2 * 32 * kRowBytes), q[ks], s[t2]);
+    }
+    if constexpr (BLOCKS && !BF) {
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t2][i] *= ls[2 * t2 + i / 8];
+    }
+    if (j + kKeys > wave_min) {
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (j + 32 * t2 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[t2][i] = -__builtin_inff();
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+    top = fmaxf(top, other_half(top)) * p.c;
+    if (__any(top > m + 8.f)) {
+      const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+      m = up, l *= f;
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[cb][i] *= f;
+    }
+    constexpr bool kSplit = BLOCKS && !BF;  // p as two bf16 parts: an fp16 result shows one rounding to bf16
+    u32x4 pk[4], rest[kSplit ? 4 : 1];
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[t2][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t2][i], p.c, -m));
+        l += s[t2][i];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t pair = pack2<BF || BLOCKS>(s[t2][2 * i], s[t2][2 * i + 1]);
+        pk[2 * t2 + i / 4][i % 4] = pair;
+        if constexpr (kSplit)
+          rest[2 * t2 + i / 4][i % 4] =
+              pack2<true>(s[t2][2 * i] - u2f(pair << 16), s[t2][2 * i + 1] - u2f(pair & 0xffff0000u));
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        union {
+          short4v part[2];
+          u32x4 whole;
+        } a;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+          a.part[s2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4*)(lds_void*)(lv + vaddr[cb][s2] + ks * 16 * kRowBytes));
+        o[cb] = mfma32<BF || BLOCKS>(a.whole, pk[ks], o[cb]);
+        if constexpr (kSplit) o[cb] = mfma32<true>(a.whole, rest[ks], o[cb]);
+      }
+    }
+    if constexpr (BLOCKS)
+      if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 4 * buf);
+  }
+
+  l += other_half(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (!real) return;
+  char* dst = (char*)p.o + 2 * (qb * p.o_sb + (t.q0 + token) * p.o_st + head * p.o_sh);
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ch = 32 * cb + 8 * i + 4 * half;
+      const u32x2 w = {pack2<BF>(o[cb][4 * i] * inv, o[cb][4 * i + 1] * inv),
+                       pack2<BF>(o[cb][4 * i + 2] * inv, o[cb][4 * i + 3] * inv)};
+      if (ch < p.D) *(u32x2*)(dst + 2 * ch) = w;
+    }
+}
+
+}  // namespace prompt
+}  // namespace dkv

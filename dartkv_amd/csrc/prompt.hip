@@ -1,0 +1,75 @@
+// Attention over whole prompts (dkv_prompt_attention): the host's checks and choice of tile.
+#include "dkv_capi_util.h"
+#include "dkv_prompt_tile.h"
+
+using namespace dkv;
+
+namespace {
+
+template <int DP, bool BF, int WAVES>
+int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
+  constexpr int lds = 4 * prompt::kKeys * 2 * DP;
+  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false>), dim3((unsigned)grid), dim3(64 * WAVES), lds, stream, p);
+  return dkv_check_launch("dkv_prompt_attention");
+}
+
+template <int DP, bool BF>
+int launch_waves(const PromptParams& p, int waves, int64_t grid, hipStream_t stream) {
+  return waves == 8 ? launch<DP, BF, 8>(p, grid, stream) : launch<DP, BF, 4>(p, grid, stream);
+}
+
+template <bool BF>
+int launch_dim(const PromptParams& p, int waves, int64_t grid, hipStream_t stream) {
+  if (p.D <= 64) return launch_waves<64, BF>(p, waves, grid, stream);
+  if (p.D <= 128) return launch_waves<128, BF>(p, waves, grid, stream);
+  return launch<256, BF, 4>(p, grid, stream);  // (eight waves would spill: 128 accumulators, 64 query registers)
+}
+
+}  // namespace
+
+extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream) {
+  DKV_CHECK(args != nullptr, DKV_ERR_INVALID, "dkv_prompt_attention: args is NULL");
+  const dkv_prompt_attention_args& a = *args;
+  DKV_CHECK(a.dtype == kF16 || a.dtype == kBF16, DKV_ERR_DTYPE, "dkv_prompt_attention: tensors must be bf16 or fp16");
+  DKV_CHECK(a.Hkv >= 1 && a.Hq >= a.Hkv && a.Hq % a.Hkv == 0, DKV_ERR_INVALID,
+            "dkv_prompt_attention: query heads must be divisible by KV heads");
+  DKV_CHECK(a.D >= 8 && a.D <= 256 && a.D % 8 == 0, DKV_ERR_INVALID,
+            "dkv_prompt_attention: head_dim must be a multiple of 8 up to 256");
+  DKV_CHECK(a.requests >= 1 && a.requests < (1 << 24) && a.q_tokens >= 0 && a.k_tokens >= 0, DKV_ERR_INVALID,
+            "dkv_prompt_attention: bad counts");
+  DKV_CHECK((a.q_starts == nullptr) == (a.k_starts == nullptr), DKV_ERR_INVALID,
+            "dkv_prompt_attention: query and key starts come together");
+  const int64_t G = a.Hq / a.Hkv;
+  DKV_CHECK(a.q_tokens < (1ll << 31) / G && a.k_tokens < (1ll << 31) - 64, DKV_ERR_INVALID,
+            "dkv_prompt_attention: too many tokens");
+  DKV_CHECK(a.scale > 0 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_prompt_attention: scale must be positive and finite");
+  if (a.q_tokens == 0) return DKV_OK;
+  DKV_CHECK(a.query && a.out && (a.k_tokens == 0 || (a.keys && a.values)), DKV_ERR_INVALID,
+            "dkv_prompt_attention: NULL pointer");
+  DKV_CHECK((((uintptr_t)a.query | (uintptr_t)a.keys | (uintptr_t)a.values |
+              (uintptr_t)(2 * (a.q_sb | a.q_st | a.q_sh | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh))) & 15) ==
+                    0 &&
+                (((uintptr_t)a.out | (uintptr_t)(2 * (a.o_sb | a.o_st | a.o_sh))) & 7) == 0,
+            DKV_ERR_INVALID, "dkv_prompt_attention: rows must be 16-byte aligned (output rows 8-byte)");
+  // offsets within a tile of 64 keys are 31-bit
+  DKV_CHECK(a.k_st >= 0 && a.v_st >= 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23), DKV_ERR_INVALID,
+            "dkv_prompt_attention: token strides of keys and values must be under 2^23 elements");
+  PromptParams p = {};
+  p.q = a.query, p.k = a.keys, p.v = a.values, p.o = a.out;
+  p.q_sb = a.q_sb, p.q_st = a.q_st, p.q_sh = a.q_sh, p.k_sb = a.k_sb, p.k_st = a.k_st, p.k_sh = a.k_sh;
+  p.v_sb = a.v_sb, p.v_st = a.v_st, p.v_sh = a.v_sh, p.o_sb = a.o_sb, p.o_st = a.o_st, p.o_sh = a.o_sh;
+  p.q_starts = a.q_starts, p.k_starts = a.k_starts;
+  p.R = (int32_t)a.requests, p.H = (int32_t)a.Hkv, p.G = (int32_t)G, p.D = (int32_t)a.D;
+  p.q_tokens = a.q_tokens, p.k_tokens = a.k_tokens;
+  p.c = (float)(a.scale * 1.4426950408889634);
+  p.causal = a.causal ? 1 : 0, p.fill = a.fill && a.q_starts ? 1 : 0, p.skip_rows = 0;
+  auto tiles_of = [&](int64_t bm) {
+    if (!a.q_starts) return a.requests * ((a.q_tokens * G + bm - 1) / bm);
+    return (a.q_tokens * G + bm - 1) / bm + a.requests + (p.fill ? 1 : 0);
+  };
+  const int waves = a.D <= 128 && tiles_of(256) * a.Hkv >= 512 ? 8 : 4;
+  const int64_t grid = tiles_of(32 * waves) * a.Hkv;
+  DKV_CHECK(grid < (1ll << 31), DKV_ERR_INVALID, "dkv_prompt_attention: too many tokens");
+  return a.dtype == kBF16 ? launch_dim<true>(p, waves, grid, (hipStream_t)stream)
+                          : launch_dim<false>(p, waves, grid, (hipStream_t)stream);
+}

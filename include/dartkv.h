@@ -52,7 +52,7 @@ extern "C" {
 /* Thread-local description of the last error on this thread. */
 const char* dkv_last_error(void);
 
-/* ABI version (15); bumps when a struct or an entry point below changes. */
+/* ABI version (16); bumps when a struct or an entry point below changes. */
 int dkv_abi_version(void);
 
 /*
@@ -443,6 +443,145 @@ int dkv_decode_attention(const dkv_decode_args* args, void* stream);
  */
 int dkv_decode_attention_noalloc(const dkv_decode_args* args, void* stream);
 int64_t dkv_decode_scratch_bytes(void);
+
+/*
+ * Attention over whole prompts: query [.., Hq, D], keys and values [.., Hkv, D]
+ * in bf16 or fp16, element (b, t, h, d) at base[b * sb + t * st + h * sh + d].
+ * Query head h uses KV head h / (Hq / Hkv); out = softmax(scale q.k) v in fp32
+ * statistics and accumulators, out in the same dtype.
+ *
+ * Without starts: `requests` sequences of q_tokens query and k_tokens key
+ * tokens each (a batch).  With q_starts and k_starts (device int32
+ * [requests + 1], ascending): packed sequences, request r's query tokens at
+ * rows [q_starts[r], q_starts[r + 1]) of q_tokens, its keys likewise; sb is
+ * not used.  Starts outside the tensors are clamped to them.  fill: output rows
+ * behind q_starts[requests] become 0 (0: they are left as they were).
+ *
+ * causal: the last query token sees all nk keys, token i of nq the first
+ * i + 1 + nk - nq.  A row that sees no key is 0.  D a multiple of 8 up to 256;
+ * rows 16-byte aligned (out: 8).  Forward only.
+ *
+ * No counterpart in the reference, whose prefill runs the model's attention
+ * backend (src/dart/integrations/qwen3.py:85-97).
+ */
+typedef struct dkv_prompt_attention_args {
+  const void* query;
+  const void* keys;
+  const void* values;
+  void* out;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh;
+  const int32_t* q_starts;
+  const int32_t* k_starts;
+  int64_t requests, Hq, Hkv, D, q_tokens, k_tokens;
+  int64_t dtype;
+  double scale;
+  int64_t causal, fill;
+} dkv_prompt_attention_args;
+
+int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
+
+/*
+ * A block cache: requests of different lengths whose keys and values lie in
+ * blocks of block_size tokens (16, 32, 64, 128 or 256), found through a table
+ * (no counterpart in the reference, whose sequences all have one length).
+ * Device state, all int32:
+ *   table   [requests][max_blocks]: a request's blocks in order, -1 behind them
+ *   lengths [requests]: tokens of each request
+ *   free    [blocks]: free[0 .. state[0]) is the stack of free blocks
+ *   state   [4]: free blocks, status, the ticket of a running call, 0
+ *
+ * dkv_reserve_blocks gives request r tokens[r] new tokens behind its lengths[r]
+ * and the blocks they need, from the top of the stack in the requests' order.
+ * slots [total] (int64) becomes block * block_size + offset of every new token,
+ * packed in the requests' order, and -1 behind the last; starts [requests + 1]
+ * their first places.  Stack entries that are taken become -1.
+ * dkv_release_blocks drops the last tokens[r] of each request (all of them when
+ * tokens is NULL, or more than it has) and returns the blocks that no token is
+ * left in; it undoes a reserve of the same counts exactly.
+ *
+ * A call that cannot be met changes nothing but the status, where it sets 1
+ * (too few free blocks), 2 (a request needs more than max_blocks), 4 (a
+ * negative count) or 8 (more new tokens than total); a reserve's slots are
+ * then -1 and its starts 0.  Calls on one state run in order: two streams must
+ * not run them at once.  At most 8,190 requests.
+ */
+typedef struct dkv_block_tables_args {
+  int32_t* table;
+  int32_t* lengths;
+  int32_t* free;
+  int32_t* state;
+  const int32_t* tokens;
+  int64_t* slots;
+  int32_t* starts;
+  int64_t total, requests, max_blocks, blocks, block_size;
+} dkv_block_tables_args;
+
+int dkv_reserve_blocks(const dkv_block_tables_args* args, void* stream);
+int dkv_release_blocks(const dkv_block_tables_args* args, void* stream);
+
+/*
+ * New keys and values [tokens][H][D] (bf16, fp16 or fp32; element (t, h, d) at
+ * base[t * st + h * sh + d], rows 16-byte aligned) into the e4m3 blocks
+ * key_codes, value_codes [blocks][H][block_size][D] with one float scale per
+ * block and head, key_scale, value_scale [blocks][H], at `slots` as
+ * dkv_reserve_blocks gives them (each slot once, a block's slots next to each
+ * other and ascending; a slot outside the blocks writes nothing).  The scale is
+ * 2^e with the least e in [-120, 121] that brings the largest magnitude of the
+ * block's tokens so far to at most 448 (-120 for zeros); codes are value /
+ * scale rounded half to even.  A token at offset 0 begins its block anew; when
+ * later tokens raise the scale, the codes before them are rounded to it.
+ * A NaN or an infinity becomes e4m3's NaN, does not count for the scale, and
+ * sets *nonfinite (optional) to 1.  D a multiple of 16 up to 512.
+ */
+typedef struct dkv_append_blocks_args {
+  const void* keys;
+  const void* values;
+  int64_t dtype, k_st, k_sh, v_st, v_sh;
+  const int64_t* slots;
+  int64_t tokens, H, D, blocks, block_size;
+  uint8_t* key_codes;
+  uint8_t* value_codes;
+  float* key_scale;
+  float* value_scale;
+  uint32_t* nonfinite;
+} dkv_append_blocks_args;
+
+int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
+
+/*
+ * Attention of each request's newest tokens over its blocks: query [tokens][Hq][D]
+ * (bf16 or fp16), request r's at rows [starts[r], starts[r + 1]) (starts NULL:
+ * one token each), the last of them at position lengths[r] - 1, so token i of n
+ * sees the first lengths[r] - n + 1 + i keys.  A row that sees no key is 0.
+ * fill: rows behind starts[requests] become 0 (0: they are left as they were).
+ * max_tokens: no request has more new tokens (a request that has more than that
+ * may be left out).  Bytes of blocks behind a request's length are not used; a
+ * table entry outside [0, blocks) makes the rows that see it NaN.  D a multiple
+ * of 16 up to 256.  workspace: dkv_block_attention_workspace_bytes(Hq, Hkv, D,
+ * max(1, min(max_tokens, tokens))) bytes; its contents need not be kept.
+ */
+typedef struct dkv_block_attention_args {
+  const void* query;
+  void* out;
+  int64_t dtype, q_st, q_sh, o_st, o_sh;
+  int64_t tokens;
+  const int32_t* starts;
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t requests, max_blocks, blocks, block_size;
+  const uint8_t* key_codes;
+  const uint8_t* value_codes;
+  const float* key_scale;
+  const float* value_scale;
+  int64_t Hq, Hkv, D;
+  double scale;
+  int64_t max_tokens, fill;
+  void* workspace;
+  int64_t workspace_bytes;
+} dkv_block_attention_args;
+
+int64_t dkv_block_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_tokens);
+int dkv_block_attention(const dkv_block_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }
