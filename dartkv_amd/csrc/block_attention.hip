@@ -113,6 +113,16 @@ __device__ __forceinline__ uint32_t two(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
 }
 
+// LDS traffic of this wave before and after stays in program order.
+__device__ __forceinline__ void lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 1 in each byte of w that is e4m3's NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u; }
+
 template <int DP>
 struct Unit {
   typedef uint32_t dwords __attribute__((ext_vector_type(DP / 64)));
@@ -132,6 +142,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
   const int worker = (int)(wave / p.H);
   if (worker >= bp.workers) return;
   const int most_rows = bp.rows;
+  __shared__ int32_t first_nan[kThreads / 64][DP];
+  int32_t* first = first_nan[threadIdx.x >> 6];
 
   if (p.fill && p.q_starts) {  // rows behind the last request
     int64_t end = p.q_starts[p.R];
@@ -215,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
       my_vs = p.vscale[(int64_t)my_block * p.H + h];
       if (!good) my_ks = __builtin_nanf(""), my_vs = 1.f;  // a row that sees a bad entry is NaN
     };
+    bool nans = false;
     const int klane = i16 * p.D + g * (DP / 4);
     auto load = [&](Unit<DP>& x, int u) {
       const int key = u * kUnit;
@@ -310,6 +323,29 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
         }
       }
       const bool tail = key + kUnit > length;
+      // Where drafted tokens hide keys from each other, 0 * NaN must not reach the rows that do not see a NaN code: such
+      // codes become 0 here, and the first key of each channel that has one is kept; a row sees the keys before its
+      // limit, so it sees one exactly if that key is before it (e4m3 has no infinities).
+      bool any_nan = false;
+      if (n > 1 && key + kUnit > min_limit) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int c = 0; c < KC; ++c) any_nan |= nan_bytes(x.v[j][c]) != 0;
+        any_nan = __any(any_nan);
+        if (any_nan) {
+          if (!nans)
+            for (int c = lane; c < DP; c += 64) first[c] = 0x7fffffff;
+          nans = true;
+          lds_order();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+              for (uint32_t is = nan_bytes(x.v[j][c]); is; is &= is - 1)
+                atomicMin(&first[i16 * NB + 4 * c + (__builtin_ctz(is) >> 3)], key + 16 * (j / 4) + 4 * g + j % 4);
+        }
+      }
       u32x4 vf[NB];
 #pragma unroll
       for (int c = 0; c < KC; ++c)
@@ -321,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
             a = tok < length ? a : 0u;
             b = tok + 1 < length ? b : 0u;
           }
+          if (any_nan) a &= ~(nan_bytes(a) * 0xffu), b &= ~(nan_bytes(b) * 0xffu);
           const uint32_t a0 = two<true, false>(a), a1 = two<true, true>(a);
           const uint32_t b0 = two<true, false>(b), b1 = two<true, true>(b);
           vf[4 * c][j / 2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
@@ -349,6 +386,19 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
         if (u + 2 < u1) load(even, u + 2);
         compute(odd, u + 1);
       }
+    }
+
+    if (nans) {
+      lds_order();
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = first[(4 * g + e) * NB + b];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (key < limit[t]) o[t][b][e] = __builtin_nanf("");
+        }
     }
 
     // lane (row, g) has channels (4 g + e) * NB + b of its row

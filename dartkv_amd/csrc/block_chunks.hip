@@ -9,10 +9,9 @@ namespace {
 
 template <int DP, bool BF, int WAVES>
 void launch(const PromptParams& p, int64_t rows_bound, hipStream_t stream) {
-  constexpr int lds = 4 * prompt::kKeys * 2 * DP + 32;
   const int64_t tiles = (rows_bound + 32 * WAVES - 1) / (32 * WAVES) + p.R;
-  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, true>), dim3((unsigned)(tiles * p.H)), dim3(64 * WAVES), lds,
-                     stream, p);
+  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, true>), dim3((unsigned)(tiles * p.H)), dim3(64 * WAVES),
+                     prompt::lds_bytes(DP, !BF), stream, p);
 }
 
 template <bool BF>

@@ -60,7 +60,11 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kKeys = 64;  // keys of a tile
+// Keys of a tile: 64; 32 where the accumulators (head_dims over 128) or the split weights (fp16 queries over blocks)
+// leave no registers for more.
+constexpr int keys_of(int DP, bool split) { return DP <= (split ? 64 : 128) ? 64 : 32; }
+// LDS of a workgroup: two buffers of keys and values, the blocks' scales, the careful pass's first keys.
+constexpr int lds_bytes(int DP, bool split) { return 4 * keys_of(DP, split) * 2 * DP + 32 + 8 * DP; }
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -165,9 +169,30 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
   return t;
 }
 
+// A product adds 0 * v for a key that its row does not see, which is NaN where v is an infinity or a NaN.  Where a
+// tile's result is not finite, it is computed again with such values set to 0 in LDS, and what they do is added at
+// the end: a row sees the keys before its limit, so it sees one exactly if the channel's first one is before it.
+// first[ch] is the first key with an infinity or NaN, first[DP + ch] with a negative infinity or NaN.
+template <int DP, int KEYS, bool BF, int THREADS>
+__device__ __forceinline__ void set_apart(char* lv, int j, int32_t* first) {
+  constexpr uint32_t kExp = BF ? 0x7f80u : 0x7c00u;
+  for (int at = threadIdx.x; at < KEYS * DP; at += THREADS) {
+    const int row = at / DP, ch = at % DP;
+    uint16_t* place = (uint16_t*)(lv + row * 2 * DP + (((ch >> 3) ^ swizzle<DP>(row)) << 4)) + (ch & 7);
+    const uint32_t x = *place;
+    if ((x & kExp) == kExp) {
+      const bool nan = (x & 0x7fffu) > kExp;
+      if (nan || !(x & 0x8000u)) atomicMin(&first[ch], j + row);
+      if (nan || (x & 0x8000u)) atomicMin(&first[DP + ch], j + row);
+      *place = 0;
+    }
+  }
+}
+
 // Copies of 16-bit keys and values: straight from memory to LDS.
 template <int DP, int WAVES>
 struct DenseSource {
+  static constexpr int kKeys = keys_of(DP, false);
   const char *k, *v;
   int64_t kst, vst;  // bytes
   int nk, valid;     // valid: bytes of a row
@@ -208,7 +233,7 @@ struct DenseSource {
 // leave fp16's range), whose scale goes to the logits, and values as scaled bf16.
 template <int DP, bool BF, int WAVES>
 struct BlockSource {
-  static constexpr int kChunks = 4 * DP / (64 * WAVES);  // 16 codes each, of a thread
+  static constexpr int kChunks = keys_of(DP, !BF) * DP / 16 / (64 * WAVES);  // 16 codes each, of a thread
   static constexpr int kRowBytes = 2 * DP;
   const PromptParams& p;
   const int32_t* table;
@@ -279,8 +304,8 @@ struct BlockSource {
 };
 
 template <int DP, bool BF, int WAVES, bool BLOCKS>
-__global__ void __launch_bounds__(64 * WAVES) prompt_tiles(PromptParams p) {
-  constexpr int BM = 32 * WAVES, KS = DP / 16, CB = DP / 32;
+__global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(PromptParams p) {
+  constexpr int BM = 32 * WAVES, KS = DP / 16, CB = DP / 32, kKeys = keys_of(DP, BLOCKS && !BF), T2 = kKeys / 32;
   constexpr int kRowBytes = 2 * DP, kTileBytes = kKeys * kRowBytes;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
@@ -334,11 +359,7 @@ __global__ void __launch_bounds__(64 * WAVES) prompt_tiles(PromptParams p) {
   }
 
   f32x16 o[CB];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[cb][i] = 0.f;
-  float m = -3.402823466e38f, l = 0.f;
+  float m, l;
 
   // LDS bytes of this lane's operand chunks within a tile
   int kaddr[KS], vaddr[CB][2];
@@ -361,110 +382,145 @@ __global__ void __launch_bounds__(64 * WAVES) prompt_tiles(PromptParams p) {
   DenseSource<DP, WAVES> dense;
   BlockSource<DP, BF, WAVES> blocks(p, t.request, h, nk);
   float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][4]
-  if (tile_limit > 0) {
-    if constexpr (BLOCKS) {
-      blocks.blocks(0);
-      blocks.issue(0);
-      blocks.blocks(kKeys);
-      blocks.finish(lds, lds + kTileBytes, lscale);
-    } else {
-      dense.init(p, t, h, k0, nk);
-      dense.issue(0, lds0, lds0 + kTileBytes);
-    }
-  }
-  int buf = 0;
-  for (int j = 0; j < tile_limit; j += kKeys) {
-    // this wave's copies are done, then everybody's; and everybody has read the other buffer
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int at = buf * 2 * kTileBytes;
-    const float* ls = lscale + 4 * buf;
-    buf ^= 1;
-    const int next = buf * 2 * kTileBytes;
-    const bool more = j + kKeys < tile_limit;
-    if (more) {
+  if constexpr (!BLOCKS) dense.init(p, t, h, k0, nk);
+  int32_t* first = (int32_t*)(lds + 4 * kTileBytes + 32);  // [2][DP], of the careful pass
+  bool careful = false;  // (the same for the whole workgroup)
+  for (;;) {
+    m = -3.402823466e38f, l = 0.f;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[cb][i] = 0.f;
+    if (tile_limit > 0) {
       if constexpr (BLOCKS) {
-        blocks.issue(j + kKeys);
-        blocks.blocks(j + 2 * kKeys);
+        blocks.blocks(0);
+        blocks.issue(0);
+        blocks.blocks(kKeys);
+        blocks.finish(lds, lds + kTileBytes, lscale);
       } else {
-        dense.issue(j + kKeys, lds0 + next, lds0 + next + kTileBytes);
+        dense.issue(0, lds0, lds0 + kTileBytes);
       }
     }
-    if (j < wave_max) {
-    const char* lk = lds + at;
-    const char* lv = lds + at + kTileBytes;
+    int buf = 0;
+    for (int j = 0; j < tile_limit; j += kKeys) {
+      // this wave's copies are done, then everybody's; and everybody has read the other buffer
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const int at = buf * 2 * kTileBytes;
+      const float* ls = lscale + 4 * buf;
+      buf ^= 1;
+      const int next = buf * 2 * kTileBytes;
+      const bool more = j + kKeys < tile_limit;
+      if (more) {
+        if constexpr (BLOCKS) {
+          blocks.issue(j + kKeys);
+          blocks.blocks(j + 2 * kKeys);
+        } else {
+          dense.issue(j + kKeys, lds0 + next, lds0 + next + kTileBytes);
+        }
+      }
+      if (careful) {
+        set_apart<DP, kKeys, BF || BLOCKS, 64 * WAVES>(lds + at + kTileBytes, j, first);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      if (j < wave_max) {
+      const char* lk = lds + at;
+      const char* lv = lds + at + kTileBytes;
 
-    f32x16 s[2];
+      f32x16 s[T2];
 #pragma unroll
-    for (int t2 = 0; t2 < 2; ++t2) {
+      for (int t2 = 0; t2 < T2; ++t2) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[t2][i] = 0.f;
+        for (int i = 0; i < 16; ++i) s[t2][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        s[t2] = mfma32<BF>(*(const u32x4*)(lk + kaddr[ks] + t2 * 32 * kRowBytes), q[ks], s[t2]);
+        for (int ks = 0; ks < KS; ++ks)
+          s[t2] = mfma32<BF>(*(const u32x4*)(lk + kaddr[ks] + t2 * 32 * kRowBytes), q[ks], s[t2]);
+      }
+      if constexpr (BLOCKS && !BF) {
+#pragma unroll
+        for (int t2 = 0; t2 < T2; ++t2)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[t2][i] *= ls[2 * t2 + i / 8];
+      }
+      if (j + kKeys > wave_min) {
+#pragma unroll
+        for (int t2 = 0; t2 < T2; ++t2)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (j + 32 * t2 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[t2][i] = -__builtin_inff();
+      }
+      float top = s[0][0];  // of this lane's half of the row's keys
+#pragma unroll
+      for (int t2 = 0; t2 < T2; ++t2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t2][i]);
+      top *= p.c;
+      if (__any(top > m + 8.f)) {
+        top = fmaxf(top, other_half(top));
+        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
+        m = up, l *= f;
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[cb][i] *= f;
+      }
+      constexpr bool kSplit = BLOCKS && !BF;  // p as two bf16 parts: an fp16 result shows one rounding to bf16
+      u32x4 pk[2 * T2], rest[kSplit ? 2 * T2 : 1];
+#pragma unroll
+      for (int t2 = 0; t2 < T2; ++t2) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[t2][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t2][i], p.c, -m));
+          l += s[t2][i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t pair = pack2<BF || BLOCKS>(s[t2][2 * i], s[t2][2 * i + 1]);
+          pk[2 * t2 + i / 4][i % 4] = pair;
+          if constexpr (kSplit)
+            rest[2 * t2 + i / 4][i % 4] =
+                pack2<true>(s[t2][2 * i] - u2f(pair << 16), s[t2][2 * i + 1] - u2f(pair & 0xffff0000u));
+        }
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2 * T2; ++ks)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          union {
+            short4v part[2];
+            u32x4 whole;
+          } a;
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2)
+            a.part[s2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_short4*)(lds_void*)(lv + vaddr[cb][s2] + ks * 16 * kRowBytes));
+          o[cb] = mfma32<BF || BLOCKS>(a.whole, pk[ks], o[cb]);
+          if constexpr (kSplit) o[cb] = mfma32<true>(a.whole, rest[ks], o[cb]);
+        }
+      }
+      if constexpr (BLOCKS)
+        if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 4 * buf);
     }
-    if constexpr (BLOCKS && !BF) {
+    if (careful || !p.causal) break;
+    float zero = 0.f;
 #pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2)
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t2][i] *= ls[2 * t2 + i / 8];
-    }
-    if (j + kKeys > wave_min) {
+      for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[cb][i], 0.f, zero);
+    if (!__syncthreads_or(real && zero != 0.f)) break;  // (NaN is not 0)
+    careful = true;
+    for (int i = threadIdx.x; i < 2 * DP; i += 64 * WAVES) first[i] = 0x7fffffff;
+  }
+
+  if (careful) {
 #pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (j + 32 * t2 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[t2][i] = -__builtin_inff();
-    }
-    float top = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-    top = fmaxf(top, other_half(top)) * p.c;
-    if (__any(top > m + 8.f)) {
-      const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
-      m = up, l *= f;
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[cb][i] *= f;
-    }
-    constexpr bool kSplit = BLOCKS && !BF;  // p as two bf16 parts: an fp16 result shows one rounding to bf16
-    u32x4 pk[4], rest[kSplit ? 4 : 1];
-#pragma unroll
-    for (int t2 = 0; t2 < 2; ++t2) {
+    for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[t2][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t2][i], p.c, -m));
-        l += s[t2][i];
+        const int ch = 32 * cb + 8 * (i / 4) + 4 * half + i % 4;
+        if (first[ch] < limit) o[cb][i] += __builtin_inff();
+        if (first[DP + ch] < limit) o[cb][i] -= __builtin_inff();
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t pair = pack2<BF || BLOCKS>(s[t2][2 * i], s[t2][2 * i + 1]);
-        pk[2 * t2 + i / 4][i % 4] = pair;
-        if constexpr (kSplit)
-          rest[2 * t2 + i / 4][i % 4] =
-              pack2<true>(s[t2][2 * i] - u2f(pair << 16), s[t2][2 * i + 1] - u2f(pair & 0xffff0000u));
-      }
-    }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        union {
-          short4v part[2];
-          u32x4 whole;
-        } a;
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-          a.part[s2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_short4*)(lds_void*)(lv + vaddr[cb][s2] + ks * 16 * kRowBytes));
-        o[cb] = mfma32<BF || BLOCKS>(a.whole, pk[ks], o[cb]);
-        if constexpr (kSplit) o[cb] = mfma32<true>(a.whole, rest[ks], o[cb]);
-      }
-    }
-    if constexpr (BLOCKS)
-      if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 4 * buf);
   }
-
   l += other_half(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   if (!real) return;

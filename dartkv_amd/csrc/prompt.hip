@@ -8,8 +8,7 @@ namespace {
 
 template <int DP, bool BF, int WAVES>
 int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
-  constexpr int lds = 4 * prompt::kKeys * 2 * DP;
-  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false>), dim3((unsigned)grid), dim3(64 * WAVES), lds, stream, p);
+  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false>), dim3((unsigned)grid), dim3(64 * WAVES), prompt::lds_bytes(DP, false), stream, p);
   return dkv_check_launch("dkv_prompt_attention");
 }
 

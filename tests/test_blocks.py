@@ -376,6 +376,33 @@ def test_a_few_tokens(dtype, D, G, new, limit):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,G,new", [(64, 4, 4), (128, 4, 8), (128, 1, 3), (256, 4, 4), (64, 4, 150), (128, 8, 60)])
+def test_nan_codes_reach_only_the_rows_that_see_them(dtype, D, G, new):
+    import dartkv_amd as dart
+    lengths, H = [new, 100 + new, 37 + new], 2
+    cache = _cache(lengths, H, D, 32, D)
+    q = _query(3 * new, H * G, D, dtype, 9)
+    starts = _starts([new] * 3)
+    want = dart.block_attention(q, *cache, starts, max_tokens=new)
+    raw = [c.view(torch.uint8) for c in cache[:2]]
+    bad = [new // 2, new - 1, 0]  # of each request's new tokens, the one with a NaN value (channel 3 + r of head 1)
+    for r, i in enumerate(bad):
+        t = lengths[r] - new + i
+        raw[1][int(cache[4][r, t // 32]), 1, t % 32, 3 + r] = 0xff
+    t = lengths[1] - 2
+    raw[0][int(cache[4][1, t // 32]), 0, t % 32, 5] = 0x7f  # and a NaN key of head 0
+    got = dart.block_attention(q, *cache, starts, max_tokens=new).view(3, new, H, G, D)
+    want = want.view(3, new, H, G, D)
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    for r, i in enumerate(bad):
+        hit[r, i:, 1, :, 3 + r] = True
+    hit[1, new - 2:, 0] = True
+    assert torch.equal(torch.isnan(got).cpu(), hit)
+    assert torch.equal(got[~hit.to(DEV)], want[~hit.to(DEV)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D", [64, 80, 128, 256])
 @pytest.mark.parametrize("bs", [16, 64])
 def test_chunks_beside_single_tokens(dtype, D, bs):

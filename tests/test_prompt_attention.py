@@ -149,6 +149,32 @@ def test_large_and_small_logits(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,lengths", [(64, [70, 5, 200]), (128, [300, 1]), (256, [100, 40])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_that_a_row_does_not_see_do_not_reach_it(dtype, D, lengths, causal):
+    """Infinities and NaN among keys and values: rows before them are as without them, rows behind them show them."""
+    import dartkv_amd as dart
+    n = sum(lengths)
+    q, k, v = (_rand((n, h, D), dtype, D + h) for h in (4, 2, 2))
+    inf = float("inf")
+    for t, h, ch, x in ((3, 0, 1, inf), (3, 1, 2, -inf), (66, 0, 5, float("nan")), (69, 1, 7, inf), (69, 1, 7, inf),
+                        (n - 2, 0, D - 1, -inf), (n - 1, 0, D - 1, inf), (n - 1, 1, 0, float("nan"))):
+        v[t, h, ch] = x
+    k[n - 3, 1, 4] = float("nan")
+    got = dart.prompt_attention(q, k, v, _starts(lengths), causal=causal).double().cpu()
+    at = 0
+    for m in lengths:
+        part = slice(at, at + m)
+        o, w = _reference(q[part], k[part], v[part], causal, 1 / math.sqrt(D))
+        fine = torch.isfinite(o)
+        assert torch.equal(torch.isnan(got[part]), torch.isnan(o))
+        assert torch.equal(got[part][~fine & ~torch.isnan(o)], o[~fine & ~torch.isnan(o)])
+        _check(got[part][fine], o[fine], w[fine], dtype)
+        at += m
+
+
+@pytest.mark.gpu
 def test_long_sequence_against_64_bits():
     """Many tiles with eight waves a workgroup: rows of the beginning, the middle and the end."""
     import dartkv_amd as dart
