@@ -163,7 +163,7 @@ def append_blocks(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor,
         raise TypeError("nonfinite must be an int32 tensor of one element on the same device")
     if T == 0:
         return
-    keys, values, slots = aligned_rows(keys.detach()), aligned_rows(values.detach()), slots.contiguous()
+    keys, values, slots = aligned_rows(keys.detach(), 0), aligned_rows(values.detach(), 0), slots.contiguous()
     a = _lib.AppendBlocksArgs()
     a.keys, a.values, a.slots = keys.data_ptr(), values.data_ptr(), slots.data_ptr()
     a.dtype = _lib.dtype_code(keys.dtype)
@@ -239,7 +239,7 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
         raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
     if T == 0:
         return out
-    query = aligned_rows(query)
+    query = aligned_rows(query, 0)
     lib = _lib.load()
     a = _lib.BlockAttentionArgs()
     a.query, a.out, a.dtype = query.data_ptr(), out.data_ptr(), _lib.dtype_code(query.dtype)

@@ -8,8 +8,10 @@
 // size or one step of the block's smallest.  With scales that are not powers of two every growth would round all
 // codes again.
 //
-// One wave has one run (the tokens of a call that lie in one block, next to each other) of one KV head's keys or
-// values: it finds the run from the slots alone.
+// One wave has one run (the tokens of a call that follow each other in one block) of one KV head's keys or values: it
+// finds the runs that begin among its 64 tokens (one, where there are few) from the slots alone.  A block's rows are
+// read once, all at once (64 registers for 64 rows of 128 in 16 bits), and stay there until the scale is known.
+// Bound: memory, 3 bytes an element from 16 bits.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -36,27 +38,6 @@ struct AppendParams {
   int32_t H, D, shift, span, dtype;
 };
 
-// Eight elements at `at` (element index, a multiple of 8 elements from an aligned base).
-template <int SRC>
-__device__ __forceinline__ void load8(const void* src, int64_t at, float (&x)[8]) {
-  if constexpr (SRC == kF32) {
-    const float4 a = *(const float4*)((const float*)src + at), b = *(const float4*)((const float*)src + at + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 w = *(const uint4*)((const uint16_t*)src + at);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (SRC == kBF16) {
-        x[2 * i] = u2f(u[i] << 16), x[2 * i + 1] = u2f(u[i] & 0xffff0000u);
-      } else {
-        x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)u[i]);
-        x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[i] >> 16));
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ int exponent_for(float amax) {
   int k;
   const float f = frexpf(amax, &k);  // amax = f 2^k, f in [1/2, 1); 448 = 7/8 2^9
@@ -78,6 +59,72 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
   return make_uint2(w[0], w[1]);
 }
 
+// Rows of a run that stay in registers between the scale and the codes: all 64 of a block for head_dim 128 in 16 bits.
+template <int SRC>
+constexpr int kHeld = SRC == kF32 ? 8 : 16;  // passes of 64 / (D / 8) rows
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+
+template <int SRC>
+struct Raw {  // eight elements as they are
+  static constexpr int kWords = SRC == kF32 ? 2 : 1;
+  u32x4 w[kWords];
+  __device__ __forceinline__ void load(const char* at) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = ((const u32x4*)at)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = (u32x4){0, 0, 0, 0};
+  }
+  // `top`: the largest magnitude's bits so far (magnitudes order as their bits do, infinities and NaN above all; two
+  // maxima of 16 bits each).
+  __device__ __forceinline__ void largest(uint32_t& top) const {
+#pragma unroll
+    for (int i = 0; i < 4 * kWords; ++i) {
+      const uint32_t u = w[i / 4][i % 4];
+      if constexpr (SRC == kF32) {
+        top = (u & 0x7fffffffu) > top ? u & 0x7fffffffu : top;
+      } else {
+        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, top),
+                                                                     __builtin_bit_cast(ushort2v, u & 0x7fff7fffu)));
+      }
+    }
+  }
+  // The registers hold something unknown from here: what was made of them is not kept.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    if constexpr (SRC == kF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = u2f(w[i / 4][i % 4]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = w[0][i];
+        if constexpr (SRC == kBF16) {
+          x[2 * i] = u2f(u << 16), x[2 * i + 1] = u2f(u & 0xffff0000u);
+        } else {
+          x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+          x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+        }
+      }
+    }
+  }
+};
+
+// The magnitude that `largest` found.
+template <int SRC>
+__device__ __forceinline__ float magnitude(uint32_t top) {
+  if constexpr (SRC == kF32) return u2f(top);
+  const uint32_t u = (top & 0xffffu) > (top >> 16) ? top & 0xffffu : top >> 16;
+  if constexpr (SRC == kBF16) return u2f(u << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+}
+
 template <int SRC>
 __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
   const int lane = threadIdx.x & 63;
@@ -86,59 +133,93 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
   const int64_t first = unit / kinds * p.span;
   if (first >= p.T) return;
   const int kind = (int)(unit % kinds), which = kind & 1, h = kind >> 1;
-  const int64_t stop = first + p.span < p.T ? first + p.span : p.T;
   const int bs = 1 << p.shift;
   const int lpr = p.D >> 3, rpp = 64 / lpr;  // lanes of a row, rows of a pass
   const int my_row = lane / lpr, my_ch = (lane % lpr) * 8;
   const bool active = my_row < rpp;
+  const void* src = p.src[which];
+  constexpr int kSize = SRC == kF32 ? 4 : 2;
+  const uint32_t my_at = (uint32_t)((my_row * p.st[which] + my_ch) * kSize), my_code = my_row * p.D + my_ch;
 
-  for (int64_t t = first; t < stop; ++t) {
-    const int64_t slot = p.slots[t];
-    if (slot < 0 || (slot >> p.shift) >= p.blocks) continue;
-    const int64_t block = slot >> p.shift;
-    if (t > 0 && p.slots[t - 1] >= 0 && (p.slots[t - 1] >> p.shift) == block) continue;  // inside a run
-    int n = 0;  // tokens of the run
-    while (n < bs) {
+  // the runs that begin among this wave's tokens
+  const int64_t mine = first + lane;
+  const int64_t slot = mine < p.T ? p.slots[mine] : -1, prev = mine > 0 && mine < p.T ? p.slots[mine - 1] : -1;
+  const bool in = slot >= 0 && (slot >> p.shift) < p.blocks;
+  const bool goes_on = prev >= 0 && prev + 1 == slot && (slot & (bs - 1)) != 0;
+  uint64_t runs = __ballot(lane < p.span && in && !goes_on);
+
+  while (runs) {
+    const int l = __builtin_ctzll(runs);
+    runs &= runs - 1;
+    const int64_t t = first + l;
+    const int64_t begin = ((int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(slot >> 32), l) << 32) |
+                          (uint32_t)__builtin_amdgcn_readlane((int)slot, l);
+    const int64_t block = begin >> p.shift;
+    const int held = (int)(begin & (bs - 1));
+    const int most = bs - held;  // tokens of the run, found from the slots that follow each other
+    int n = 1;
+    while (n < most) {
       const int64_t at = t + n + lane;
-      const bool same = n + lane < bs && at < p.T && p.slots[at] >= 0 && (p.slots[at] >> p.shift) == block;
-      const uint64_t mask = ~__ballot(same);
-      const int more = mask ? __builtin_ctzll(mask) : 64;
+      const bool same = n + lane < most && at < p.T && p.slots[at] == begin + n + lane;
+      const uint64_t others = ~__ballot(same);
+      const int more = others ? __builtin_ctzll(others) : 64;
       n += more;
       if (more < 64) break;
     }
-    const int held = (int)(slot & (bs - 1));
-    const void* src = p.src[which];
-    const int64_t base = t * p.st[which] + h * p.sh[which] + my_ch;
-    float amax = 0.f;
-    bool bad = false;
-    for (int row = 0; row < n; row += rpp) {
+    // rows of a pass: a wave-uniform address and this lane's offset
+    const char* base = (const char*)src + (t * p.st[which] + h * p.sh[which]) * kSize;
+    const int64_t pass = rpp * p.st[which] * kSize;
+    float* scale = p.scale[which] + block * p.H + h;
+    const float before = held > 0 ? *scale : 0.f;
+    Raw<SRC> raw[kHeld<SRC>];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kHeld<SRC>; ++i) {
+      const int r = i * rpp + my_row;
+      raw[i].zero();
+      if (active && r < n) raw[i].load(base + i * pass + my_at);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld<SRC>; ++i) {
+      raw[i].largest(top);
+      raw[i].forget();
+    }
+    for (int row = kHeld<SRC> * rpp; row < n; row += rpp) {
       const int r = row + my_row;
       if (active && r < n) {
-        float x[8];
-        load8<SRC>(src, base + r * p.st[which], x);
+        Raw<SRC> more;
+        more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+        more.largest(top);
+      }
+    }
+    float amax = magnitude<SRC>(top);
+    if (__any(!(amax < __builtin_inff()))) {  // the largest of the finite ones
+      amax = 0.f;
+      if (p.nonfinite && lane == 0) *p.nonfinite = 1;
+#pragma unroll 1
+      for (int row = 0; row < n; row += rpp) {
+        const int r = row + my_row;
+        if (active && r < n) {
+          float x[8];
+          Raw<SRC> again;
+          again.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+          again.get(x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = fabsf(x[i]);
-          if (a < __builtin_inff())
-            amax = fmaxf(amax, a);
-          else
-            bad = true;
+          for (int i = 0; i < 8; ++i)
+            if (fabsf(x[i]) < __builtin_inff()) amax = fmaxf(amax, fabsf(x[i]));
         }
       }
     }
     amax = wave_max(amax);
-    if (p.nonfinite && __any(bad) && lane == 0) *p.nonfinite = 1;
-    float* scale = p.scale[which] + block * p.H + h;
-    const float before = *scale;
     float now = pow2(amax > 0.f ? exponent_for(amax) : kMinExponent);
     if (held > 0) now = fmaxf(now, before);
-    uint8_t* codes = p.codes[which] + (block * p.H + h) * (int64_t)bs * p.D + my_ch;
+    uint8_t* codes = p.codes[which] + (block * p.H + h) * (int64_t)bs * p.D;
     if (held > 0 && now != before) {  // the block's earlier codes at the new scale
       const float f = before / now;
       for (int row = 0; row < held; row += rpp) {
         const int r = row + my_row;
         if (active && r < held) {
-          uint2* at = (uint2*)(codes + (int64_t)r * p.D);
+          uint2* at = (uint2*)(codes + row * p.D + my_code);
           const uint2 w = *at;
           const uint32_t u[2] = {w.x, w.y};
           float x[8];
@@ -153,13 +234,22 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
       }
     }
     const float inv = 1.f / now;
-    for (int row = 0; row < n; row += rpp) {
+    codes += (int64_t)held * p.D;
+#pragma unroll
+    for (int i = 0; i < kHeld<SRC>; ++i) {
+      const int r = i * rpp + my_row;
+      float x[8];
+      raw[i].get(x);
+      if (active && r < n) *(uint2*)(codes + i * rpp * p.D + my_code) = codes8(x, inv);
+    }
+    for (int row = kHeld<SRC> * rpp; row < n; row += rpp) {
       const int r = row + my_row;
       if (active && r < n) {
         float x[8];
-        load8<SRC>(src, base + r * p.st[which], x);
-        const int at = (int)(p.slots[t + r] & (bs - 1));
-        *(uint2*)(codes + (int64_t)at * p.D) = codes8(x, inv);
+        Raw<SRC> more;
+        more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+        more.get(x);
+        *(uint2*)(codes + row * p.D + my_code) = codes8(x, inv);
       }
     }
     if (lane == 0 && (held == 0 || now != before)) *scale = now;
@@ -186,6 +276,8 @@ extern "C" int dkv_append_blocks(const dkv_append_blocks_args* args, void* strea
               (uintptr_t)(a.v_st * esize) | (uintptr_t)(a.v_sh * esize) | (uintptr_t)a.key_codes |
               (uintptr_t)a.value_codes) & 15) == 0,
             DKV_ERR_INVALID, "dkv_append_blocks: rows must be 16-byte aligned");
+  DKV_CHECK(a.k_st >= 0 && a.v_st >= 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23), DKV_ERR_INVALID,
+            "dkv_append_blocks: token strides must be under 2^23 elements");
   AppendParams p = {{a.keys, a.values}, {a.k_st, a.v_st}, {a.k_sh, a.v_sh}, {a.key_codes, a.value_codes},
                     {a.key_scale, a.value_scale}, a.slots, a.nonfinite, a.tokens, a.blocks,
                     (int32_t)a.H, (int32_t)a.D, __builtin_ctzll((uint64_t)a.block_size), 1, (int32_t)a.dtype};

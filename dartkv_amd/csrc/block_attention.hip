@@ -36,7 +36,7 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 32;       // keys of a unit of work
-constexpr int kMinShare = 4;    // units of a wave at least
+constexpr int kMinShare = 2;    // units of a wave at least
 constexpr int kThreads = 256;
 
 struct BlockParams {
@@ -69,6 +69,10 @@ __device__ __forceinline__ Work work_of(const PromptParams& p, int r, int most_r
   return w;
 }
 
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  return (int64_t)(((uint64_t)uniform((uint32_t)(x >> 32)) << 32) | uniform((uint32_t)x));
+}
+
 __device__ __forceinline__ int wave_scan(int x, int lane) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -76,17 +80,6 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
     if (lane >= off) x += up;
   }
   return x;
-}
-
-__device__ __forceinline__ int64_t total_units(const PromptParams& p, int most_rows, int lane) {
-  int64_t total = 0;
-  for (int base = 0; base < p.R; base += 64) {
-    int x = work_of(p, base + lane, most_rows).units;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-    total += x;
-  }
-  return total;
 }
 
 __device__ __forceinline__ int64_t share_of(int64_t total, int workers) {
@@ -132,7 +125,7 @@ struct Unit {
 };
 
 template <int DP, bool BF, int NT>
-__global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_decode(BlockParams bp) {
+__global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(BlockParams bp) {
   const PromptParams& p = bp.a;
   constexpr int KC = DP / 64;  // 16-byte pieces of a lane's key, dwords of a lane's value
   constexpr int KS = DP / 32, NB = DP / 16;
@@ -153,26 +146,32 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
         ((uint16_t*)p.o)[t * p.o_st + (h * p.G + c / p.D) * p.o_sh + c % p.D] = 0;
   }
 
-  const int64_t total = total_units(p, most_rows, lane);
+  // all units, then the request that this wave's first lies in
+  Work mine = work_of(p, lane, most_rows);
+  int scan = wave_scan(mine.units, lane);
+  int64_t total = uniform(__shfl(scan, 63, 64));
+  for (int b = 64; b < p.R; b += 64) {
+    int x = work_of(p, b + lane, most_rows).units;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    total += uniform(x);
+  }
   const int64_t share = share_of(total, bp.workers);
   int64_t unit = worker * share;
   const int64_t stop = unit + share < total ? unit + share : total;
   if (unit >= stop) return;
-
-  // the request that `unit` lies in
   int base = 0, lane_r = 0;
   int64_t before = 0;  // units before request `base`
-  Work mine;
-  int scan = 0;
-  for (;; base += 64) {
-    mine = work_of(p, base + lane, most_rows);
-    scan = wave_scan(mine.units, lane);
+  for (;;) {
     const uint64_t hit = __ballot(before + scan > unit);
     if (hit) {
       lane_r = __builtin_ctzll(hit);
       break;
     }
-    before += __shfl(scan, 63, 64);
+    before += uniform(__shfl(scan, 63, 64));
+    base += 64;
+    mine = work_of(p, base + lane, most_rows);
+    scan = wave_scan(mine.units, lane);
   }
 
   while (unit < stop) {
@@ -228,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
       if (!good) my_ks = __builtin_nanf(""), my_vs = 1.f;  // a row that sees a bad entry is NaN
     };
     bool nans = false;
-    const int klane = i16 * p.D + g * (DP / 4);
+    const uint32_t klane = i16 * p.D + g * (DP / 4), vlane = 4 * g * p.D + i16 * NB;
     auto load = [&](Unit<DP>& x, int u) {
       const int key = u * kUnit;
       const int last_block = (key + 16) >> p.bs_shift;
@@ -246,13 +245,13 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
           const bool in = g * (DP / 4) + c * 16 < p.D;
-          x.k[s][c] = *(const u32x4*)(kp + (in ? klane + c * 16 : 0));
+          x.k[s][c] = *(const u32x4*)(kp + (in ? klane + c * 16 : 0u));
           if (!in) x.k[s][c] = (u32x4){0, 0, 0, 0};
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bool in = i16 * NB < p.D;
-          x.v[4 * s + j] = *(const typename Unit<DP>::dwords*)(vp + (in ? (4 * g + j) * p.D + i16 * NB : 0));
+          x.v[4 * s + j] = *(const typename Unit<DP>::dwords*)(vp + j * p.D + (in ? vlane : 0u));
           if (!in)
 #pragma unroll
             for (int c = 0; c < KC; ++c) x.v[4 * s + j][c] = 0;
@@ -261,28 +260,32 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
     };
     auto compute = [&](const Unit<DP>& x, int u) {
       const int key = u * kUnit;
-      u32x4 kf[2][KS];
+      f32x4 scores[NT][2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        u32x4 kf[KS];
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
           const uint32_t a = x.k[s][c / 2][2 * (c % 2)], b = x.k[s][c / 2][2 * (c % 2) + 1];
-          kf[s][c] = (u32x4){two<BF, false>(a), two<BF, true>(a), two<BF, false>(b), two<BF, true>(b)};
+          kf[c] = (u32x4){two<BF, false>(a), two<BF, true>(a), two<BF, false>(b), two<BF, true>(b)};
         }
+        const float f = p.c * x.ks[s];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (NT > 1 && t >= nt) break;
+          f32x4 sc = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KS; ++c) sc = mfma16<BF>(kf[c], q[t][c], sc);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) scores[t][s][e] = sc[e] * f;
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (one half's operands in registers at a time)
+      }
       u32x4 hi[NT], lo[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (NT > 1 && t >= nt) break;
-        f32x4 sc[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          sc[s] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < KS; ++c) sc[s] = mfma16<BF>(kf[s][c], q[t][c], sc[s]);
-          const float f = p.c * x.ks[s];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[s][e] *= f;
-        }
+        f32x4 (&sc)[2] = scores[t];
         if (key + kUnit > min_limit) {
 #pragma unroll
           for (int s = 0; s < 2; ++s)
@@ -346,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
                 atomicMin(&first[i16 * NB + 4 * c + (__builtin_ctz(is) >> 3)], key + 16 * (j / 4) + 4 * g + j % 4);
         }
       }
-      u32x4 vf[NB];
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
+      for (int c = 0; c < KC; ++c) {
+        u32x4 vf[4];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           uint32_t a = x.v[j][c], b = x.v[j + 1][c];
@@ -360,31 +363,41 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
           if (any_nan) a &= ~(nan_bytes(a) * 0xffu), b &= ~(nan_bytes(b) * 0xffu);
           const uint32_t a0 = two<true, false>(a), a1 = two<true, true>(a);
           const uint32_t b0 = two<true, false>(b), b1 = two<true, true>(b);
-          vf[4 * c][j / 2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
-          vf[4 * c + 1][j / 2] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
-          vf[4 * c + 2][j / 2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
-          vf[4 * c + 3][j / 2] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+          vf[0][j / 2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+          vf[1][j / 2] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+          vf[2][j / 2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+          vf[3][j / 2] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
         }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (NT > 1 && t >= nt) break;
+        for (int t = 0; t < NT; ++t) {
+          if (NT > 1 && t >= nt) break;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          o[t][b] = mfma16<true>(vf[b], hi[t], o[t][b]);
-          o[t][b] = mfma16<true>(vf[b], lo[t], o[t][b]);
+          for (int b = 0; b < 4; ++b) {
+            o[t][4 * c + b] = mfma16<true>(vf[b], hi[t], o[t][4 * c + b]);
+            o[t][4 * c + b] = mfma16<true>(vf[b], lo[t], o[t][4 * c + b]);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
     if (length > 0) {
-      Unit<DP> even, odd;
-      load(even, u0);
-      for (int u = u0; u < u1; u += 2) {
-        if (u + 1 < u1) load(odd, u + 1);
-        compute(even, u);
-        if (u + 1 >= u1) break;
-        if (u + 2 < u1) load(even, u + 2);
-        compute(odd, u + 1);
+      if constexpr (NT == 1) {
+        Unit<DP> even, odd;
+        load(even, u0);
+        for (int u = u0; u < u1; u += 2) {
+          if (u + 1 < u1) load(odd, u + 1);
+          compute(even, u);
+          if (u + 1 >= u1) break;
+          if (u + 2 < u1) load(even, u + 2);
+          compute(odd, u + 1);
+        }
+      } else {  // (the accumulators of more rows leave no room for a second unit; the other waves' loads overlap)
+        Unit<DP> x;
+        for (int u = u0; u < u1; ++u) {
+          load(x, u);
+          compute(x, u);
+        }
       }
     }
 
@@ -441,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
     if (unit < stop) {
       uint64_t after = lane_r == 63 ? 0 : __ballot(mine.units > 0) >> (lane_r + 1) << (lane_r + 1);
       while (!after) {
-        before += __shfl(scan, 63, 64);
+        before += uniform(__shfl(scan, 63, 64));
         base += 64;
         mine = work_of(p, base + lane, most_rows);
         scan = wave_scan(mine.units, lane);
@@ -456,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 && NT == 1 ? 2 : 1) block_
 template <bool BF>
 __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
   const PromptParams& p = bp.a;
-  __shared__ float part[4][512];
+  constexpr int kAhead = 8;
+  __shared__ float part[4][256];
   __shared__ float sums[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int most_rows = bp.rows;
@@ -483,20 +497,29 @@ __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
   for (int x = w0 + lane; x <= w1; x += 64) top = fmaxf(top, record(x)[0]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int x = w0 + wave; x <= w1; x += 4) {
-    const float* rec = record(x);
-    const float f = __builtin_amdgcn_exp2f(rec[0] - top);
-    l += rec[1] * f;
+  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int x0 = w0 + wave; x0 <= w1; x0 += 4 * kAhead) {
+    // kAhead records in flight, each a round trip to memory that other XCDs have written
+    float m[kAhead], sum[kAhead];
+    f32x2 v[kAhead][2];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (2 * (lane + 64 * c) < p.D) {
-        const f32x2 v = *(const f32x2*)(rec + 2 + 2 * (lane + 64 * c));
-        acc[2 * c] += v[0] * f, acc[2 * c + 1] += v[1] * f;
-      }
+    for (int i = 0; i < kAhead; ++i) {
+      const int x = x0 + 4 * i;
+      const float* rec = record(x <= w1 ? x : x0);
+      m[i] = x <= w1 ? rec[0] : -__builtin_inff(), sum[i] = rec[1];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) v[i][c] = *(const f32x2*)(rec + 2 + (2 * (lane + 64 * c) < p.D ? 2 * (lane + 64 * c) : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float f = __builtin_amdgcn_exp2f(m[i] - top);
+      l += sum[i] * f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) acc[2 * c] += v[i][c][0] * f, acc[2 * c + 1] += v[i][c][1] * f;
+    }
   }
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < 2; ++c)
     if (2 * (lane + 64 * c) < p.D) {
       part[wave][2 * (lane + 64 * c)] = acc[2 * c];
       part[wave][2 * (lane + 64 * c) + 1] = acc[2 * c + 1];
@@ -530,9 +553,9 @@ void launch_decode(const BlockParams& bp, hipStream_t stream) {
   hipLaunchKernelGGL((block_merge<BF>), dim3((unsigned)rows), dim3(kThreads), 0, stream, bp);
 }
 
-// Waves of a KV head: about eight for each of the 1,024 SIMDs' three resident ones would be one round; one round.
+// Waves of a KV head: two resident on each of 1,024 SIMDs, one round.
 int workers_for(int64_t H) {
-  const int64_t w = (3072 + H - 1) / H;
+  const int64_t w = (2048 + H - 1) / H;
   return (int)(w < 1 ? 1 : w);
 }
 

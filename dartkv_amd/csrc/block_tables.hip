@@ -9,10 +9,11 @@
 // release: the last d_r tokens of each request go; its blocks from ceil((len - d) / bs) on return to the stack at
 // state[0] + sum(gone) - 1 - (P_r + j): a release of what a reserve gave restores the stack exactly.
 //
-// One launch.  Every workgroup makes the prefix sums over all requests in LDS for itself (8 bytes a request) and
-// writes its share of the slots and of the table's rows; what all of them read (lengths, the stack's count) is
-// changed by the last workgroup to finish, which the ticket tells.  Bound: the latency of reading the lengths and
-// of the ticket's round trip; a second launch for the update would cost as much again.
+// One launch.  Every workgroup makes the prefix sums over all requests in LDS for itself (12 bytes a request) and
+// writes its share of the slots and of the moved blocks, whose requests it finds in the sums by bisection; what all of
+// them read (lengths, the stack's count) is changed by the last workgroup to finish, which the ticket tells.  It needs
+// no fence: the others have only read what it changes, and nothing that they wrote is read.  Bound: latency, a load of
+// the lengths, one of the blocks and the ticket's round trip after each other.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -21,8 +22,8 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRequests = 8190;  // prefix sums of 8 bytes a request in 64 KiB of LDS
-constexpr int kSlotsPerGroup = 1024;
+constexpr int kMaxRequests = 8190;  // 12 bytes each of 160 KiB of LDS
+constexpr int kSlots = 4;  // of a thread
 
 struct TablesParams {
   int32_t *table, *lengths, *free, *state;
@@ -66,15 +67,29 @@ __device__ __forceinline__ Row row_of(const TablesParams& p, int r, int32_t& bad
   return x;
 }
 
+// The last request whose sum (after `shift`) is at most i.
+__device__ __forceinline__ int find(const int64_t* sums, int R, int64_t i, bool tokens) {
+  int lo = 0, hi = R - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((tokens ? sums[mid] >> 32 : (int64_t)(int32_t)sums[mid]) <= i)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
 template <bool RESERVE>
 __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   extern __shared__ int64_t sums[];  // [R + 1]: (tokens before) << 32 | blocks before
-  __shared__ int64_t wave_sum[4];
+  int32_t* lens = (int32_t*)(sums + p.R + 1);  // [R]: the lengths before
+  __shared__ int64_t wave_sum[2][4];
   __shared__ int32_t flags, last;
   __shared__ unsigned long long all_tokens, all_blocks;  // the sums' halves may overflow, these do not
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) flags = 0, all_tokens = 0, all_blocks = 0;
-  __syncthreads();
+  const int64_t count = p.state[0];
 
   int64_t running = 0, my_tokens = 0, my_blocks = 0;
   int32_t bad = 0;
@@ -85,6 +100,7 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
       const Row row = row_of<RESERVE>(p, r, bad);
       x = ((int64_t)row.moved << 32) + row.count;
       my_tokens += row.moved, my_blocks += row.count;
+      lens[r] = row.length;
     }
     int64_t sum = x;
 #pragma unroll
@@ -92,21 +108,21 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
       const int64_t up = __shfl_up(sum, off, 64);
       if (lane >= off) sum += up;
     }
-    if (lane == 63) wave_sum[wave] = sum;
+    int64_t* wsum = wave_sum[base / kThreads & 1];
+    if (lane == 63) wsum[wave] = sum;
     __syncthreads();
     int64_t before = running;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += wave_sum[w];
-      running += wave_sum[w];
+      if (w < wave) before += wsum[w];
+      running += wsum[w];
     }
     if (r < p.R) sums[r] = before + sum - x;
-    __syncthreads();
   }
   if (tid == 0) sums[p.R] = running;
   if (bad) atomicOr(&flags, bad);
   if (my_tokens) atomicAdd(&all_tokens, (unsigned long long)my_tokens);
   if (my_blocks) atomicAdd(&all_blocks, (unsigned long long)my_blocks);
-  const int64_t count = p.state[0];
   __syncthreads();
   bad = flags;
   const int64_t used = (int64_t)all_blocks, moved = (int64_t)all_tokens;
@@ -115,64 +131,65 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   if (!RESERVE && count + used > p.blocks) bad |= kNoBlocks;
   if (RESERVE && moved > p.total) bad |= kBadTotal;
   const bool fits = bad == 0;
+  const int64_t me = (int64_t)blockIdx.x * kThreads + tid, all = (int64_t)gridDim.x * kThreads;
 
   if constexpr (RESERVE) {
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i <= p.R; i += (int64_t)gridDim.x * kThreads)
-      p.starts[i] = fits ? (int32_t)(sums[i] >> 32) : 0;
-    for (int64_t at = (int64_t)blockIdx.x * kSlotsPerGroup + tid; at < p.total; at += (int64_t)gridDim.x * kSlotsPerGroup) {
-      const int64_t stop = at - tid + kSlotsPerGroup;
-      for (int64_t i = at; i < stop && i < p.total; i += kThreads) {
-        int64_t slot = -1;
-        if (fits && i < moved) {
-          int lo = 0, hi = p.R - 1;  // the last request that starts at or before i
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if ((sums[mid] >> 32) <= i)
-              lo = mid;
-            else
-              hi = mid - 1;
-          }
-          const int64_t position = p.lengths[lo] + (i - (sums[lo] >> 32));
-          const int32_t block = (int32_t)(position >> p.shift);
-          const int32_t old = (int32_t)blocks_of(p.lengths[lo], p.shift);
-          const int32_t id = block < old ? p.table[(int64_t)lo * p.max_blocks + block]
-                                         : p.free[count - 1 - ((int32_t)sums[lo] + block - old)];
-          slot = ((int64_t)id << p.shift) + (position & ((1 << p.shift) - 1));
+    for (int64_t i = me; i <= p.R; i += all) p.starts[i] = fits ? (int32_t)(sums[i] >> 32) : 0;
+    const int mask = (1 << p.shift) - 1;
+    for (int64_t at = me * kSlots; at < p.total; at += all * kSlots) {
+      int64_t slot[kSlots];
+      int r = fits && at < moved ? find(sums, p.R, at, true) : 0;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        slot[i] = -1;
+        if (fits && at + i < moved) {
+          while (sums[r + 1] >> 32 <= at + i) ++r;
+          const int64_t position = lens[r] + (at + i - (sums[r] >> 32));
+          const int32_t block = (int32_t)(position >> p.shift), old = (int32_t)blocks_of(lens[r], p.shift);
+          const int32_t id = block < old ? p.table[(int64_t)r * p.max_blocks + block]
+                                         : p.free[count - 1 - ((int32_t)sums[r] + block - old)];
+          slot[i] = ((int64_t)id << p.shift) + (position & mask);
         }
-        p.slots[i] = slot;
+      }
+      if (at + kSlots <= p.total) {
+#pragma unroll
+        for (int i = 0; i < kSlots; i += 2) *(longlong2*)(p.slots + at + i) = make_longlong2(slot[i], slot[i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i)
+          if (at + i < p.total) p.slots[at + i] = slot[i];
       }
     }
   }
-  // the table's rows, one for each wave in turn
+  // the blocks, in the stack's order
   if (fits) {
-    for (int r = blockIdx.x * 4 + wave; r < p.R; r += gridDim.x * 4) {
-      const int32_t before = (int32_t)sums[r], n = (int32_t)sums[r + 1] - before;
-      if (n == 0) continue;
-      int32_t ignored = 0;
-      const Row row = row_of<RESERVE>(p, r, ignored);
-      int32_t* entry = p.table + (int64_t)r * p.max_blocks + row.old;
-      for (int j = lane; j < n; j += 64) {
-        if constexpr (RESERVE) {
-          entry[j] = p.free[count - 1 - (before + j)];
-        } else {
-          p.free[count + used - 1 - (before + j)] = entry[j];
-          entry[j] = -1;
-        }
+    for (int64_t i = me; i < used; i += all) {
+      const int r = find(sums, p.R, i, false);
+      const int64_t j = i - (int32_t)sums[r], length = lens[r];
+      const int64_t old = RESERVE ? blocks_of(length, p.shift)
+                                  : blocks_of(length - ((sums[r + 1] >> 32) - (sums[r] >> 32)), p.shift);
+      int32_t* entry = p.table + (int64_t)r * p.max_blocks + old + j;
+      if constexpr (RESERVE) {
+        *entry = p.free[count - 1 - i];
+      } else {
+        p.free[count + used - 1 - i] = *entry;
+        *entry = -1;
       }
     }
   }
 
   // the last workgroup changes what the others read
-  __threadfence();
   __syncthreads();
-  if (tid == 0) last = atomicAdd(&p.state[2], 1) == (int32_t)gridDim.x - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
+  if (gridDim.x > 1) {
+    if (tid == 0)
+      last = __hip_atomic_fetch_add(&p.state[2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+  }
   if (fits) {
     for (int r = tid; r < p.R; r += kThreads) {
-      int32_t n = (int32_t)((sums[r + 1] >> 32) - (sums[r] >> 32));
-      if (n) p.lengths[r] += RESERVE ? n : -n;
+      const int32_t n = (int32_t)((sums[r + 1] >> 32) - (sums[r] >> 32));
+      if (n) p.lengths[r] = lens[r] + (RESERVE ? n : -n);
     }
     if constexpr (RESERVE)
       for (int64_t i = count - used + tid; i < count; i += kThreads) p.free[i] = -1;
@@ -207,9 +224,11 @@ extern "C" int dkv_reserve_blocks(const dkv_block_tables_args* args, void* strea
   DKV_CHECK(args->tokens && args->starts && (args->slots || args->total == 0), DKV_ERR_INVALID,
             "dkv_reserve_blocks: NULL pointer");
   DKV_CHECK(args->total >= 0 && args->total < (1ll << 31), DKV_ERR_INVALID, "dkv_reserve_blocks: bad total");
-  int64_t groups = (args->total + kSlotsPerGroup - 1) / kSlotsPerGroup;
-  groups = groups < 1 ? 1 : groups > 1024 ? 1024 : groups;
-  hipLaunchKernelGGL(block_tables<true>, dim3((unsigned)groups), dim3(kThreads), 8 * (p.R + 1), (hipStream_t)stream, p);
+  DKV_CHECK(((uintptr_t)args->slots & 15) == 0, DKV_ERR_INVALID, "dkv_reserve_blocks: slots must be 16-byte aligned");
+  int64_t groups = (args->total + kSlots * kThreads - 1) / (kSlots * kThreads);
+  groups = groups < 1 ? 1 : groups > 512 ? 512 : groups;
+  hipLaunchKernelGGL(block_tables<true>, dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8,
+                     (hipStream_t)stream, p);
   return dkv_check_launch("dkv_reserve_blocks");
 }
 
@@ -218,8 +237,9 @@ extern "C" int dkv_release_blocks(const dkv_block_tables_args* args, void* strea
   TablesParams p;
   const int rc = check_tables(*args, "dkv_release_blocks", p);
   if (rc != DKV_OK) return rc;
-  int64_t groups = (p.R + 63) / 64;
-  groups = groups > 128 ? 128 : groups;
-  hipLaunchKernelGGL(block_tables<false>, dim3((unsigned)groups), dim3(kThreads), 8 * (p.R + 1), (hipStream_t)stream, p);
+  int64_t groups = (p.blocks + 4 * kThreads - 1) / (4 * kThreads);  // (at most that many blocks return)
+  groups = groups > 64 ? 64 : groups;
+  hipLaunchKernelGGL(block_tables<false>, dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8,
+                     (hipStream_t)stream, p);
   return dkv_check_launch("dkv_release_blocks");
 }

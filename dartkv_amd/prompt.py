@@ -44,10 +44,15 @@ def int32_vector(t: torch.Tensor, what: str, device: torch.device) -> torch.Tens
     return t.to(torch.int32).contiguous()
 
 
-def aligned_rows(t: torch.Tensor) -> torch.Tensor:
+MAX_TOKEN_STRIDE = (1 << 23) - 1  # elements: the kernels' offsets within a tile have 31 bits
+
+
+def aligned_rows(t: torch.Tensor, token_axis: int) -> torch.Tensor:
     """``t`` with contiguous, 16-byte aligned last-dimension rows (a copy where it has others)."""
     step = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % step for s in t.stride()[:-1]):
+    strides = t.stride()
+    if strides[-1] != 1 or t.data_ptr() % 16 or any(s % step for s in strides[:-1]) \
+            or strides[token_axis] > MAX_TOKEN_STRIDE:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -107,7 +112,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1 \
             or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
         raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
-    query, keys, values = aligned_rows(query), aligned_rows(keys), aligned_rows(values)
+    query, keys, values = aligned_rows(query, t_axis), aligned_rows(keys, t_axis), aligned_rows(values, t_axis)
 
     a = _lib.PromptAttentionArgs()
     if packed:
