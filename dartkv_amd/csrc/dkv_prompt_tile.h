@@ -115,38 +115,62 @@ __device__ __forceinline__ u32x4 buffer(const void* base, uint32_t bytes) {
   return (u32x4){uniform((uint32_t)a), uniform((uint32_t)(a >> 32)) & 0xffffu, uniform(bytes), 0x00027000u};
 }
 
-// Which request and row tile a workgroup has: the requests' tiles in order, found by a wave's scan over them.
+// Which request and row tile a workgroup has.
 struct Tile {
   int request;  // -1: none
   int tile, rows;
-  int64_t q0;   // first token
-  int nq;
+  int nq, nk;
+  int64_t q0, k0;  // first tokens
 };
 
-template <int BM>
+__device__ __forceinline__ int64_t clamped(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// The requests' tiles one after the other, those of more keys first (up to 64 requests; else in their order), found
+// by a wave's scan over the requests: the longest work begins first, and what begins last is short.
+template <int BM, bool BLOCKS>
 __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) {
-  Tile t = {-1, 0, 0, 0, 0};
+  Tile t = {-1, 0, 0, 0, 0, 0, 0};
   const int lane = threadIdx.x & 63;
+  const int64_t most = (int64_t)p.max_blocks << p.bs_shift;
   if (!p.q_starts) {
     const int rows = (int)p.q_tokens * p.G, tiles = (rows + BM - 1) / BM;
     const int r = (int)(index / tiles);
     if (r >= p.R) return t;
-    t = {r, (int)(index - (int64_t)r * tiles), rows, 0, (int)p.q_tokens};
+    const int nk = BLOCKS ? (int)clamped(p.lengths[r], 0, most) : (int)p.k_tokens;
+    t = {r, (int)(index - (int64_t)r * tiles), rows, (int)p.q_tokens, nk, 0, 0};
     return t;
   }
   int64_t before = 0;
   const int total = p.R + (p.fill ? 1 : 0);
   for (int base = 0; base < total; base += 64) {
-    const int r = base + lane;
-    int64_t a = 0, b = 0;
-    if (r < total) {
-      a = p.q_starts[r];
-      b = r < p.R ? p.q_starts[r + 1] : p.q_tokens;
-      a = a < 0 ? 0 : a > p.q_tokens ? p.q_tokens : a;  // (never outside the tensor, whatever the starts say)
-      b = b < a ? a : b > p.q_tokens ? p.q_tokens : b;
+    int r = base + lane;
+    int64_t a = 0, b = 0, ka = 0, kb = 0;
+    if (r < total) {  // (never outside the tensors, whatever the starts say)
+      a = clamped(p.q_starts[r], 0, p.q_tokens);
+      b = r < p.R ? clamped(p.q_starts[r + 1], a, p.q_tokens) : p.q_tokens;
+      if (r < p.R) {
+        if constexpr (BLOCKS) {
+          kb = clamped(p.lengths[r], 0, most);
+        } else {
+          ka = clamped(p.k_starts[r], 0, p.k_tokens);
+          kb = clamped(p.k_starts[r + 1], ka, p.k_tokens);
+        }
+      }
     }
-    int rows = (int)(b - a) * p.G;
+    int rows = (int)(b - a) * p.G, nk = (int)(kb - ka);
     if (rows <= p.skip_rows && r < p.R) rows = 0;
+    if (total > 1 && total <= 64) {  // lane i takes the request of the i-th most keys
+      int rank = 0;
+      for (int i = 0; i < total; ++i) {
+        const int other = __builtin_amdgcn_readlane(nk, i);
+        rank += other > nk || (other == nk && i < lane) ? 1 : 0;
+      }
+      if (lane >= total) rank = lane;
+      r = __builtin_amdgcn_ds_permute(4 * rank, r);
+      rows = __builtin_amdgcn_ds_permute(4 * rank, rows), nk = __builtin_amdgcn_ds_permute(4 * rank, nk);
+      a = __builtin_amdgcn_ds_permute(4 * rank, (int)a), b = __builtin_amdgcn_ds_permute(4 * rank, (int)b);
+      ka = __builtin_amdgcn_ds_permute(4 * rank, (int)ka);
+    }
     const int tiles = (rows + BM - 1) / BM;
     int sum = tiles;
 #pragma unroll
@@ -157,14 +181,14 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
     const uint64_t hit = __ballot(before + sum > index);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      t.request = base + l;
-      t.rows = __shfl(rows, l, 64);
-      t.tile = (int)(index - before) - (__shfl(sum, l, 64) - __shfl(tiles, l, 64));
-      t.q0 = __shfl((int)a, l, 64);
-      t.nq = (int)(__shfl((int)b, l, 64) - t.q0);
+      t.request = __builtin_amdgcn_readlane(r, l);
+      t.rows = __builtin_amdgcn_readlane(rows, l), t.nk = __builtin_amdgcn_readlane(nk, l);
+      t.tile = (int)(index - before) - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));
+      t.q0 = __builtin_amdgcn_readlane((int)a, l), t.k0 = __builtin_amdgcn_readlane((int)ka, l);
+      t.nq = __builtin_amdgcn_readlane((int)b, l) - (int)t.q0;
       return t;
     }
-    before += __shfl(sum, 63, 64);
+    before += __builtin_amdgcn_readlane(sum, 63);
   }
   return t;
 }
@@ -200,11 +224,11 @@ struct DenseSource {
   static constexpr int kCopies = kKeys * DP / 512 / WAVES;  // of a wave, for keys and for values
   static constexpr int kRowBytes = 2 * DP;
 
-  __device__ __forceinline__ void init(const PromptParams& p, const Tile& t, int h, int64_t k0, int nk_) {
+  __device__ __forceinline__ void init(const PromptParams& p, const Tile& t, int h) {
     const int64_t b = p.k_starts ? 0 : t.request;
-    k = (const char*)p.k + 2 * (b * p.k_sb + k0 * p.k_st + h * p.k_sh);
-    v = (const char*)p.v + 2 * (b * p.v_sb + k0 * p.v_st + h * p.v_sh);
-    kst = 2 * p.k_st, vst = 2 * p.v_st, nk = nk_, valid = 2 * p.D;
+    k = (const char*)p.k + 2 * (b * p.k_sb + t.k0 * p.k_st + h * p.k_sh);
+    v = (const char*)p.v + 2 * (b * p.v_sb + t.k0 * p.v_st + h * p.v_sh);
+    kst = 2 * p.k_st, vst = 2 * p.v_st, nk = t.nk, valid = 2 * p.D;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) {
@@ -304,31 +328,19 @@ struct BlockSource {
 };
 
 template <int DP, bool BF, int WAVES, bool BLOCKS>
-__global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(PromptParams p) {
+__global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 128 ? 2 : 1) prompt_tiles(PromptParams p) {
   constexpr int BM = 32 * WAVES, KS = DP / 16, CB = DP / 32, kKeys = keys_of(DP, BLOCKS && !BF), T2 = kKeys / 32;
   constexpr int kRowBytes = 2 * DP, kTileBytes = kKeys * kRowBytes;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
 
   const int h = (int)(blockIdx.x % p.H);
-  Tile t = find_tile<BM>(p, blockIdx.x / p.H);
+  Tile t = find_tile<BM, BLOCKS>(p, blockIdx.x / p.H);
   if (t.request < 0) return;
   t.request = uniform(t.request), t.tile = uniform(t.tile), t.rows = uniform(t.rows), t.nq = uniform(t.nq);
-  t.q0 = (int64_t)uniform((uint32_t)t.q0);
+  t.nk = uniform(t.nk), t.q0 = uniform((uint32_t)t.q0), t.k0 = uniform((uint32_t)t.k0);
   t.tile = (t.rows + BM - 1) / BM - 1 - t.tile;  // the longest tiles first
-  int64_t k0 = 0;
-  int nk = (int)p.k_tokens;
-  if (t.request >= p.R) {
-    nk = 0;
-  } else if constexpr (BLOCKS) {
-    const int64_t most = (int64_t)p.max_blocks << p.bs_shift, length = p.lengths[t.request];
-    nk = uniform((int)(length < 0 ? 0 : length > most ? most : length));
-  } else if (p.k_starts) {
-    int64_t a = p.k_starts[t.request], b = p.k_starts[t.request + 1];
-    a = a < 0 ? 0 : a > p.k_tokens ? p.k_tokens : a;
-    b = b < a ? a : b > p.k_tokens ? p.k_tokens : b;
-    k0 = (int64_t)uniform((uint32_t)a), nk = uniform((int)(b - a));
-  }
+  const int nk = t.nk;
 
   // this lane's row, how many keys it sees, and its query in the products' operand layout
   const int row = t.tile * BM + wave * 32 + (lane & 31);
@@ -346,17 +358,6 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(Pr
   const bool wave_real = t.tile * BM + wave * 32 < t.rows;
   const int wave_min = uniform(limit_of(wave_first / p.G));
   const int wave_max = wave_real ? uniform(limit_of(wave_last / p.G)) : 0;
-
-  u32x4 q[KS];
-  {
-    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + (t.q0 + token) * p.q_st + head * p.q_sh);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int ch = 16 * ks + 8 * half;
-      q[ks] = (u32x4){0, 0, 0, 0};
-      if (real && ch < p.D) q[ks] = *(const u32x4*)(src + 2 * ch);
-    }
-  }
 
   f32x16 o[CB];
   float m, l;
@@ -382,7 +383,25 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(Pr
   DenseSource<DP, WAVES> dense;
   BlockSource<DP, BF, WAVES> blocks(p, t.request, h, nk);
   float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][4]
-  if constexpr (!BLOCKS) dense.init(p, t, h, k0, nk);
+  if constexpr (!BLOCKS) {
+    dense.init(p, t, h);
+    if (tile_limit > 0) dense.issue(0, lds0, lds0 + kTileBytes);
+  }
+
+  u32x4 q[KS];
+  {
+    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + (t.q0 + token) * p.q_st + head * p.q_sh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int ch = 16 * ks + 8 * half;
+      q[ks] = (u32x4){0, 0, 0, 0};
+      if (real && ch < p.D) q[ks] = *(const u32x4*)(src + 2 * ch);
+    }
+    // They are there before the loop: a load that may still be out in it makes the compiler wait in every tile for all
+    // memory traffic, the copies among it (a prompt of 16,384 tokens: 2.16 ms, 2.07 with this).
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(q[ks]));
+  }
   int32_t* first = (int32_t*)(lds + 4 * kTileBytes + 32);  // [2][DP], of the careful pass
   bool careful = false;  // (the same for the whole workgroup)
   for (;;) {
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(Pr
         blocks.issue(0);
         blocks.blocks(kKeys);
         blocks.finish(lds, lds + kTileBytes, lscale);
-      } else {
+      } else if (careful) {
         dense.issue(0, lds0, lds0 + kTileBytes);
       }
     }
@@ -428,12 +447,23 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(Pr
 
       f32x16 s[T2];
 #pragma unroll
-      for (int t2 = 0; t2 < T2; ++t2) {
+      for (int t2 = 0; t2 < T2; ++t2)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[t2][i] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t2 = 0; t2 < T2; ++t2)
           s[t2] = mfma32<BF>(*(const u32x4*)(lk + kaddr[ks] + t2 * 32 * kRowBytes), q[ks], s[t2]);
+      {  // three steps of operands ahead of the matrix instructions
+        constexpr int kMfma = 0x8, kRead = 0x100;
+        __builtin_amdgcn_sched_group_barrier(kRead, 3 * T2, 0);
+#pragma unroll
+        for (int ks = 0; ks < KS - 3; ++ks) {
+          __builtin_amdgcn_sched_group_barrier(kMfma, T2, 0);
+          __builtin_amdgcn_sched_group_barrier(kRead, T2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 3 * T2, 0);
       }
       if constexpr (BLOCKS && !BF) {
 #pragma unroll
@@ -464,38 +494,62 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) prompt_tiles(Pr
           for (int i = 0; i < 16; ++i) o[cb][i] *= f;
       }
       constexpr bool kSplit = BLOCKS && !BF;  // p as two bf16 parts: an fp16 result shows one rounding to bf16
-      u32x4 pk[2 * T2], rest[kSplit ? 2 * T2 : 1];
-#pragma unroll
-      for (int t2 = 0; t2 < T2; ++t2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[t2][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t2][i], p.c, -m));
-          l += s[t2][i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t pair = pack2<BF || BLOCKS>(s[t2][2 * i], s[t2][2 * i + 1]);
-          pk[2 * t2 + i / 4][i % 4] = pair;
-          if constexpr (kSplit)
-            rest[2 * t2 + i / 4][i % 4] =
-                pack2<true>(s[t2][2 * i] - u2f(pair << 16), s[t2][2 * i + 1] - u2f(pair & 0xffff0000u));
-        }
-      }
-#pragma unroll
-      for (int ks = 0; ks < 2 * T2; ++ks)
+      // Step ks: the weights of 16 keys, p = 2^(s c - m) in the operand type, and their products with the values.  A
+      // step's matrix instructions run beside the exponentials and the operands' reads of the step after.
+      u32x4 pk[2], rest[2], a[2][CB];
+      auto values = [&](int ks) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
           union {
             short4v part[2];
             u32x4 whole;
-          } a;
+          } x;
 #pragma unroll
           for (int s2 = 0; s2 < 2; ++s2)
-            a.part[s2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            x.part[s2] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (lds_short4*)(lds_void*)(lv + vaddr[cb][s2] + ks * 16 * kRowBytes));
-          o[cb] = mfma32<BF || BLOCKS>(a.whole, pk[ks], o[cb]);
-          if constexpr (kSplit) o[cb] = mfma32<true>(a.whole, rest[ks], o[cb]);
+          a[ks & 1][cb] = x.whole;
         }
+      };
+      auto weights = [&](int ks) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = 8 * (ks % 2) + 2 * i;
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at], p.c, -m));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at + 1], p.c, -m));
+          l += x, l += y;
+          const uint32_t pair = pack2<BF || BLOCKS>(x, y);
+          pk[ks & 1][i] = pair;
+          if constexpr (kSplit) rest[ks & 1][i] = pack2<true>(x - u2f(pair << 16), y - u2f(pair & 0xffff0000u));
+        }
+      };
+      constexpr bool kAhead = !BLOCKS && DP > 64;  // (not where registers are short: the blocks' loads, three waves a SIMD)
+      if constexpr (kAhead) values(0);
+      weights(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < 2 * T2; ++ks) {
+        if constexpr (!kAhead) values(ks);
+        if (ks + 1 < 2 * T2) {
+          if constexpr (kAhead) values(ks + 1);
+          weights(ks + 1);
+        }
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          o[cb] = mfma32<BF || BLOCKS>(a[ks & 1][cb], pk[ks & 1], o[cb]);
+          if constexpr (kSplit) o[cb] = mfma32<true>(a[ks & 1][cb], rest[ks & 1], o[cb]);
+        }
+        if (ks + 1 < 2 * T2) {
+          constexpr int kMfma = 0x8, kValu = 0x2, kRead = 0x100;
+#pragma unroll
+          for (int i = 0; i < CB; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, kSplit ? 2 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(kValu, (kSplit ? 44 : 28) / CB, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       }
       if constexpr (BLOCKS)
         if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 4 * buf);

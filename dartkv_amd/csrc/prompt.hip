@@ -19,7 +19,7 @@ int launch_waves(const PromptParams& p, int waves, int64_t grid, hipStream_t str
 
 template <bool BF>
 int launch_dim(const PromptParams& p, int waves, int64_t grid, hipStream_t stream) {
-  if (p.D <= 64) return launch_waves<64, BF>(p, waves, grid, stream);
+  if (p.D <= 64) return launch<64, BF, 4>(p, grid, stream);
   if (p.D <= 128) return launch_waves<128, BF>(p, waves, grid, stream);
   return launch<256, BF, 4>(p, grid, stream);  // (eight waves would spill: 128 accumulators, 64 query registers)
 }
@@ -66,7 +66,7 @@ extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void*
     if (!a.q_starts) return a.requests * ((a.q_tokens * G + bm - 1) / bm);
     return (a.q_tokens * G + bm - 1) / bm + a.requests + (p.fill ? 1 : 0);
   };
-  const int waves = a.D <= 128 && tiles_of(256) * a.Hkv >= 512 ? 8 : 4;
+  const int waves = a.D > 64 && a.D <= 128 && tiles_of(256) * a.Hkv >= 512 ? 8 : 4;
   const int64_t grid = tiles_of(32 * waves) * a.Hkv;
   DKV_CHECK(grid < (1ll << 31), DKV_ERR_INVALID, "dkv_prompt_attention: too many tokens");
   return a.dtype == kBF16 ? launch_dim<true>(p, waves, grid, (hipStream_t)stream)
