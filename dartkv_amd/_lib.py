@@ -6,7 +6,6 @@ points raise if the library is missing or a tensor is not on a ROCm device.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -159,6 +158,7 @@ class PromptAttentionArgs(ctypes.Structure):
         *_fields("query keys values out", "q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh o_sb o_st o_sh"),
         *_fields("q_starts k_starts", "requests Hq Hkv D q_tokens k_tokens dtype"),
         ("scale", ctypes.c_double), ("causal", ctypes.c_int64), ("fill", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -190,7 +190,7 @@ EXPORTED = (
     "dkv_dequantize_mixed", "dkv_decode_workspace_bytes", "dkv_decode_attention", "dkv_decode_attention_noalloc",
     "dkv_decode_scratch_bytes", "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize",
     "dkv_decode_route", "dkv_prompt_attention", "dkv_reserve_blocks", "dkv_release_blocks", "dkv_append_blocks",
-    "dkv_block_attention", "dkv_block_attention_workspace_bytes",
+    "dkv_block_attention", "dkv_block_attention_workspace_bytes", "dkv_prompt_attention_workspace_bytes",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -234,7 +234,9 @@ def load() -> ctypes.CDLL:
         lib.dkv_release_blocks.argtypes = [ctypes.POINTER(BlockTablesArgs), vp]
         lib.dkv_append_blocks.argtypes = [ctypes.POINTER(AppendBlocksArgs), vp]
         lib.dkv_block_attention.argtypes = [ctypes.POINTER(BlockAttentionArgs), vp]
-        lib.dkv_block_attention_workspace_bytes.argtypes = [i64, i64, i64, i64]
+        lib.dkv_prompt_attention_workspace_bytes.argtypes = [ctypes.POINTER(PromptAttentionArgs)]
+        lib.dkv_prompt_attention_workspace_bytes.restype = i64
+        lib.dkv_block_attention_workspace_bytes.argtypes = [ctypes.POINTER(BlockAttentionArgs)]
         lib.dkv_block_attention_workspace_bytes.restype = i64
         for name in ("dkv_quantize_rows", "dkv_quantize_row_blocks", "dkv_quantize_value_rows", "dkv_quantize_key_pages",
                      "dkv_dequantize_rows",
@@ -289,14 +291,41 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-def on_device(device: torch.device):
-    """A context in which ``device`` is the current one (HIP launches go to the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE_ALREADY
-    return torch.cuda.device(device)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-_HERE_ALREADY = contextlib.nullcontext()
+def launch(function, args: ctypes.Structure, device: torch.device, where: str, stream: Optional[int] = None) -> None:
+    """Call a C entry point on ``device`` and its current stream (HIP launches go to the current device)."""
+    if stream is None:
+        stream = stream_ptr(device)
+    if device.index == _current_device():
+        rc = function(args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = function(args, stream)
+    if rc != DKV_OK:
+        check(rc, where)
+
+
+# Argument structs of calls that passed their checks, by the tensors' layouts: a later call of the same layouts
+# copies the struct and sets the pointers.
+_templates: dict = {}
+_MAX_TEMPLATES = 1024
+
+
+def layouts(*tensors: torch.Tensor) -> tuple:
+    """What a call's checks look at in its tensors, apart from their addresses."""
+    return tuple([(t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+
+
+def template(key: tuple) -> Optional[ctypes.Structure]:
+    return _templates.get(key)
+
+
+def keep_template(key: tuple, args: ctypes.Structure) -> None:
+    if len(_templates) >= _MAX_TEMPLATES:
+        _templates.clear()
+    _templates[key] = args
 
 
 def ptr(t: Optional[torch.Tensor]) -> int:

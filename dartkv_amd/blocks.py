@@ -49,11 +49,27 @@ def _check_state(table, lengths, free, state, block_size) -> torch.device:
     return device
 
 
-def _tables_args(table, lengths, free, state, block_size) -> _lib.BlockTablesArgs:
-    a = _lib.BlockTablesArgs()
+def _tables_args(name, table, lengths, free, state, tokens, block_size):
+    """Checked arguments of a call on the tables' state, and the counts as an int32 vector."""
+    key = (name, block_size, _lib.layouts(table, lengths, free, state, *(() if tokens is None else (tokens,))))
+    known = _lib.template(key)
+    if known is None:
+        device = _check_state(table, lengths, free, state, block_size)
+        a = _lib.BlockTablesArgs()
+        a.requests, a.max_blocks, a.blocks, a.block_size = table.shape[0], table.shape[1], free.shape[0], block_size
+        if tokens is not None:
+            checked = _counts(tokens, lengths, device)
+            if checked is tokens:
+                _lib.keep_template(key, a)
+            tokens = checked
+        else:
+            _lib.keep_template(key, a)
+        known = a
+    a = _lib.BlockTablesArgs.from_buffer_copy(known)
     a.table, a.lengths, a.free, a.state = table.data_ptr(), lengths.data_ptr(), free.data_ptr(), state.data_ptr()
-    a.requests, a.max_blocks, a.blocks, a.block_size = table.shape[0], table.shape[1], free.shape[0], block_size
-    return a
+    if tokens is not None:
+        a.tokens = tokens.data_ptr()
+    return a, tokens
 
 
 def _counts(tokens, lengths, device) -> torch.Tensor:
@@ -78,17 +94,17 @@ def reserve_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     more tokens than total) changes nothing but ``state[1]``, and its slots are -1 and its starts 0, so that
     appends and attention of that call do nothing (``BlockKVCache.check`` raises).
     """
-    device = _check_state(table, lengths, free, state, block_size)
-    tokens = _counts(tokens, lengths, device)
+    if not isinstance(tokens, torch.Tensor):
+        raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
+    a, tokens = _tables_args("reserve", table, lengths, free, state, tokens, block_size)
     total = int(total)
     if not 0 <= total < 1 << 31:
         raise ValueError("total must not be negative")
+    device = table.device
     slots = torch.empty(total, dtype=torch.int64, device=device)
-    starts = torch.empty(lengths.numel() + 1, dtype=torch.int32, device=device)
-    a = _tables_args(table, lengths, free, state, block_size)
-    a.tokens, a.slots, a.starts, a.total = tokens.data_ptr(), slots.data_ptr(), starts.data_ptr(), total
-    with _lib.on_device(device):
-        _lib.check(_lib.load().dkv_reserve_blocks(a, _lib.stream_ptr(device)), "dkv_reserve_blocks")
+    starts = torch.empty(a.requests + 1, dtype=torch.int32, device=device)
+    a.slots, a.starts, a.total = slots.data_ptr(), starts.data_ptr(), total
+    _lib.launch(_lib.load().dkv_reserve_blocks, a, device, "dkv_reserve_blocks")
     return slots, starts
 
 
@@ -97,13 +113,10 @@ def release_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     """Drop the last ``tokens[r]`` tokens of each request (None: all of them; more than it has: all it has) and
     return the blocks in which none is left to the free stack.  The exact inverse of ``reserve_blocks`` with the
     same counts: rejected draft tokens are given back as they were taken."""
-    device = _check_state(table, lengths, free, state, block_size)
-    a = _tables_args(table, lengths, free, state, block_size)
-    if tokens is not None:
-        tokens = _counts(tokens, lengths, device)
-        a.tokens = tokens.data_ptr()
-    with _lib.on_device(device):
-        _lib.check(_lib.load().dkv_release_blocks(a, _lib.stream_ptr(device)), "dkv_release_blocks")
+    if tokens is not None and not isinstance(tokens, torch.Tensor):
+        raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
+    a, tokens = _tables_args("release", table, lengths, free, state, tokens, block_size)
+    _lib.launch(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
 
 
 def _check_pool(key_codes, value_codes, key_scale, value_scale, device):
@@ -140,6 +153,29 @@ def append_blocks(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor,
     not count for the scale, and set ``nonfinite`` (an int32 scalar tensor) to 1.  head_dim: a multiple of 16 up to
     256.
     """
+    key = ("append", _lib.layouts(keys, values, slots, key_codes, value_codes, key_scale, value_scale))
+    known = _lib.template(key)
+    if known is None or (keys.data_ptr() | values.data_ptr()) % 16:
+        a, keys, values, slots, whole = _checked_append(keys, values, slots, key_codes, value_codes, key_scale, value_scale)
+        if whole:
+            _lib.keep_template(key, a)
+    else:
+        a = known
+    device = keys.device
+    if nonfinite is not None and (nonfinite.dtype != torch.int32 or nonfinite.numel() != 1
+                                  or nonfinite.device != device):
+        raise TypeError("nonfinite must be an int32 tensor of one element on the same device")
+    if a.tokens == 0:
+        return
+    a = _lib.AppendBlocksArgs.from_buffer_copy(a)
+    a.keys, a.values, a.slots = keys.data_ptr(), values.data_ptr(), slots.data_ptr()
+    a.key_codes, a.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
+    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
+    a.nonfinite = 0 if nonfinite is None else nonfinite.data_ptr()
+    _lib.launch(_lib.load().dkv_append_blocks, a, device, "dkv_append_blocks")
+
+
+def _checked_append(keys, values, slots, key_codes, value_codes, key_scale, value_scale):
     _lib.require_device(keys, values, slots, key_codes, value_codes, key_scale, value_scale)
     device = keys.device
     if keys.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -158,23 +194,14 @@ def append_blocks(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor,
         raise TypeError("slots must be an int64 tensor with one entry per token")
     if values.device != device or slots.device != device:
         raise ValueError("the tensors must be on the same device")
-    if nonfinite is not None and (nonfinite.dtype != torch.int32 or nonfinite.numel() != 1
-                                  or nonfinite.device != device):
-        raise TypeError("nonfinite must be an int32 tensor of one element on the same device")
-    if T == 0:
-        return
-    keys, values, slots = aligned_rows(keys.detach(), 0), aligned_rows(values.detach(), 0), slots.contiguous()
+    given = (keys, values, slots)
+    keys, values, slots = aligned_rows(keys, 0), aligned_rows(values, 0), slots.contiguous()
     a = _lib.AppendBlocksArgs()
-    a.keys, a.values, a.slots = keys.data_ptr(), values.data_ptr(), slots.data_ptr()
     a.dtype = _lib.dtype_code(keys.dtype)
     a.k_st, a.k_sh, a.v_st, a.v_sh = keys.stride(0), keys.stride(1), values.stride(0), values.stride(1)
     a.tokens, a.H, a.D = T, H, D
     a.blocks, a.block_size = key_codes.shape[0], key_codes.shape[2]
-    a.key_codes, a.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
-    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
-    a.nonfinite = 0 if nonfinite is None else nonfinite.data_ptr()
-    with _lib.on_device(device):
-        _lib.check(_lib.load().dkv_append_blocks(a, _lib.stream_ptr(device)), "dkv_append_blocks")
+    return a, keys, values, slots, all(x is y for x, y in zip(given, (keys, values, slots)))
 
 
 def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scale: torch.Tensor,
@@ -197,6 +224,43 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     Statistics and sums are fp32.  Forward only: a query that requires gradients is refused outside
     torch.no_grad().
     """
+    fill = out is None
+    scale = None if scale is None else float(scale)
+    max_tokens = None if max_tokens is None else int(max_tokens)
+    key = None
+    if starts is None or starts.dtype == torch.int32:
+        key = ("attend", max_tokens, scale, fill,
+               _lib.layouts(query, key_codes, value_codes, key_scale, value_scale, table, lengths,
+                            *(() if starts is None else (starts,)), *(() if fill else (out,))), starts is None)
+    known = _lib.template(key) if key is not None else None
+    if known is not None and not query.data_ptr() % 16 and (fill or not out.data_ptr() % 8):
+        no_gradients("block_attention", query)
+        a = known
+    else:
+        a, query, starts, whole = _checked_attention(query, key_codes, value_codes, key_scale, value_scale, table,
+                                                     lengths, starts, max_tokens, scale, out)
+        if whole and key is not None:
+            _lib.keep_template(key, a)
+    device = query.device
+    if fill:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if a.tokens == 0:
+        return out
+    stream = _lib.stream_ptr(device)
+    a = _lib.BlockAttentionArgs.from_buffer_copy(a)
+    workspace = _workspace(device, a.workspace_bytes, stream)
+    a.query, a.out, a.workspace = query.data_ptr(), out.data_ptr(), workspace.data_ptr()
+    if starts is not None:
+        a.starts = starts.data_ptr()
+    a.table, a.lengths = table.data_ptr(), lengths.data_ptr()
+    a.key_codes, a.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
+    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
+    _lib.launch(_lib.load().dkv_block_attention, a, device, "dkv_block_attention", stream)
+    return out
+
+
+def _checked_attention(query, key_codes, value_codes, key_scale, value_scale, table, lengths, starts, max_tokens, scale,
+                       out):
     _lib.require_device(query, key_codes, value_codes, key_scale, value_scale, table, lengths)
     device = query.device
     if query.dtype not in (torch.bfloat16, torch.float16):
@@ -217,6 +281,7 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
         raise TypeError("lengths must be a contiguous int32 [requests] tensor")
     if table.device != device or lengths.device != device:
         raise ValueError("the tensors must be on the same device")
+    given = (query, starts)
     if starts is None:
         if T != table.shape[0]:
             raise ValueError("without starts the query holds one token per request")
@@ -225,40 +290,28 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
         starts = int32_vector(starts, "starts", device)
         if starts.numel() != table.shape[0] + 1:
             raise ValueError("starts must hold one more entry than there are requests")
-        most = T
+        most = max(1, T)
     if max_tokens is not None:
         if max_tokens < 1:
             raise ValueError("max_tokens must be positive")
         most = min(most, int(max_tokens))
     factor = scale_factor(scale, D, "block_attention")
     fill = out is None
-    if out is None:
-        out = torch.empty(T, Hq, D, dtype=query.dtype, device=device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1 \
-            or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
+    if not fill and (out.shape != query.shape or out.dtype != query.dtype or out.device != device
+                     or out.stride(-1) != 1 or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1])):
         raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
-    if T == 0:
-        return out
     query = aligned_rows(query, 0)
-    lib = _lib.load()
     a = _lib.BlockAttentionArgs()
-    a.query, a.out, a.dtype = query.data_ptr(), out.data_ptr(), _lib.dtype_code(query.dtype)
-    a.q_st, a.q_sh, a.o_st, a.o_sh = query.stride(0), query.stride(1), out.stride(0), out.stride(1)
-    a.tokens, a.starts = T, _lib.ptr(starts)
-    a.table, a.lengths = table.data_ptr(), lengths.data_ptr()
+    a.dtype = _lib.dtype_code(query.dtype)
+    a.q_st, a.q_sh = query.stride(0), query.stride(1)
+    a.o_st, a.o_sh = (Hq * D, D) if fill else out.stride()[:2]
+    a.tokens = T
     a.requests, a.max_blocks = table.shape
     a.blocks, a.block_size = blocks, block_size
-    a.key_codes, a.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
-    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
     a.Hq, a.Hkv, a.D = Hq, Hkv, D
     a.scale, a.max_tokens, a.fill = factor, most, fill
-    with _lib.on_device(device):
-        stream = _lib.stream_ptr(device)
-        a.workspace_bytes = lib.dkv_block_attention_workspace_bytes(Hq, Hkv, D, most)
-        workspace = _workspace(device, a.workspace_bytes, stream)
-        a.workspace = workspace.data_ptr()
-        _lib.check(lib.dkv_block_attention(a, stream), "dkv_block_attention")
-    return out
+    a.workspace_bytes = _lib.load().dkv_block_attention_workspace_bytes(a)
+    return a, query, starts, query is given[0] and starts is given[1]
 
 
 class BlockPlan(NamedTuple):

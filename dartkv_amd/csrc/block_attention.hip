@@ -227,40 +227,43 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
       if (!good) my_ks = __builtin_nanf(""), my_vs = 1.f;  // a row that sees a bad entry is NaN
     };
     bool nans = false;
-    const uint32_t klane = i16 * p.D + g * (DP / 4), vlane = 4 * g * p.D + i16 * NB;
-    auto load = [&](Unit<DP>& x, int u) {
+    // This lane's bytes of a half tile.  Channels behind head_dim read the first ones' bytes: their key operands are set
+    // to 0 where they are used (a select beside the load would wait for it), their values' sums are not stored.
+    const bool behind = p.D < DP;
+    uint32_t kat[KC];
+#pragma unroll
+    for (int c = 0; c < KC; ++c) kat[c] = i16 * p.D + (g * (DP / 4) + c * 16 < p.D ? g * (DP / 4) + c * 16 : 0);
+    const uint32_t vat = 4 * g * p.D + (i16 * NB < p.D ? i16 * NB : 0);
+    auto place = [&](int key, int s, int& at) {  // the byte of a half tile's first key in the codes
+      at = ((key + 16 * s) >> p.bs_shift) - cached;
+      const int id = uniform(__builtin_amdgcn_readlane(my_block, at));
+      return (((int64_t)id * p.H + h) * (1 << p.bs_shift) + ((key + 16 * s) & ((1 << p.bs_shift) - 1))) * p.D;
+    };
+    auto load_keys = [&](Unit<DP>& x, int u) {
       const int key = u * kUnit;
       const int last_block = (key + 16) >> p.bs_shift;
       if (last_block >= cached + 64 || (key >> p.bs_shift) < cached || cached < 0) fetch_blocks(key >> p.bs_shift);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const int at = ((key + 16 * s) >> p.bs_shift) - cached;
-        const int id = uniform(__builtin_amdgcn_readlane(my_block, at));
+        int at;
+        const uint8_t* kp = p.kc + place(key, s, at);
         x.ks[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_ks), at));
-        x.vs[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_vs), at));
-        const int64_t off =
-            (((int64_t)id * p.H + h) * (1 << p.bs_shift) + ((key + 16 * s) & ((1 << p.bs_shift) - 1))) * p.D;
-        const uint8_t* kp = p.kc + off;
-        const uint8_t* vp = p.vc + off;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const bool in = g * (DP / 4) + c * 16 < p.D;
-          x.k[s][c] = *(const u32x4*)(kp + (in ? klane + c * 16 : 0u));
-          if (!in) x.k[s][c] = (u32x4){0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool in = i16 * NB < p.D;
-          x.v[4 * s + j] = *(const typename Unit<DP>::dwords*)(vp + j * p.D + (in ? vlane : 0u));
-          if (!in)
-#pragma unroll
-            for (int c = 0; c < KC; ++c) x.v[4 * s + j][c] = 0;
-        }
+        for (int c = 0; c < KC; ++c) x.k[s][c] = *(const u32x4*)(kp + kat[c]);
       }
     };
-    auto compute = [&](const Unit<DP>& x, int u) {
+    auto load_values = [&](Unit<DP>& x, int u) {  // after the unit's keys
       const int key = u * kUnit;
-      f32x4 scores[NT][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        int at;
+        const uint8_t* vp = p.vc + place(key, s, at);
+        x.vs[s] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_vs), at));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.v[4 * s + j] = *(const typename Unit<DP>::dwords*)(vp + j * p.D + vat);
+      }
+    };
+    auto products = [&](const Unit<DP>& x, f32x4 (&scores)[NT][2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         u32x4 kf[KS];
@@ -268,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
         for (int c = 0; c < KS; ++c) {
           const uint32_t a = x.k[s][c / 2][2 * (c % 2)], b = x.k[s][c / 2][2 * (c % 2) + 1];
           kf[c] = (u32x4){two<BF, false>(a), two<BF, true>(a), two<BF, false>(b), two<BF, true>(b)};
+          if (behind && g * (DP / 4) + c * 8 >= p.D) kf[c] = (u32x4){0, 0, 0, 0};
         }
         const float f = p.c * x.ks[s];
 #pragma unroll
@@ -281,6 +285,9 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
         }
         __builtin_amdgcn_sched_barrier(0);  // (one half's operands in registers at a time)
       }
+    };
+    auto sums = [&](const Unit<DP>& x, f32x4 (&scores)[NT][2], int u) {
+      const int key = u * kUnit;
       u32x4 hi[NT], lo[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -382,8 +389,11 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
     };
 
     if (length > 0) {
+      f32x4 scores[NT][2];
       if constexpr (NT == 1) {
         Unit<DP> even, odd;
+        auto load = [&](Unit<DP>& x, int u) { load_keys(x, u), load_values(x, u); };
+        auto compute = [&](const Unit<DP>& x, int u) { products(x, scores), sums(x, scores, u); };
         load(even, u0);
         for (int u = u0; u < u1; u += 2) {
           if (u + 1 < u1) load(odd, u + 1);
@@ -392,11 +402,16 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
           if (u + 2 < u1) load(even, u + 2);
           compute(odd, u + 1);
         }
-      } else {  // (the accumulators of more rows leave no room for a second unit; the other waves' loads overlap)
+      } else {
+        // The accumulators of more rows leave no room for a second unit: the next keys are read once the products
+        // have used these, the next values after the sums.
         Unit<DP> x;
+        load_keys(x, u0), load_values(x, u0);
         for (int u = u0; u < u1; ++u) {
-          load(x, u);
-          compute(x, u);
+          products(x, scores);
+          if (u + 1 < u1) load_keys(x, u + 1);
+          sums(x, scores, u);
+          if (u + 1 < u1) load_values(x, u + 1);
         }
       }
     }
@@ -465,75 +480,92 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
   }
 }
 
-// Joins the records of the requests that several waves had: one workgroup per (request, KV head, row).
-template <bool BF>
+// Joins the records of the requests that several waves had, a row of a request and KV head at a time: by one wave, or
+// (WIDE) by a workgroup's four where there are few rows, so that all of a long request's records are in flight.
+template <bool BF, bool WIDE>
 __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
   const PromptParams& p = bp.a;
-  constexpr int kAhead = 8;
-  __shared__ float part[4][256];
-  __shared__ float sums[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int most_rows = bp.rows;
-  const int h = (int)(blockIdx.x % p.H), row = (int)(blockIdx.x / p.H % most_rows);
-  const int r = (int)(blockIdx.x / p.H / most_rows);
-  const Work w = work_of(p, r, most_rows);
+  constexpr int kAhead = 8;  // records in flight of a wave, each a round trip to memory that other XCDs have written
+  __shared__ float part[WIDE ? 4 : 1][256];
+  __shared__ float sums[4], tops[4];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int64_t unit = WIDE ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int h = (int)(unit % p.H), row = (int)(unit / p.H % bp.rows);
+  const int r = (int)(unit / p.H / bp.rows);
+  if (r >= p.R) return;
+  const Work w = work_of(p, r, bp.rows);
   if (row >= w.rows) return;
   int64_t total = 0, start = 0;
   for (int base = 0; base < p.R; base += 64) {
-    int x = work_of(p, base + lane, most_rows).units;
+    int x = work_of(p, base + lane, bp.rows).units;
     int y = base + lane < r ? x : 0;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64), y += __shfl_xor(y, off, 64);
     total += x, start += y;
   }
-  const int64_t share = share_of(total, bp.workers);
-  const int w0 = (int)(start / share), w1 = (int)((start + w.units - 1) / share);
+  const int64_t share = share_of(uniform64(total), bp.workers);
+  start = uniform64(start);
+  const int w0 = uniform((int)(start / share)), w1 = uniform((int)((start + w.units - 1) / share));
   if (w0 == w1) return;
-  auto record = [&](int x) {
-    const int slot = x == w0 ? 1 : 0;  // a part that begins the request, or goes on with it
-    return bp.records + ((((int64_t)x * 2 + slot) * p.H + h) * most_rows + row) * (p.D + 2);
-  };
-  float top = -3.402823466e38f;
-  for (int x = w0 + lane; x <= w1; x += 64) top = fmaxf(top, record(x)[0]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int x0 = w0 + wave; x0 <= w1; x0 += 4 * kAhead) {
-    // kAhead records in flight, each a round trip to memory that other XCDs have written
-    float m[kAhead], sum[kAhead];
+  float m = -3.402823466e38f, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int kStep = WIDE ? 4 : 1;
+  for (int x0 = w0 + (WIDE ? wave : 0); x0 <= w1; x0 += kStep * kAhead) {
+    float rm[kAhead], rl[kAhead];
     f32x2 v[kAhead][2];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int x = x0 + 4 * i;
-      const float* rec = record(x <= w1 ? x : x0);
-      m[i] = x <= w1 ? rec[0] : -__builtin_inff(), sum[i] = rec[1];
+      const int x = x0 + kStep * i <= w1 ? x0 + kStep * i : x0;
+      const int slot = x == w0 ? 1 : 0;  // a part that begins the request, or goes on with it
+      const float* rec = bp.records + ((((int64_t)x * 2 + slot) * p.H + h) * bp.rows + row) * (p.D + 2);
+      rm[i] = x0 + kStep * i <= w1 ? rec[0] : -__builtin_inff(), rl[i] = rec[1];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[i][c] = *(const f32x2*)(rec + 2 + (2 * (lane + 64 * c) < p.D ? 2 * (lane + 64 * c) : 0));
+      for (int c = 0; c < 2; ++c)
+        v[i][c] = *(const f32x2*)(rec + 2 + (2 * (lane + 64 * c) < p.D ? 2 * (lane + 64 * c) : 0));
     }
+    float up = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) up = fmaxf(up, rm[i]);
+    const float f0 = __builtin_amdgcn_exp2f(m - up);
+    m = up, l *= f0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] *= f0;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const float f = __builtin_amdgcn_exp2f(m[i] - top);
-      l += sum[i] * f;
+      const float f = __builtin_amdgcn_exp2f(rm[i] - up);
+      l += rl[i] * f;
 #pragma unroll
       for (int c = 0; c < 2; ++c) acc[2 * c] += v[i][c][0] * f, acc[2 * c + 1] += v[i][c][1] * f;
     }
   }
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (2 * (lane + 64 * c) < p.D) {
-      part[wave][2 * (lane + 64 * c)] = acc[2 * c];
-      part[wave][2 * (lane + 64 * c) + 1] = acc[2 * c + 1];
-    }
-  if (lane == 0) sums[wave] = l;
-  __syncthreads();
-  l = sums[0] + sums[1] + sums[2] + sums[3];
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int token = row / p.G, head = h * p.G + row % p.G;
   uint16_t* dst = (uint16_t*)p.o + (w.q0 + token) * p.o_st + head * p.o_sh;
-  for (int c = 2 * threadIdx.x; c < p.D; c += 2 * kThreads) {
-    const float a = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
-    const float b = (part[0][c + 1] + part[1][c + 1]) + (part[2][c + 1] + part[3][c + 1]);
-    *(uint32_t*)(dst + c) = pack2<BF>(a * inv, b * inv);
+  if constexpr (!WIDE) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (2 * (lane + 64 * c) < p.D)
+        *(uint32_t*)(dst + 2 * (lane + 64 * c)) = pack2<BF>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (2 * (lane + 64 * c) < p.D) {
+        part[wave][2 * (lane + 64 * c)] = acc[2 * c];
+        part[wave][2 * (lane + 64 * c) + 1] = acc[2 * c + 1];
+      }
+    }
+    if (lane == 0) sums[wave] = l, tops[wave] = m;
+    __syncthreads();
+    const float up = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float f[4], all = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __builtin_amdgcn_exp2f(tops[i] - up), all += sums[i] * f[i];
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    for (int c = 2 * threadIdx.x; c < p.D; c += 2 * kThreads) {
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a += part[i][c] * f[i], b += part[i][c + 1] * f[i];
+      *(uint32_t*)(dst + c) = pack2<BF>(a * inv, b * inv);
+    }
   }
 }
 
@@ -543,14 +575,15 @@ void launch_decode(const BlockParams& bp, hipStream_t stream) {
   const dim3 grid((unsigned)((waves + 3) / 4));
   if (bp.rows <= 16)
     hipLaunchKernelGGL((block_decode<DP, BF, 1>), grid, dim3(kThreads), 0, stream, bp);
-  else if constexpr (DP <= 128) {
-    if (bp.rows <= 32)
-      hipLaunchKernelGGL((block_decode<DP, BF, 2>), grid, dim3(kThreads), 0, stream, bp);
-    else if constexpr (DP == 64)
-      hipLaunchKernelGGL((block_decode<DP, BF, 4>), grid, dim3(kThreads), 0, stream, bp);
-  }
+  else if constexpr (DP <= 128)
+    hipLaunchKernelGGL((block_decode<DP, BF, 2>), grid, dim3(kThreads), 0, stream, bp);
+  // one wave a row where that gives the CUs eight each (16 requests of four tokens, 32 rows a KV head: 19.7 us with
+  // four waves a row), else four (one request of 4,000 tokens: 64 records in two rounds)
   const int64_t rows = (int64_t)bp.a.R * bp.rows * bp.a.H;
-  hipLaunchKernelGGL((block_merge<BF>), dim3((unsigned)rows), dim3(kThreads), 0, stream, bp);
+  if (rows >= 2048)
+    hipLaunchKernelGGL((block_merge<BF, false>), dim3((unsigned)((rows + 3) / 4)), dim3(kThreads), 0, stream, bp);
+  else
+    hipLaunchKernelGGL((block_merge<BF, true>), dim3((unsigned)rows), dim3(kThreads), 0, stream, bp);
 }
 
 // Waves of a KV head: two resident on each of 1,024 SIMDs, one round.
@@ -562,22 +595,18 @@ int workers_for(int64_t H) {
 // Rows of a request that this kernel takes: all up to what the accumulators leave registers for, else those of at
 // most 16 rows.
 int rows_for(int64_t max_tokens, int64_t G, int64_t D) {
-  const int64_t most = D <= 64 ? 64 : D <= 128 ? 32 : 16;
+  const int64_t most = D <= 128 ? 32 : 16;
   return max_tokens <= most / G ? (int)(max_tokens * G) : 16;
 }
 
-}  // namespace
-
-extern "C" int64_t dkv_block_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_tokens) {
-  if (Hkv < 1 || Hq < Hkv || D < 1 || max_tokens < 1) return 0;
-  return 2 * (int64_t)workers_for(Hkv) * Hkv * rows_for(max_tokens, Hq / Hkv, D) * (D + 2) * 4;
+int64_t most_tokens(const dkv_block_attention_args& a) {
+  const int64_t most = a.max_tokens < a.tokens ? a.max_tokens : a.tokens;
+  return most < 1 ? 1 : most;
 }
 
-extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* stream) {
-  DKV_CHECK(args != nullptr, DKV_ERR_INVALID, "dkv_block_attention: args is NULL");
-  const dkv_block_attention_args& a = *args;
+int check_blocks(const dkv_block_attention_args& a) {
   DKV_CHECK(a.dtype == kF16 || a.dtype == kBF16, DKV_ERR_DTYPE, "dkv_block_attention: the query must be bf16 or fp16");
-  DKV_CHECK(a.Hkv >= 1 && a.Hq >= a.Hkv && a.Hq % a.Hkv == 0, DKV_ERR_INVALID,
+  DKV_CHECK(a.Hkv >= 1 && a.Hq >= a.Hkv && a.Hq % a.Hkv == 0 && a.Hq < (1 << 20), DKV_ERR_INVALID,
             "dkv_block_attention: query heads must be divisible by the cache's KV heads");
   DKV_CHECK(a.D >= 16 && a.D <= 256 && a.D % 16 == 0, DKV_ERR_INVALID,
             "dkv_block_attention: head_dim must be a multiple of 16 up to 256");
@@ -585,9 +614,48 @@ extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* s
             "dkv_block_attention: block_size must be 16, 32, 64, 128 or 256");
   DKV_CHECK(a.requests >= 1 && a.tokens >= 0 && a.blocks >= 1 && a.max_blocks >= 1 && a.max_tokens >= 1,
             DKV_ERR_INVALID, "dkv_block_attention: bad counts");
-  DKV_CHECK(a.tokens * (a.Hq / a.Hkv) < (1ll << 31) && a.max_blocks * a.block_size < (1ll << 31) &&
-                a.blocks < (1ll << 31) && a.requests < (1 << 24),
+  DKV_CHECK(a.tokens < (1ll << 31) / (a.Hq / a.Hkv) - 1024 && a.max_blocks < ((1ll << 31) - 1024) / a.block_size &&
+                a.blocks < (1ll << 31) && a.requests < (1 << 24) && a.requests * 32 * a.Hkv < (1ll << 31),
             DKV_ERR_INVALID, "dkv_block_attention: too many tokens");
+  return DKV_OK;
+}
+
+BlockParams params_of(const dkv_block_attention_args& a) {
+  BlockParams bp = {};
+  PromptParams& p = bp.a;
+  p.q = a.query, p.o = a.out;
+  p.q_st = a.q_st, p.q_sh = a.q_sh, p.o_st = a.o_st, p.o_sh = a.o_sh;
+  p.q_starts = a.starts;
+  p.R = (int32_t)a.requests, p.H = (int32_t)a.Hkv, p.G = (int32_t)(a.Hq / a.Hkv), p.D = (int32_t)a.D;
+  p.q_tokens = a.tokens;
+  p.c = (float)(a.scale * 1.4426950408889634);
+  p.causal = 1, p.fill = a.fill ? 1 : 0, p.splits = 1;
+  p.kc = a.key_codes, p.vc = a.value_codes, p.kscale = a.key_scale, p.vscale = a.value_scale;
+  p.table = a.table, p.lengths = a.lengths, p.blocks = a.blocks, p.max_blocks = (int32_t)a.max_blocks;
+  p.bs_shift = __builtin_ctzll((uint64_t)a.block_size);
+  bp.workers = workers_for(a.Hkv), bp.rows = rows_for(most_tokens(a), p.G, p.D);
+  return bp;
+}
+
+int64_t workspace_of(const dkv_block_attention_args& a, const BlockParams& bp) {
+  const int64_t few = 2 * (int64_t)bp.workers * a.Hkv * bp.rows * (a.D + 2) * 4;
+  if (most_tokens(a) <= bp.rows / bp.a.G) return few;
+  const int64_t many = block_chunks_workspace_bytes(bp.a, a.tokens * bp.a.G, a.dtype == kBF16);
+  return few > many ? few : many;  // (one after the other on the stream)
+}
+
+}  // namespace
+
+extern "C" int64_t dkv_block_attention_workspace_bytes(const dkv_block_attention_args* args) {
+  if (!args || check_blocks(*args) != DKV_OK) return 0;
+  return workspace_of(*args, params_of(*args));
+}
+
+extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* stream) {
+  DKV_CHECK(args != nullptr, DKV_ERR_INVALID, "dkv_block_attention: args is NULL");
+  const dkv_block_attention_args& a = *args;
+  const int bad = check_blocks(a);
+  if (bad != DKV_OK) return bad;
   DKV_CHECK(a.starts || a.tokens == a.requests, DKV_ERR_INVALID,
             "dkv_block_attention: without starts every request has one token");
   DKV_CHECK(a.scale > 0 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_block_attention: scale must be positive and finite");
@@ -598,23 +666,10 @@ extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* s
               (uintptr_t)a.value_codes) & 15) == 0 &&
                 (((uintptr_t)a.out | (uintptr_t)(2 * a.o_st) | (uintptr_t)(2 * a.o_sh)) & 7) == 0,
             DKV_ERR_INVALID, "dkv_block_attention: query rows must be 16-byte aligned, output rows 8-byte");
-  BlockParams bp = {};
+  BlockParams bp = params_of(a);
   PromptParams& p = bp.a;
-  p.q = a.query, p.o = a.out;
-  p.q_st = a.q_st, p.q_sh = a.q_sh, p.o_st = a.o_st, p.o_sh = a.o_sh;
-  p.q_starts = a.starts;
-  p.R = (int32_t)a.requests, p.H = (int32_t)a.Hkv, p.G = (int32_t)(a.Hq / a.Hkv), p.D = (int32_t)a.D;
-  p.q_tokens = a.tokens;
-  p.c = (float)(a.scale * 1.4426950408889634);
-  p.causal = 1, p.fill = a.fill ? 1 : 0;
-  p.kc = a.key_codes, p.vc = a.value_codes, p.kscale = a.key_scale, p.vscale = a.value_scale;
-  p.table = a.table, p.lengths = a.lengths, p.blocks = a.blocks, p.max_blocks = (int32_t)a.max_blocks;
-  p.bs_shift = __builtin_ctzll((uint64_t)a.block_size);
-  const int64_t most = a.max_tokens < a.tokens ? a.max_tokens : a.tokens;
-  bp.workers = workers_for(a.Hkv), bp.rows = rows_for(most, p.G, p.D);
-  DKV_CHECK(a.workspace && a.workspace_bytes >= dkv_block_attention_workspace_bytes(a.Hq, a.Hkv, a.D, most),
+  DKV_CHECK(a.workspace && ((uintptr_t)a.workspace & 15) == 0 && a.workspace_bytes >= workspace_of(a, bp),
             DKV_ERR_INVALID, "dkv_block_attention: workspace too small");
-  DKV_CHECK(a.requests * bp.rows * a.Hkv < (1ll << 31), DKV_ERR_INVALID, "dkv_block_attention: too many requests");
   bp.records = (float*)a.workspace;
   const bool bf = a.dtype == kBF16;
   const hipStream_t s = (hipStream_t)stream;
@@ -625,8 +680,8 @@ extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* s
   else
     bf ? launch_decode<256, true>(bp, s) : launch_decode<256, false>(bp, s);
   const int rc = dkv_check_launch("dkv_block_attention");
-  if (rc != DKV_OK || most <= bp.rows / p.G) return rc;
+  if (rc != DKV_OK || most_tokens(a) <= bp.rows / p.G) return rc;
   p.skip_rows = bp.rows, p.fill = 0;
   if (!a.starts) p.q_tokens = 1, p.q_sb = a.q_st, p.o_sb = a.o_st;  // a batch of one token each
-  return launch_block_chunks(p, a.tokens * p.G, bf, stream);
+  return launch_block_chunks(p, a.tokens * p.G, bf, a.workspace, stream);
 }

@@ -6,7 +6,8 @@
 
 namespace dkv {
 
-// The chunk kernel (blocks_chunk.hip): the requests of more than p.skip_rows query rows.
-int launch_block_chunks(const PromptParams& p, int64_t rows_bound, bool bf16, void* stream);
+// The chunk kernel (block_chunks.hip): the requests of more than p.skip_rows query rows, of rows_bound rows in all.
+int64_t block_chunks_workspace_bytes(const PromptParams& p, int64_t rows_bound, bool bf16);
+int launch_block_chunks(PromptParams p, int64_t rows_bound, bool bf16, void* workspace, void* stream);
 
 }  // namespace dkv

@@ -44,6 +44,10 @@ struct PromptParams {
   int64_t blocks;
   int32_t max_blocks, bs_shift;
   int32_t skip_rows;  // requests of at most this many rows are another kernel's
+  // A tile's keys in up to `splits` parts of at least kMinPart key tiles, where there are few tiles: each part leaves a
+  // record, o [BM][D] and (m, l) [BM], that prompt_merge joins.
+  int32_t splits;
+  float *records, *stats;
 };
 
 namespace prompt {
@@ -55,6 +59,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
@@ -113,6 +118,18 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgc
 __device__ __forceinline__ u32x4 buffer(const void* base, uint32_t bytes) {
   const uint64_t a = (uint64_t)(uintptr_t)base;
   return (u32x4){uniform((uint32_t)a), uniform((uint32_t)(a >> 32)) & 0xffffu, uniform(bytes), 0x00027000u};
+}
+
+constexpr int kMinPart = 8;
+
+// Key tiles of a part, and how many parts there are.
+struct Parts {
+  int per, count;
+};
+__device__ __forceinline__ Parts parts_of(int limit, int keys, int splits) {
+  const int n = (limit + keys - 1) / keys;
+  const int per = max((n + splits - 1) / splits, kMinPart);
+  return {per, max(1, (n + per - 1) / per)};
 }
 
 // Which request and row tile a workgroup has.
@@ -265,6 +282,8 @@ struct BlockSource {
   int id[kChunks];
   u32x4 k[kChunks], v[kChunks];
   float ks[kChunks], vs[kChunks];
+  enum { kCodes, kNothing, kBad };
+  int what[kChunks];
 
   __device__ __forceinline__ BlockSource(const PromptParams& p_, int request, int h_, int nk_)
       : p(p_), table(p_.table + (int64_t)request * p_.max_blocks), h(h_), nk(nk_) {}
@@ -278,6 +297,7 @@ struct BlockSource {
       id[i] = table[at < p.max_blocks ? at : p.max_blocks - 1];
     }
   }
+  // (What a load brings is not looked at here: that would wait for it.)
   __device__ __forceinline__ void issue(int j) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
@@ -287,9 +307,7 @@ struct BlockSource {
       const int64_t off = ((bh << p.bs_shift) + (key & ((1 << p.bs_shift) - 1))) * p.D + (in ? ch : 0);
       k[i] = *(const u32x4*)(p.kc + off), v[i] = *(const u32x4*)(p.vc + off);
       ks[i] = p.kscale[bh], vs[i] = p.vscale[bh];
-      if (!in || !good) v[i] = (u32x4){0, 0, 0, 0};
-      if (!in) k[i] = (u32x4){0, 0, 0, 0};
-      else if (!good) k[i] = (u32x4){0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};  // NaN: a bad entry shows
+      what[i] = !in ? kNothing : good ? kCodes : kBad;
     }
   }
   template <bool AS_BF>
@@ -318,6 +336,10 @@ struct BlockSource {
       const int a = row * kRowBytes + (((2 * chunk) ^ swizzle<DP>(row)) << 4);
       const int b = row * kRowBytes + (((2 * chunk + 1) ^ swizzle<DP>(row)) << 4);
       u32x4 x, y;
+      if (what[i] != kCodes) {
+        const uint32_t fill = what[i] == kBad ? 0x7f7f7f7fu : 0u;  // NaN: a bad entry shows
+        k[i] = (u32x4){fill, fill, fill, fill}, v[i] = (u32x4){0, 0, 0, 0};
+      }
       convert<BF>(k[i], ks[i], x, y);
       *(u32x4*)(lk + a) = x, *(u32x4*)(lk + b) = y;
       convert<true>(v[i], vs[i], x, y);
@@ -334,8 +356,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
 
-  const int h = (int)(blockIdx.x % p.H);
-  Tile t = find_tile<BM, BLOCKS>(p, blockIdx.x / p.H);
+  const int h = (int)(blockIdx.x % p.H), part = (int)(blockIdx.x / p.H % p.splits);
+  Tile t = find_tile<BM, BLOCKS>(p, blockIdx.x / p.H / p.splits);
   if (t.request < 0) return;
   t.request = uniform(t.request), t.tile = uniform(t.tile), t.rows = uniform(t.rows), t.nq = uniform(t.nq);
   t.nk = uniform(t.nk), t.q0 = uniform((uint32_t)t.q0), t.k0 = uniform((uint32_t)t.k0);
@@ -353,7 +375,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
   };
   const int limit = real ? limit_of(token) : 0;
   const int last_row = min(t.tile * BM + BM, t.rows) - 1;
-  const int tile_limit = uniform(limit_of(last_row / p.G));
+  const Parts parts = parts_of(uniform(limit_of(last_row / p.G)), kKeys, p.splits);
+  if (part >= parts.count) return;
+  const int part_first = part * parts.per * kKeys;
+  const int tile_limit = min(uniform(limit_of(last_row / p.G)), part_first + parts.per * kKeys);
   const int wave_first = min(t.tile * BM + wave * 32, t.rows - 1), wave_last = min(wave_first + 31, t.rows - 1);
   const bool wave_real = t.tile * BM + wave * 32 < t.rows;
   const int wave_min = uniform(limit_of(wave_first / p.G));
@@ -385,7 +410,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
   float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][4]
   if constexpr (!BLOCKS) {
     dense.init(p, t, h);
-    if (tile_limit > 0) dense.issue(0, lds0, lds0 + kTileBytes);
+    if (tile_limit > 0) dense.issue(part_first, lds0, lds0 + kTileBytes);
   }
 
   u32x4 q[KS];
@@ -412,16 +437,16 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
       for (int i = 0; i < 16; ++i) o[cb][i] = 0.f;
     if (tile_limit > 0) {
       if constexpr (BLOCKS) {
-        blocks.blocks(0);
-        blocks.issue(0);
-        blocks.blocks(kKeys);
+        blocks.blocks(part_first);
+        blocks.issue(part_first);
+        blocks.blocks(part_first + kKeys);
         blocks.finish(lds, lds + kTileBytes, lscale);
       } else if (careful) {
-        dense.issue(0, lds0, lds0 + kTileBytes);
+        dense.issue(part_first, lds0, lds0 + kTileBytes);
       }
     }
     int buf = 0;
-    for (int j = 0; j < tile_limit; j += kKeys) {
+    for (int j = part_first; j < tile_limit; j += kKeys) {
       // this wave's copies are done, then everybody's; and everybody has read the other buffer
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const int at = buf * 2 * kTileBytes;
@@ -576,8 +601,22 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
       }
   }
   l += other_half(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   if (!real) return;
+  if (parts.count > 1) {
+    const int64_t at = (int64_t)blockIdx.x * BM + wave * 32 + (lane & 31);
+    if (half == 0) *(f32x2*)(p.stats + 2 * at) = (f32x2){m, l};
+    float* rec = p.records + at * p.D;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ch = 32 * cb + 8 * i + 4 * half;
+        if (ch < p.D)
+          *(f32x4*)(rec + ch) = (f32x4){o[cb][4 * i], o[cb][4 * i + 1], o[cb][4 * i + 2], o[cb][4 * i + 3]};
+      }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   char* dst = (char*)p.o + 2 * (qb * p.o_sb + (t.q0 + token) * p.o_st + head * p.o_sh);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb)
@@ -588,6 +627,80 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
                        pack2<BF>(o[cb][4 * i + 2] * inv, o[cb][4 * i + 3] * inv)};
       if (ch < p.D) *(u32x2*)(dst + 2 * ch) = w;
     }
+}
+
+// Joins the parts' records of a tile: a workgroup has 32 of its rows, a wave one at a time.
+template <int BM, int KEYS, bool BF, bool BLOCKS>
+__global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int sub = (int)(blockIdx.x % (BM / 32)), h = (int)(blockIdx.x / (BM / 32) % p.H);
+  const int64_t index = blockIdx.x / (BM / 32) / p.H;
+  Tile t = find_tile<BM, BLOCKS>(p, index);
+  if (t.request < 0) return;
+  t.request = uniform(t.request), t.tile = uniform(t.tile), t.rows = uniform(t.rows), t.nq = uniform(t.nq);
+  t.nk = uniform(t.nk), t.q0 = uniform((uint32_t)t.q0);
+  t.tile = (t.rows + BM - 1) / BM - 1 - t.tile;
+  const int last_row = min(t.tile * BM + BM, t.rows) - 1;
+  int limit = p.causal ? last_row / p.G + 1 + t.nk - t.nq : t.nk;
+  limit = limit < 0 ? 0 : limit > t.nk ? t.nk : limit;
+  const Parts parts = parts_of(limit, KEYS, p.splits);
+  if (parts.count == 1) return;
+  const int64_t qb = p.q_starts ? 0 : t.request;
+  for (int i = wave; i < 32; i += 4) {
+    const int place = sub * 32 + i, row = t.tile * BM + place;
+    if (row >= t.rows) return;
+    float m = -3.402823466e38f, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int x0 = 0; x0 < parts.count; x0 += 4) {
+      f32x2 ml[4], v[4][2];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int part = x0 + x < parts.count ? x0 + x : x0;
+        const int64_t at = ((index * p.splits + part) * p.H + h) * BM + place;
+        ml[x] = *(const f32x2*)(p.stats + 2 * at);
+        if (x0 + x >= parts.count) ml[x] = (f32x2){-__builtin_inff(), 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int ch = 2 * (lane + 64 * c);
+          v[x][c] = *(const f32x2*)(p.records + at * p.D + (ch < p.D ? ch : 0));
+        }
+      }
+      float up = m;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) up = fmaxf(up, ml[x][0]);
+      const float f0 = __builtin_amdgcn_exp2f(m - up);
+      m = up, l *= f0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] *= f0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (ml[x][1] == 0.f) continue;  // no key seen
+        // (not 0, so that an infinity among the part's values stays one)
+        const float f = fmaxf(__builtin_amdgcn_exp2f(ml[x][0] - up), 1.1754944e-38f);
+        l += ml[x][1] * f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc[2 * c] += v[x][c][0] * f, acc[2 * c + 1] += v[x][c][1] * f;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* dst = (uint16_t*)p.o + qb * p.o_sb + (t.q0 + row / p.G) * p.o_st + (h * p.G + row % p.G) * p.o_sh;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int ch = 2 * (lane + 64 * c);
+      if (ch < p.D) *(uint32_t*)(dst + ch) = pack2<BF>(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+    }
+  }
+}
+
+// Parts for a launch of `grid` workgroups over at most `keys` keys: two on each of 256 CUs, where there would not be one
+// (32 heads x 1,024 tokens are 256 workgroups: 25 us, in two parts 26 and 15 for joining them).
+inline int splits_for(int64_t grid, int64_t keys, int tile_keys) {
+  const int64_t most = (keys + tile_keys * kMinPart - 1) / (tile_keys * kMinPart);
+  int64_t s = grid >= 256 ? 1 : (512 + grid - 1) / (grid < 1 ? 1 : grid);
+  s = s > 16 ? 16 : s;
+  return (int)(s > most ? (most < 1 ? 1 : most) : s);
+}
+inline int64_t record_bytes(int64_t grid, int splits, int rows, int64_t D) {
+  return splits > 1 ? grid * splits * rows * (D + 2) * 4 : 0;
 }
 
 }  // namespace prompt

@@ -16,6 +16,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .attention import _workspace
 
 MAX_PROMPT_HEAD_DIM = 256
 
@@ -77,6 +78,44 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     Softmax statistics and sums are fp32; the weights are rounded to the tensors' type for the second product.
     Forward only: tensors that require gradients are refused outside torch.no_grad().
     """
+    packed = query_starts is not None
+    if packed and key_starts is None:
+        key_starts = query_starts
+    fill = out is None
+    scale = None if scale is None else float(scale)
+    key = None
+    if not packed or (query_starts.dtype == torch.int32 == key_starts.dtype):
+        key = ("prompt", bool(causal), scale, fill, packed,
+               _lib.layouts(query, keys, values, *((query_starts, key_starts) if packed else ()),
+                            *(() if fill else (out,))))
+    known = _lib.template(key) if key is not None else None
+    if known is not None and not (query.data_ptr() | keys.data_ptr() | values.data_ptr()) % 16 \
+            and (fill or not out.data_ptr() % 8):
+        no_gradients("prompt_attention", query, keys, values)
+        if fill:
+            out = torch.empty_like(query)
+        a = _lib.PromptAttentionArgs.from_buffer_copy(known)
+    else:
+        a, query, keys, values, query_starts, key_starts, out, whole = _checked(query, keys, values, query_starts,
+                                                                               key_starts, causal, scale, out)
+        if a is None:
+            return out
+        if whole and key is not None:  # (no copy of an input was made)
+            _lib.keep_template(key, a)
+            a = _lib.PromptAttentionArgs.from_buffer_copy(a)
+    a.query, a.keys, a.values, a.out = query.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr()
+    if packed:
+        a.q_starts, a.k_starts = query_starts.data_ptr(), key_starts.data_ptr()
+    stream = _lib.stream_ptr(query.device)
+    if a.workspace_bytes:
+        a.workspace = _workspace(query.device, a.workspace_bytes, stream).data_ptr()
+    _lib.launch(_lib.load().dkv_prompt_attention, a, query.device, "dkv_prompt_attention", stream)
+    return out
+
+
+def _checked(query, keys, values, query_starts, key_starts, causal, scale, out):
+    """The checks of a call and its arguments without pointers (None where there is nothing to compute)."""
+    packed = query_starts is not None
     _lib.require_device(query, keys, values)
     if query.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("prompt_attention takes bf16 and fp16 tensors")
@@ -85,7 +124,6 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     device = query.device
     if keys.device != device or values.device != device:
         raise ValueError("query, keys and values must be on the same device")
-    packed = query_starts is not None
     if key_starts is not None and not packed:
         raise ValueError("key_starts needs query_starts")
     dims = 3 if packed else 4
@@ -94,7 +132,6 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if keys.shape != values.shape or query.shape[-1] != keys.shape[-1]:
         raise ValueError("query/key/value head_dim, and key/value shapes must be compatible")
     no_gradients("prompt_attention", query, keys, values)
-    # axes: (batch, tokens, heads) of each tensor
     t_axis, h_axis = (0, 1) if packed else (2, 1)
     Hq, Hkv, D = query.shape[h_axis], keys.shape[h_axis], query.shape[-1]
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
@@ -104,30 +141,32 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     if not packed and query.shape[0] != keys.shape[0]:
         raise ValueError("query and keys must have one batch size")
     factor = scale_factor(scale, D, "prompt_attention")
-    fill = out is None
+    fill, whole = out is None, True
     if out is None:
         out = torch.empty_like(query)
-        if out.stride(-1) != 1 or any(s % 4 for s in out.stride()):  # (a query whose own layout is not rows of D)
+        if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]):  # (a query whose layout is not rows of D)
             out = torch.empty(query.shape, dtype=query.dtype, device=device)
+            whole = False
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1 \
             or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
         raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
-    query, keys, values = aligned_rows(query, t_axis), aligned_rows(keys, t_axis), aligned_rows(values, t_axis)
+    given = (query, keys, values)
+    query, keys, values = (aligned_rows(t, t_axis) for t in given)
+    whole = whole and all(a is b for a, b in zip(given, (query, keys, values)))
 
     a = _lib.PromptAttentionArgs()
     if packed:
-        q_starts = int32_vector(query_starts, "query_starts", device)
-        k_starts = q_starts if key_starts is None else int32_vector(key_starts, "key_starts", device)
-        if q_starts.numel() < 2 or k_starts.numel() != q_starts.numel():
+        query_starts = int32_vector(query_starts, "query_starts", device)
+        key_starts = int32_vector(key_starts, "key_starts", device)
+        if query_starts.numel() < 2 or key_starts.numel() != query_starts.numel():
             raise ValueError("query_starts and key_starts must hold one more entry than there are sequences")
-        a.q_starts, a.k_starts = q_starts.data_ptr(), k_starts.data_ptr()
-        a.requests = q_starts.numel() - 1
+        a.requests = query_starts.numel() - 1
     else:
         a.requests = query.shape[0]
         a.q_sb, a.k_sb, a.v_sb, a.o_sb = query.stride(0), keys.stride(0), values.stride(0), out.stride(0)
     if a.requests == 0 or query.numel() == 0:
-        return out
-    a.query, a.keys, a.values, a.out = query.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr()
+        a = None
+        return a, query, keys, values, query_starts, key_starts, out, whole
     a.q_st, a.q_sh = query.stride(t_axis), query.stride(h_axis)
     a.k_st, a.k_sh = keys.stride(t_axis), keys.stride(h_axis)
     a.v_st, a.v_sh = values.stride(t_axis), values.stride(h_axis)
@@ -136,9 +175,10 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     a.q_tokens, a.k_tokens = query.shape[t_axis], keys.shape[t_axis]
     a.dtype = _lib.dtype_code(query.dtype)
     a.scale, a.causal, a.fill = factor, bool(causal), fill
-    with _lib.on_device(device):
-        _lib.check(_lib.load().dkv_prompt_attention(a, _lib.stream_ptr(device)), "dkv_prompt_attention")
-    return out
+    if packed:
+        a.q_starts = query_starts.data_ptr()
+    a.workspace_bytes = _lib.load().dkv_prompt_attention_workspace_bytes(a)
+    return a, query, keys, values, query_starts, key_starts, out, whole
 
 
 __all__ = ["prompt_attention"]

@@ -459,7 +459,10 @@ int64_t dkv_decode_scratch_bytes(void);
  *
  * causal: the last query token sees all nk keys, token i of nq the first
  * i + 1 + nk - nq.  A row that sees no key is 0.  D a multiple of 8 up to 256;
- * rows 16-byte aligned (out: 8).  Forward only.
+ * rows 16-byte aligned (out: 8).  Forward only.  workspace (16-byte aligned):
+ * dkv_prompt_attention_workspace_bytes of the same arguments (pointers apart
+ * from whether there are starts are not looked at), 0 where the keys are not
+ * split; its contents need not be kept.
  *
  * No counterpart in the reference, whose prefill runs the model's attention
  * backend (src/dart/integrations/qwen3.py:85-97).
@@ -476,8 +479,11 @@ typedef struct dkv_prompt_attention_args {
   int64_t dtype;
   double scale;
   int64_t causal, fill;
+  void* workspace;
+  int64_t workspace_bytes;
 } dkv_prompt_attention_args;
 
+int64_t dkv_prompt_attention_workspace_bytes(const dkv_prompt_attention_args* args);
 int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
 
 /*
@@ -557,8 +563,9 @@ int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
  * max_tokens: no request has more new tokens (a request that has more than that
  * may be left out).  Bytes of blocks behind a request's length are not used; a
  * table entry outside [0, blocks) makes the rows that see it NaN.  D a multiple
- * of 16 up to 256.  workspace: dkv_block_attention_workspace_bytes(Hq, Hkv, D,
- * max(1, min(max_tokens, tokens))) bytes; its contents need not be kept.
+ * of 16 up to 256.  workspace (16-byte aligned):
+ * dkv_block_attention_workspace_bytes of the same arguments (pointers are not
+ * looked at); its contents need not be kept.
  */
 typedef struct dkv_block_attention_args {
   const void* query;
@@ -580,7 +587,7 @@ typedef struct dkv_block_attention_args {
   int64_t workspace_bytes;
 } dkv_block_attention_args;
 
-int64_t dkv_block_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_tokens);
+int64_t dkv_block_attention_workspace_bytes(const dkv_block_attention_args* args);
 int dkv_block_attention(const dkv_block_attention_args* args, void* stream);
 
 #ifdef __cplusplus

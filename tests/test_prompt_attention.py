@@ -190,6 +190,24 @@ def test_long_sequence_against_64_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("qn,kn", [([3], [5000]), ([40, 1, 17], [2000, 700, 3001]), ([130], [1030])])
+def test_few_queries_over_many_keys(dtype, D, qn, kn):
+    """The keys come in parts that are joined; infinities in one part, and a part that some rows see nothing of."""
+    import dartkv_amd as dart
+    q = _rand((sum(qn), 4, D), dtype, 1)
+    k, v = _rand((sum(kn), 2, D), dtype, 2), _rand((sum(kn), 2, D), dtype, 3)
+    got = dart.prompt_attention(q, k, v, _starts(qn), _starts(kn))
+    _packed_check(got, q, k, v, qn, kn, True, 1 / math.sqrt(D), dtype)
+    v[5, 0, 3] = float("inf")
+    again = dart.prompt_attention(q, k, v, _starts(qn), _starts(kn))
+    hit = torch.zeros(q.shape, dtype=torch.bool, device=DEV)
+    hit[max(0, 5 - kn[0] + qn[0]):qn[0], :2, 3] = True
+    assert bool((again[hit] == float("inf")).all()) and torch.equal(again[~hit], got[~hit])
+
+
+@pytest.mark.gpu
 def test_out_and_rows_behind_the_last_sequence():
     import dartkv_amd as dart
     q, k, v = (_rand((90, h, 64), torch.bfloat16, h) for h in (4, 2, 2))
