@@ -6,6 +6,11 @@ configured attention on the dense tensors ``DartHFCache.update`` returns; a
 one-token decode calls ``fused_dart_attention`` on the layer's packed cache,
 which runs the HIP split-K page kernels.
 
+``attach_dart_fused_attention(model, prompt_attention=True)`` runs a prefill
+that the model's backend would run as plain causal attention without a mask
+(``sdpa``, bf16 or fp16, no gradients, no sliding window) on
+``prompt_attention`` instead; every other call keeps the backend.
+
 The forward accepts the cache under both keyword names Transformers has used
 (``past_key_values`` in 5.x, ``past_key_value`` in 4.x).
 
@@ -27,6 +32,7 @@ from torch import nn
 
 from .. import _lib
 from ..fused_attention import fused_dart_attention
+from ..prompt import MAX_PROMPT_HEAD_DIM, prompt_attention
 from .huggingface import DartHFCache
 
 
@@ -115,6 +121,18 @@ def _can_prepare(attn: nn.Module, hidden_states: torch.Tensor, cos: torch.Tensor
     return _fused_qkv_weight(attn)
 
 
+def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, attention_mask, kwargs: dict) -> bool:
+    """Whether the backend's attention of these tensors is causal attention of whole prompts: sdpa takes a missing
+    mask for it where there are as many keys as queries."""
+    return (getattr(attn, "dart_prompt_attention", False) and attention_mask is None
+            and attn.config._attn_implementation == "sdpa" and query.device.type == "cuda"
+            and query.shape[-2] == keys.shape[-2] and query.dtype in (torch.bfloat16, torch.float16)
+            and keys.dtype == query.dtype and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_PROMPT_HEAD_DIM
+            and attn.sliding_window is None and not (attn.training and attn.attention_dropout)
+            and kwargs.get("is_causal") in (None, True) and not kwargs.get("output_attentions")
+            and not (torch.is_grad_enabled() and (query.requires_grad or keys.requires_grad)))
+
+
 class DartQwen3Attention:  # replaced by build_dart_qwen3_attention_class()
     """Placeholder; the real class subclasses the installed Qwen3Attention."""
 
@@ -164,6 +182,9 @@ def build_dart_qwen3_attention_class():
                     query_states, cache.layer_for_attention(self.layer_idx), scale=self.scaling, fallback=True,
                 ).transpose(1, 2)
                 attn_weights = None
+            elif _can_run_prompt(self, query_states, key_states, attention_mask, kwargs):
+                attn_output = prompt_attention(query_states, key_states, value_states, scale=self.scaling).transpose(1, 2)
+                attn_weights = None
             else:
                 attention_interface = _attention_interface(modules, self.config)
                 attn_output, attn_weights = attention_interface(
@@ -187,8 +208,9 @@ def build_dart_qwen3_attention_class():
     return _DartQwen3Attention
 
 
-def attach_dart_fused_attention(model: nn.Module) -> nn.Module:
-    """Replace every Qwen3 self-attention module with the Dart adapter."""
+def attach_dart_fused_attention(model: nn.Module, *, prompt_attention: bool = False) -> nn.Module:
+    """Replace every Qwen3 self-attention module with the Dart adapter.  ``prompt_attention``: run prefills on the
+    HIP prompt kernel where it computes what the backend would (results differ by roundings)."""
     attention_class = build_dart_qwen3_attention_class()
     layers = getattr(getattr(model, "model", None), "layers", None)
     if layers is None:
@@ -202,6 +224,7 @@ def attach_dart_fused_attention(model: nn.Module) -> nn.Module:
         replacement.load_state_dict(original.state_dict())
         replacement.train(original.training)
         _share_qkv_storage(replacement)
+        replacement.dart_prompt_attention = prompt_attention
         layer.self_attn = replacement
     return model
 

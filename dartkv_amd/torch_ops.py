@@ -7,7 +7,8 @@ fake implementation gives output shapes and dtypes without touching the GPU
 runs the same C ABI call as the Python API beside it
 (``quantization.quantize``, ``QuantizedTensor.dequantize``,
 ``mixed.quantize_key_mixed``, ``MixedQuantizedKey.dequantize``,
-``attention.decode_attention``); there is no second implementation.
+``attention.decode_attention``, ``prompt.prompt_attention`` and the operators of
+``blocks``); there is no second implementation.
 
 ``decode_attention`` reads a ``DartKVCache``, which is not a tensor: the
 operator takes an integer handle from ``cache_handle(cache)``, valid while the
@@ -25,7 +26,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import attention as _attention
+from . import blocks as _blocks
 from . import mixed as _mixed
+from . import prompt as _prompt
 from . import quantization as _quantization
 from .cache import DartKVCache
 
@@ -162,5 +165,71 @@ def _(query, cache, scale=None):
     return query.new_empty((B, Hq, 1, D))
 
 
-__all__ = ["cache_handle", "decode_attention", "dequantize_key_mixed", "dequantize_rows", "quantize_key_mixed",
-           "quantize_rows"]
+# ---- prompts and block caches (no reference counterpart) ----
+
+@torch.library.custom_op("dartkv::prompt_attention", mutates_args=())
+def prompt_attention(query: Tensor, keys: Tensor, values: Tensor, query_starts: Optional[Tensor] = None,
+                     key_starts: Optional[Tensor] = None, causal: bool = True, scale: Optional[float] = None) -> Tensor:
+    """Attention over whole prompts, a batch [B, H, T, D] or packed [T, H, D] with starts."""
+    return _prompt.prompt_attention(query, keys, values, query_starts, key_starts, causal=causal, scale=scale)
+
+
+@prompt_attention.register_fake
+def _(query, keys, values, query_starts=None, key_starts=None, causal=True, scale=None):
+    return torch.empty_like(query)
+
+
+@torch.library.custom_op("dartkv::reserve_blocks", mutates_args=("table", "lengths", "free", "state"))
+def reserve_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, tokens: Tensor, total: int,
+                   block_size: int) -> Tuple[Tensor, Tensor]:
+    """Slots [total] and starts [requests + 1] of the requests' new tokens; the tables' state moves on."""
+    return _blocks.reserve_blocks(table, lengths, free, state, tokens, total, block_size=block_size)
+
+
+@reserve_blocks.register_fake
+def _(table, lengths, free, state, tokens, total, block_size):
+    return lengths.new_empty((total,), dtype=torch.int64), lengths.new_empty((lengths.shape[0] + 1,))
+
+
+@torch.library.custom_op("dartkv::release_blocks", mutates_args=("table", "lengths", "free", "state"))
+def release_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, tokens: Optional[Tensor],
+                   block_size: int) -> None:
+    """Drop each request's last tokens (None: all)."""
+    _blocks.release_blocks(table, lengths, free, state, tokens, block_size=block_size)
+
+
+@release_blocks.register_fake
+def _(table, lengths, free, state, tokens, block_size):
+    return None
+
+
+@torch.library.custom_op("dartkv::append_blocks",
+                         mutates_args=("key_codes", "value_codes", "key_scale", "value_scale"))
+def append_blocks(keys: Tensor, values: Tensor, slots: Tensor, key_codes: Tensor, value_codes: Tensor,
+                  key_scale: Tensor, value_scale: Tensor) -> None:
+    """New keys and values [T, H, D] into their slots of the e4m3 blocks."""
+    _blocks.append_blocks(keys, values, slots, key_codes, value_codes, key_scale, value_scale)
+
+
+@append_blocks.register_fake
+def _(keys, values, slots, key_codes, value_codes, key_scale, value_scale):
+    return None
+
+
+@torch.library.custom_op("dartkv::block_attention", mutates_args=())
+def block_attention(query: Tensor, key_codes: Tensor, value_codes: Tensor, key_scale: Tensor, value_scale: Tensor,
+                    table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None, max_tokens: Optional[int] = None,
+                    scale: Optional[float] = None) -> Tensor:
+    """Attention [T, Hq, D] of each request's newest tokens over its blocks."""
+    return _blocks.block_attention(query, key_codes, value_codes, key_scale, value_scale, table, lengths, starts,
+                                   max_tokens=max_tokens, scale=scale)
+
+
+@block_attention.register_fake
+def _(query, key_codes, value_codes, key_scale, value_scale, table, lengths, starts=None, max_tokens=None, scale=None):
+    return query.new_empty(query.shape)
+
+
+__all__ = ["append_blocks", "block_attention", "cache_handle", "decode_attention", "dequantize_key_mixed",
+           "dequantize_rows", "prompt_attention", "quantize_key_mixed", "quantize_rows", "release_blocks",
+           "reserve_blocks"]
