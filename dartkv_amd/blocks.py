@@ -213,9 +213,8 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     ``query`` [T, Hq, D] (bf16 or fp16) holds the requests' new tokens one after the other, request r's in rows
     ``starts[r]`` to ``starts[r + 1]`` (``reserve_blocks``; None: one token each); the last is at position
     ``lengths[r] - 1``, so token i of n sees the first ``lengths[r] - n + 1 + i`` keys, and a row that sees none is
-    0.  ``max_tokens``: no request has more new tokens in this call; up to sixteen rows (tokens times query heads
-    per KV head; 64 for head_dim 64, 32 up to 128) that choice alone runs the kernel made for them.  Default: T
-    (without starts 1).
+    0.  ``max_tokens``: no request has more new tokens in this call; where that is at most 64 rows (tokens times
+    query heads per KV head) the kernel for few rows does all of it.  Default: T (without starts 1).
     ``table`` [requests, max_blocks] and ``lengths`` [requests] (int32), the codes and scales as ``append_blocks``
     writes them.  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
     makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request are 0 in

@@ -41,8 +41,9 @@ constexpr int kThreads = 256;
 
 struct BlockParams {
   PromptParams a;
-  float* records;  // [2 * workers][H][rows][D + 2]
+  float* records;  // [2 * workers][H][record_rows][D + 2]
   int32_t workers, rows;  // rows: the most of a request
+  int32_t tile, record_rows;  // rows of a tile (16 NT), and of a record
 };
 
 struct Work {
@@ -50,8 +51,13 @@ struct Work {
   int64_t q0;
 };
 
+__device__ __forceinline__ int key_units(int length) {  // (a request without keys writes zeros)
+  return length ? (length + kUnit - 1) / kUnit : 1;
+}
+
 // A request's new tokens and units (none when it has no rows, or more than this kernel takes).
-__device__ __forceinline__ Work work_of(const PromptParams& p, int r, int most_rows) {
+__device__ __forceinline__ Work work_of(const BlockParams& bp, int r) {
+  const PromptParams& p = bp.a;
   Work w = {0, 0, 0, 0, 0};
   if (r >= p.R) return w;
   int64_t a = r, b = r + 1;
@@ -63,9 +69,9 @@ __device__ __forceinline__ Work work_of(const PromptParams& p, int r, int most_r
   length = length < 0 ? 0 : length > most ? most : length;
   w.q0 = a, w.n = (int)(b - a), w.length = (int)length;
   const int64_t rows = (b - a) * p.G;
-  if (rows > most_rows) return w;
+  if (rows > bp.rows) return w;
   w.rows = (int)rows;
-  if (rows > 0) w.units = length ? (int)((length + kUnit - 1) / kUnit) : 1;  // (a request without keys writes zeros)
+  w.units = (w.rows + bp.tile - 1) / bp.tile * key_units(w.length);
   return w;
 }
 
@@ -134,7 +140,6 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
   const int h = (int)(wave % p.H);
   const int worker = (int)(wave / p.H);
   if (worker >= bp.workers) return;
-  const int most_rows = bp.rows;
   __shared__ int32_t first_nan[kThreads / 64][DP];
   int32_t* first = first_nan[threadIdx.x >> 6];
 
@@ -147,11 +152,11 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
   }
 
   // all units, then the request that this wave's first lies in
-  Work mine = work_of(p, lane, most_rows);
+  Work mine = work_of(bp, lane);
   int scan = wave_scan(mine.units, lane);
   int64_t total = uniform(__shfl(scan, 63, 64));
   for (int b = 64; b < p.R; b += 64) {
-    int x = work_of(p, b + lane, most_rows).units;
+    int x = work_of(bp, b + lane).units;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
     total += uniform(x);
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
     }
     before += uniform(__shfl(scan, 63, 64));
     base += 64;
-    mine = work_of(p, base + lane, most_rows);
+    mine = work_of(bp, base + lane);
     scan = wave_scan(mine.units, lane);
   }
 
@@ -178,31 +183,35 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
     // the request's part in this share (its units are not 0)
     const int r = uniform(base + lane_r);
     const int units = uniform(__shfl(mine.units, lane_r, 64));
-    const int rows = uniform(__shfl(mine.rows, lane_r, 64));
+    const int all_rows = uniform(__shfl(mine.rows, lane_r, 64));
     const int length = uniform(__shfl(mine.length, lane_r, 64));
     const int n = uniform(__shfl(mine.n, lane_r, 64));
     const int64_t q0 = (int64_t)uniform((uint32_t)__shfl((int)mine.q0, lane_r, 64));
     const int64_t start = before + uniform(__shfl(scan, lane_r, 64)) - units;
-    const int u0 = (int)(unit - start);
-    const int u1 = (int)((stop < start + units ? stop : start + units) - start);
+    const int key_units_r = uniform(key_units(length));
+    const int tile = uniform((int)(unit - start) / key_units_r);
+    const int64_t tile_start = start + (int64_t)tile * key_units_r;
+    const int u0 = (int)(unit - tile_start);
+    const int u1 = (int)((stop < tile_start + key_units_r ? stop : tile_start + key_units_r) - tile_start);
+    const int row0 = tile * 16 * NT, rows = min(all_rows - row0, 16 * NT);
     const int nt = NT == 1 ? 1 : (rows + 15) / 16;
 
     u32x4 q[NT][KS];
     int limit[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int row = t * 16 + i16;
+      const int row = row0 + t * 16 + i16;
       const int token = row / p.G, head = h * p.G + row % p.G;
       const char* src = (const char*)p.q + 2 * ((q0 + token) * p.q_st + head * p.q_sh);
-      limit[t] = row < rows ? length - n + 1 + token : 0;
+      limit[t] = row < all_rows ? length - n + 1 + token : 0;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int ch = g * (DP / 4) + s * 8;
         q[t][s] = (u32x4){0, 0, 0, 0};
-        if (row < rows && ch < p.D) q[t][s] = *(const u32x4*)(src + 2 * ch);
+        if (row < all_rows && ch < p.D) q[t][s] = *(const u32x4*)(src + 2 * ch);
       }
     }
-    const int min_limit = length - n + 1;
+    const int min_limit = length - n + 1 + row0 / p.G;
 
     f32x4 o[NT][NB];
     float m[NT], l[NT];
@@ -430,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
     }
 
     // lane (row, g) has channels (4 g + e) * NB + b of its row
-    const bool whole = u0 == 0 && u1 == units;
+    const bool whole = u0 == 0 && u1 == key_units_r;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (NT > 1 && t >= nt) break;
@@ -440,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
       if (row >= rows) continue;
       if (whole) {
         const float inv = l[t] == 0.f ? 0.f : 1.f / l[t];
-        const int token = row / p.G, head = h * p.G + row % p.G;
+        const int token = (row0 + row) / p.G, head = h * p.G + (row0 + row) % p.G;
         uint16_t* dst = (uint16_t*)p.o + (q0 + token) * p.o_st + head * p.o_sh;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -452,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
         }
       } else {
         float* rec = bp.records +
-                     ((((int64_t)worker * 2 + (u0 == 0 ? 1 : 0)) * p.H + h) * bp.rows + row) * (p.D + 2);
+                     ((((int64_t)worker * 2 + (u0 == 0 ? 1 : 0)) * p.H + h) * bp.record_rows + row) * (p.D + 2);
         if (g == 0) rec[0] = m[t], rec[1] = l[t];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -464,14 +473,14 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
       }
     }
 
-    // the next request with units
-    unit = start + u1;
-    if (unit < stop) {
+    // the next tile, or the next request with units
+    unit = tile_start + u1;
+    if (unit < stop && unit == start + units) {
       uint64_t after = lane_r == 63 ? 0 : __ballot(mine.units > 0) >> (lane_r + 1) << (lane_r + 1);
       while (!after) {
         before += uniform(__shfl(scan, 63, 64));
         base += 64;
-        mine = work_of(p, base + lane, most_rows);
+        mine = work_of(bp, base + lane);
         scan = wave_scan(mine.units, lane);
         after = __ballot(mine.units > 0);
       }
@@ -493,11 +502,11 @@ __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
   const int h = (int)(unit % p.H), row = (int)(unit / p.H % bp.rows);
   const int r = (int)(unit / p.H / bp.rows);
   if (r >= p.R) return;
-  const Work w = work_of(p, r, bp.rows);
+  const Work w = work_of(bp, r);
   if (row >= w.rows) return;
   int64_t total = 0, start = 0;
   for (int base = 0; base < p.R; base += 64) {
-    int x = work_of(p, base + lane, bp.rows).units;
+    int x = work_of(bp, base + lane).units;
     int y = base + lane < r ? x : 0;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64), y += __shfl_xor(y, off, 64);
@@ -505,7 +514,9 @@ __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
   }
   const int64_t share = share_of(uniform64(total), bp.workers);
   start = uniform64(start);
-  const int w0 = uniform((int)(start / share)), w1 = uniform((int)((start + w.units - 1) / share));
+  const int key_units_r = uniform(key_units(w.length)), place = row % bp.tile;
+  start += (int64_t)(row / bp.tile) * key_units_r;
+  const int w0 = uniform((int)(start / share)), w1 = uniform((int)((start + key_units_r - 1) / share));
   if (w0 == w1) return;
   float m = -3.402823466e38f, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
   constexpr int kStep = WIDE ? 4 : 1;
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(kThreads) block_merge(BlockParams bp) {
     for (int i = 0; i < kAhead; ++i) {
       const int x = x0 + kStep * i <= w1 ? x0 + kStep * i : x0;
       const int slot = x == w0 ? 1 : 0;  // a part that begins the request, or goes on with it
-      const float* rec = bp.records + ((((int64_t)x * 2 + slot) * p.H + h) * bp.rows + row) * (p.D + 2);
+      const float* rec = bp.records + ((((int64_t)x * 2 + slot) * p.H + h) * bp.record_rows + place) * (p.D + 2);
       rm[i] = x0 + kStep * i <= w1 ? rec[0] : -__builtin_inff(), rl[i] = rec[1];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
@@ -573,7 +584,7 @@ template <int DP, bool BF>
 void launch_decode(const BlockParams& bp, hipStream_t stream) {
   const int64_t waves = (int64_t)bp.workers * bp.a.H;
   const dim3 grid((unsigned)((waves + 3) / 4));
-  if (bp.rows <= 16)
+  if (bp.tile == 16)
     hipLaunchKernelGGL((block_decode<DP, BF, 1>), grid, dim3(kThreads), 0, stream, bp);
   else if constexpr (DP <= 128)
     hipLaunchKernelGGL((block_decode<DP, BF, 2>), grid, dim3(kThreads), 0, stream, bp);
@@ -592,12 +603,9 @@ int workers_for(int64_t H) {
   return (int)(w < 1 ? 1 : w);
 }
 
-// Rows of a request that this kernel takes: all up to what the accumulators leave registers for, else those of at
-// most 16 rows.
-int rows_for(int64_t max_tokens, int64_t G, int64_t D) {
-  const int64_t most = D <= 128 ? 32 : 16;
-  return max_tokens <= most / G ? (int)(max_tokens * G) : 16;
-}
+// Rows of a request that this kernel takes: all up to 64, in tiles of 16 or (two accumulators of 16, which head_dims
+// over 128 leave no registers for) 32 that each read the keys; else those of at most 16 rows.
+int rows_for(int64_t max_tokens, int64_t G) { return max_tokens <= 64 / G ? (int)(max_tokens * G) : 16; }
 
 int64_t most_tokens(const dkv_block_attention_args& a) {
   const int64_t most = a.max_tokens < a.tokens ? a.max_tokens : a.tokens;
@@ -615,7 +623,7 @@ int check_blocks(const dkv_block_attention_args& a) {
   DKV_CHECK(a.requests >= 1 && a.tokens >= 0 && a.blocks >= 1 && a.max_blocks >= 1 && a.max_tokens >= 1,
             DKV_ERR_INVALID, "dkv_block_attention: bad counts");
   DKV_CHECK(a.tokens < (1ll << 31) / (a.Hq / a.Hkv) - 1024 && a.max_blocks < ((1ll << 31) - 1024) / a.block_size &&
-                a.blocks < (1ll << 31) && a.requests < (1 << 24) && a.requests * 32 * a.Hkv < (1ll << 31),
+                a.blocks < (1ll << 31) && a.requests < (1 << 24) && a.requests * 64 * a.Hkv < (1ll << 31),
             DKV_ERR_INVALID, "dkv_block_attention: too many tokens");
   return DKV_OK;
 }
@@ -633,12 +641,14 @@ BlockParams params_of(const dkv_block_attention_args& a) {
   p.kc = a.key_codes, p.vc = a.value_codes, p.kscale = a.key_scale, p.vscale = a.value_scale;
   p.table = a.table, p.lengths = a.lengths, p.blocks = a.blocks, p.max_blocks = (int32_t)a.max_blocks;
   p.bs_shift = __builtin_ctzll((uint64_t)a.block_size);
-  bp.workers = workers_for(a.Hkv), bp.rows = rows_for(most_tokens(a), p.G, p.D);
+  bp.workers = workers_for(a.Hkv), bp.rows = rows_for(most_tokens(a), p.G);
+  bp.tile = bp.rows > 16 && p.D <= 128 ? 32 : 16;
+  bp.record_rows = bp.rows < bp.tile ? bp.rows : bp.tile;
   return bp;
 }
 
 int64_t workspace_of(const dkv_block_attention_args& a, const BlockParams& bp) {
-  const int64_t few = 2 * (int64_t)bp.workers * a.Hkv * bp.rows * (a.D + 2) * 4;
+  const int64_t few = 2 * (int64_t)bp.workers * a.Hkv * bp.record_rows * (a.D + 2) * 4;
   if (most_tokens(a) <= bp.rows / bp.a.G) return few;
   const int64_t many = block_chunks_workspace_bytes(bp.a, a.tokens * bp.a.G, a.dtype == kBF16);
   return few > many ? few : many;  // (one after the other on the stream)
