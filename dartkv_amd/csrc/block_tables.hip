@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = 8190;  // 12 bytes each of 160 KiB of LDS
-constexpr int kSlots = 4;  // of a thread
+constexpr int kSlots = 4;  // of a thread, where there are many
 
 struct TablesParams {
   int32_t *table, *lengths, *free, *state;
@@ -67,12 +67,21 @@ __device__ __forceinline__ Row row_of(const TablesParams& p, int r, int32_t& bad
   return x;
 }
 
-// The last request whose sum (after `shift`) is at most i.
-__device__ __forceinline__ int find(const int64_t* sums, int R, int64_t i, bool tokens) {
+// Prefix sums, of blocks and of tokens; they stop at 2^32 - 1, which is more than any call can have.
+struct Sum {
+  uint32_t blocks, tokens;
+};
+__device__ __forceinline__ Sum operator+(Sum a, Sum b) {
+  return {__builtin_elementwise_add_sat(a.blocks, b.blocks), __builtin_elementwise_add_sat(a.tokens, b.tokens)};
+}
+
+// The last request whose sum is at most i.
+template <bool TOKENS>
+__device__ __forceinline__ int find(const Sum* sums, int R, uint32_t i) {
   int lo = 0, hi = R - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((tokens ? sums[mid] >> 32 : (int64_t)(int32_t)sums[mid]) <= i)
+    if ((TOKENS ? sums[mid].tokens : sums[mid].blocks) <= i)
       lo = mid;
     else
       hi = mid - 1;
@@ -80,52 +89,50 @@ __device__ __forceinline__ int find(const int64_t* sums, int R, int64_t i, bool 
   return lo;
 }
 
-template <bool RESERVE>
+template <bool RESERVE, int SLOTS>  // SLOTS: of a thread
 __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
-  extern __shared__ int64_t sums[];  // [R + 1]: (tokens before) << 32 | blocks before
+  extern __shared__ Sum sums[];                // [R + 1]: before each request
   int32_t* lens = (int32_t*)(sums + p.R + 1);  // [R]: the lengths before
-  __shared__ int64_t wave_sum[2][4];
+  __shared__ Sum wave_sum[2][4];
   __shared__ int32_t flags, last;
-  __shared__ unsigned long long all_tokens, all_blocks;  // the sums' halves may overflow, these do not
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (tid == 0) flags = 0, all_tokens = 0, all_blocks = 0;
+  if (tid == 0) flags = 0;
   const int64_t count = p.state[0];
 
-  int64_t running = 0, my_tokens = 0, my_blocks = 0;
+  Sum running = {0, 0};
   int32_t bad = 0;
   for (int base = 0; base < p.R; base += kThreads) {
     const int r = base + tid;
-    int64_t x = 0;
+    Sum x = {0, 0};
     if (r < p.R) {
       const Row row = row_of<RESERVE>(p, r, bad);
-      x = ((int64_t)row.moved << 32) + row.count;
-      my_tokens += row.moved, my_blocks += row.count;
+      x = {(uint32_t)row.count, (uint32_t)row.moved};
       lens[r] = row.length;
     }
-    int64_t sum = x;
+    Sum sum = x;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int64_t up = __shfl_up(sum, off, 64);
-      if (lane >= off) sum += up;
+      const Sum up = {(uint32_t)__shfl_up((int)sum.blocks, off, 64), (uint32_t)__shfl_up((int)sum.tokens, off, 64)};
+      if (lane >= off) sum = sum + up;
     }
-    int64_t* wsum = wave_sum[base / kThreads & 1];
+    Sum before = {(uint32_t)__shfl_up((int)sum.blocks, 1, 64), (uint32_t)__shfl_up((int)sum.tokens, 1, 64)};
+    if (lane == 0) before = {0, 0};
+    Sum* wsum = wave_sum[base / kThreads & 1];
     if (lane == 63) wsum[wave] = sum;
     __syncthreads();
-    int64_t before = running;
+    before = before + running;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += wsum[w];
-      running += wsum[w];
+      if (w < wave) before = before + wsum[w];
+      running = running + wsum[w];
     }
-    if (r < p.R) sums[r] = before + sum - x;
+    if (r < p.R) sums[r] = before;
   }
   if (tid == 0) sums[p.R] = running;
   if (bad) atomicOr(&flags, bad);
-  if (my_tokens) atomicAdd(&all_tokens, (unsigned long long)my_tokens);
-  if (my_blocks) atomicAdd(&all_blocks, (unsigned long long)my_blocks);
   __syncthreads();
   bad = flags;
-  const int64_t used = (int64_t)all_blocks, moved = (int64_t)all_tokens;
+  const int64_t used = running.blocks, moved = running.tokens;
   if (count < 0 || count > p.blocks) bad |= kNoBlocks;
   if (RESERVE && used > count) bad |= kNoBlocks;
   if (!RESERVE && count + used > p.blocks) bad |= kNoBlocks;
@@ -134,29 +141,30 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   const int64_t me = (int64_t)blockIdx.x * kThreads + tid, all = (int64_t)gridDim.x * kThreads;
 
   if constexpr (RESERVE) {
-    for (int64_t i = me; i <= p.R; i += all) p.starts[i] = fits ? (int32_t)(sums[i] >> 32) : 0;
+    for (int64_t i = me; i <= p.R; i += all) p.starts[i] = fits ? (int32_t)sums[i].tokens : 0;
     const int mask = (1 << p.shift) - 1;
-    for (int64_t at = me * kSlots; at < p.total; at += all * kSlots) {
-      int64_t slot[kSlots];
-      int r = fits && at < moved ? find(sums, p.R, at, true) : 0;
+    for (int64_t at = me * SLOTS; at < p.total; at += all * SLOTS) {
+      int64_t slot[SLOTS];
+      int r = fits && at < moved ? find<true>(sums, p.R, (uint32_t)at) : 0;
 #pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
+      for (int i = 0; i < SLOTS; ++i) {
         slot[i] = -1;
         if (fits && at + i < moved) {
-          while (sums[r + 1] >> 32 <= at + i) ++r;
-          const int64_t position = lens[r] + (at + i - (sums[r] >> 32));
+          if (i > 0)
+            while (sums[r + 1].tokens <= at + i) ++r;
+          const int64_t position = lens[r] + (at + i - sums[r].tokens);
           const int32_t block = (int32_t)(position >> p.shift), old = (int32_t)blocks_of(lens[r], p.shift);
           const int32_t id = block < old ? p.table[(int64_t)r * p.max_blocks + block]
-                                         : p.free[count - 1 - ((int32_t)sums[r] + block - old)];
+                                         : p.free[count - 1 - ((int64_t)sums[r].blocks + block - old)];
           slot[i] = ((int64_t)id << p.shift) + (position & mask);
         }
       }
-      if (at + kSlots <= p.total) {
+      if (SLOTS > 1 && at + SLOTS <= p.total) {
 #pragma unroll
-        for (int i = 0; i < kSlots; i += 2) *(longlong2*)(p.slots + at + i) = make_longlong2(slot[i], slot[i + 1]);
+        for (int i = 0; i + 1 < SLOTS; i += 2) *(longlong2*)(p.slots + at + i) = make_longlong2(slot[i], slot[i + 1]);
       } else {
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i)
+        for (int i = 0; i < SLOTS; ++i)
           if (at + i < p.total) p.slots[at + i] = slot[i];
       }
     }
@@ -164,10 +172,10 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   // the blocks, in the stack's order
   if (fits) {
     for (int64_t i = me; i < used; i += all) {
-      const int r = find(sums, p.R, i, false);
-      const int64_t j = i - (int32_t)sums[r], length = lens[r];
+      const int r = find<false>(sums, p.R, (uint32_t)i);
+      const int64_t j = i - sums[r].blocks, length = lens[r];
       const int64_t old = RESERVE ? blocks_of(length, p.shift)
-                                  : blocks_of(length - ((sums[r + 1] >> 32) - (sums[r] >> 32)), p.shift);
+                                  : blocks_of(length - (int64_t)(sums[r + 1].tokens - sums[r].tokens), p.shift);
       int32_t* entry = p.table + (int64_t)r * p.max_blocks + old + j;
       if constexpr (RESERVE) {
         *entry = p.free[count - 1 - i];
@@ -188,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   }
   if (fits) {
     for (int r = tid; r < p.R; r += kThreads) {
-      const int32_t n = (int32_t)((sums[r + 1] >> 32) - (sums[r] >> 32));
+      const int32_t n = (int32_t)(sums[r + 1].tokens - sums[r].tokens);
       if (n) p.lengths[r] = lens[r] + (RESERVE ? n : -n);
     }
     if constexpr (RESERVE)
@@ -225,10 +233,15 @@ extern "C" int dkv_reserve_blocks(const dkv_block_tables_args* args, void* strea
             "dkv_reserve_blocks: NULL pointer");
   DKV_CHECK(args->total >= 0 && args->total < (1ll << 31), DKV_ERR_INVALID, "dkv_reserve_blocks: bad total");
   DKV_CHECK(((uintptr_t)args->slots & 15) == 0, DKV_ERR_INVALID, "dkv_reserve_blocks: slots must be 16-byte aligned");
-  int64_t groups = (args->total + kSlots * kThreads - 1) / (kSlots * kThreads);
-  groups = groups < 1 ? 1 : groups > 512 ? 512 : groups;
-  hipLaunchKernelGGL(block_tables<true>, dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8,
-                     (hipStream_t)stream, p);
+  const int lds = 12 * p.R + 8;
+  if (args->total <= 4 * kThreads) {
+    const int64_t groups = args->total > kThreads ? (args->total + kThreads - 1) / kThreads : 1;
+    hipLaunchKernelGGL((block_tables<true, 1>), dim3((unsigned)groups), dim3(kThreads), lds, (hipStream_t)stream, p);
+  } else {
+    int64_t groups = (args->total + kSlots * kThreads - 1) / (kSlots * kThreads);
+    groups = groups > 512 ? 512 : groups;
+    hipLaunchKernelGGL((block_tables<true, kSlots>), dim3((unsigned)groups), dim3(kThreads), lds, (hipStream_t)stream, p);
+  }
   return dkv_check_launch("dkv_reserve_blocks");
 }
 
@@ -238,8 +251,7 @@ extern "C" int dkv_release_blocks(const dkv_block_tables_args* args, void* strea
   const int rc = check_tables(*args, "dkv_release_blocks", p);
   if (rc != DKV_OK) return rc;
   int64_t groups = (p.blocks + 4 * kThreads - 1) / (4 * kThreads);  // (at most that many blocks return)
-  groups = groups > 64 ? 64 : groups;
-  hipLaunchKernelGGL(block_tables<false>, dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8,
-                     (hipStream_t)stream, p);
+  groups = groups > 16 ? 16 : groups;
+  hipLaunchKernelGGL((block_tables<false, 1>), dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8, (hipStream_t)stream, p);
   return dkv_check_launch("dkv_release_blocks");
 }
