@@ -69,7 +69,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 // leave no registers for more.
 constexpr int keys_of(int DP, bool split) { return DP <= (split ? 64 : 128) ? 64 : 32; }
 // LDS of a workgroup: two buffers of keys and values, the blocks' scales, the careful pass's first keys.
-constexpr int lds_bytes(int DP, bool split) { return 4 * keys_of(DP, split) * 2 * DP + 32 + 8 * DP; }
+constexpr int lds_bytes(int DP, bool split, int groups) { return 4 * groups * keys_of(DP, split) * 2 * DP + 64 + 8 * DP; }
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -231,9 +231,8 @@ __device__ __forceinline__ void set_apart(char* lv, int j, int32_t* first) {
 }
 
 // Copies of 16-bit keys and values: straight from memory to LDS.
-template <int DP, int WAVES>
+template <int DP, int WAVES, int kKeys>
 struct DenseSource {
-  static constexpr int kKeys = keys_of(DP, false);
   const char *k, *v;
   int64_t kst, vst;  // bytes
   int nk, valid;     // valid: bytes of a row
@@ -272,9 +271,9 @@ struct DenseSource {
 // Keys and values held in e4m3 blocks: read into registers while the tile before is computed, then converted into
 // LDS.  bf16 queries: codes times their scale (exact), fp16 queries: keys as bare fp16 codes (a scaled value may
 // leave fp16's range), whose scale goes to the logits, and values as scaled bf16.
-template <int DP, bool BF, int WAVES>
+template <int DP, bool BF, int WAVES, int kKeys>
 struct BlockSource {
-  static constexpr int kChunks = keys_of(DP, !BF) * DP / 16 / (64 * WAVES);  // 16 codes each, of a thread
+  static constexpr int kChunks = kKeys * DP / 16 / (64 * WAVES);  // 16 codes each, of a thread
   static constexpr int kRowBytes = 2 * DP;
   const PromptParams& p;
   const int32_t* table;
@@ -349,12 +348,16 @@ struct BlockSource {
   }
 };
 
-template <int DP, bool BF, int WAVES, bool BLOCKS>
-__global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 128 ? 2 : 1) prompt_tiles(PromptParams p) {
-  constexpr int BM = 32 * WAVES, KS = DP / 16, CB = DP / 32, kKeys = keys_of(DP, BLOCKS && !BF), T2 = kKeys / 32;
-  constexpr int kRowBytes = 2 * DP, kTileBytes = kKeys * kRowBytes;
+// GROUPS 2: half of the waves have a stage's first kKeys keys, the other half its second for the same rows, and their
+// sums are joined at the end: two waves a SIMD where a launch has no more workgroups than CUs.
+template <int DP, bool BF, int WAVES, bool BLOCKS, int GROUPS>
+__global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1 ? 3 : DP <= 128 ? 2 : 1)
+    prompt_tiles(PromptParams p) {
+  constexpr int BM = 32 * WAVES / GROUPS, KS = DP / 16, CB = DP / 32, kKeys = keys_of(DP, BLOCKS && !BF), T2 = kKeys / 32;
+  constexpr int kStage = GROUPS * kKeys, kRowBytes = 2 * DP, kTileBytes = kStage * kRowBytes;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) % (WAVES / GROUPS), half = lane >> 5;
+  const int group = GROUPS == 1 ? 0 : uniform(threadIdx.x >> 6) / (WAVES / GROUPS);
 
   const int h = (int)(blockIdx.x % p.H), part = (int)(blockIdx.x / p.H % p.splits);
   Tile t = find_tile<BM, BLOCKS>(p, blockIdx.x / p.H / p.splits);
@@ -375,10 +378,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
   };
   const int limit = real ? limit_of(token) : 0;
   const int last_row = min(t.tile * BM + BM, t.rows) - 1;
-  const Parts parts = parts_of(uniform(limit_of(last_row / p.G)), kKeys, p.splits);
+  const Parts parts = parts_of(uniform(limit_of(last_row / p.G)), kStage, p.splits);
   if (part >= parts.count) return;
-  const int part_first = part * parts.per * kKeys;
-  const int tile_limit = min(uniform(limit_of(last_row / p.G)), part_first + parts.per * kKeys);
+  const int part_first = part * parts.per * kStage;
+  const int tile_limit = min(uniform(limit_of(last_row / p.G)), part_first + parts.per * kStage);
   const int wave_first = min(t.tile * BM + wave * 32, t.rows - 1), wave_last = min(wave_first + 31, t.rows - 1);
   const bool wave_real = t.tile * BM + wave * 32 < t.rows;
   const int wave_min = uniform(limit_of(wave_first / p.G));
@@ -405,9 +408,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
   }
   const uint32_t lds0 = uniform((uint32_t)(uintptr_t)(lds_void*)lds);
 
-  DenseSource<DP, WAVES> dense;
-  BlockSource<DP, BF, WAVES> blocks(p, t.request, h, nk);
-  float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][4]
+  DenseSource<DP, WAVES, kStage> dense;
+  BlockSource<DP, BF, WAVES, kStage> blocks(p, t.request, h, nk);
+  float* lscale = (float*)(lds + 4 * kTileBytes);  // [2][8]
   if constexpr (!BLOCKS) {
     dense.init(p, t, h);
     if (tile_limit > 0) dense.issue(part_first, lds0, lds0 + kTileBytes);
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(q[ks]));
   }
-  int32_t* first = (int32_t*)(lds + 4 * kTileBytes + 32);  // [2][DP], of the careful pass
+  int32_t* first = (int32_t*)(lds + 4 * kTileBytes + 64);  // [2][DP], of the careful pass
   bool careful = false;  // (the same for the whole workgroup)
   for (;;) {
     m = -3.402823466e38f, l = 0.f;
@@ -439,36 +442,37 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
       if constexpr (BLOCKS) {
         blocks.blocks(part_first);
         blocks.issue(part_first);
-        blocks.blocks(part_first + kKeys);
+        blocks.blocks(part_first + kStage);
         blocks.finish(lds, lds + kTileBytes, lscale);
       } else if (careful) {
         dense.issue(part_first, lds0, lds0 + kTileBytes);
       }
     }
     int buf = 0;
-    for (int j = part_first; j < tile_limit; j += kKeys) {
+    for (int j = part_first; j < tile_limit; j += kStage) {
       // this wave's copies are done, then everybody's; and everybody has read the other buffer
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const int at = buf * 2 * kTileBytes;
-      const float* ls = lscale + 4 * buf;
+      const float* ls = lscale + 8 * buf + 4 * group;
       buf ^= 1;
       const int next = buf * 2 * kTileBytes;
-      const bool more = j + kKeys < tile_limit;
+      const bool more = j + kStage < tile_limit;
+      const int jg = j + group * kKeys;  // this wave's keys
       if (more) {
         if constexpr (BLOCKS) {
-          blocks.issue(j + kKeys);
-          blocks.blocks(j + 2 * kKeys);
+          blocks.issue(j + kStage);
+          blocks.blocks(j + 2 * kStage);
         } else {
-          dense.issue(j + kKeys, lds0 + next, lds0 + next + kTileBytes);
+          dense.issue(j + kStage, lds0 + next, lds0 + next + kTileBytes);
         }
       }
       if (careful) {
-        set_apart<DP, kKeys, BF || BLOCKS, 64 * WAVES>(lds + at + kTileBytes, j, first);
+        set_apart<DP, kStage, BF || BLOCKS, 64 * WAVES>(lds + at + kTileBytes, j, first);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       }
-      if (j < wave_max) {
-      const char* lk = lds + at;
-      const char* lv = lds + at + kTileBytes;
+      if (jg < wave_max) {
+      const char* lk = lds + at + group * kKeys * kRowBytes;
+      const char* lv = lk + kTileBytes;
 
       f32x16 s[T2];
 #pragma unroll
@@ -496,12 +500,12 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[t2][i] *= ls[2 * t2 + i / 8];
       }
-      if (j + kKeys > wave_min) {
+      if (jg + kKeys > wave_min) {
 #pragma unroll
         for (int t2 = 0; t2 < T2; ++t2)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (j + 32 * t2 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[t2][i] = -__builtin_inff();
+            if (jg + 32 * t2 + 8 * (i / 4) + 4 * half + i % 4 >= limit) s[t2][i] = -__builtin_inff();
       }
       float top = s[0][0];  // of this lane's half of the row's keys
 #pragma unroll
@@ -577,7 +581,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
       }
       }
       if constexpr (BLOCKS)
-        if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 4 * buf);
+        if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 8 * buf);
     }
     if (careful || !p.causal) break;
     float zero = 0.f;
@@ -590,6 +594,27 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS ? 3 : DP <= 12
     for (int i = threadIdx.x; i < 2 * DP; i += 64 * WAVES) first[i] = 0x7fffffff;
   }
 
+  if constexpr (GROUPS == 2) {
+    // the second group's sums through LDS (its stages are no longer used), a register of all lanes at a time
+    float* other = (float*)lds + wave * 64 * (16 * CB + 2) + lane;
+    __syncthreads();
+    if (group == 1) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) other[64 * (16 * cb + i)] = o[cb][i];
+      other[64 * 16 * CB] = m, other[64 * (16 * CB + 1)] = l;
+    }
+    __syncthreads();
+    if (group == 1) return;
+    const float m1 = other[64 * 16 * CB], up = fmaxf(m, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m - up), f1 = __builtin_amdgcn_exp2f(m1 - up);
+    m = up, l = l * f0 + other[64 * (16 * CB + 1)] * f1;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[cb][i] = o[cb][i] * f0 + other[64 * (16 * cb + i)] * f1;
+  }
   if (careful) {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)

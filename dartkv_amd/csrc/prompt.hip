@@ -6,41 +6,47 @@ using namespace dkv;
 
 namespace {
 
-template <int DP, bool BF, int WAVES>
+template <int DP, bool BF, int WAVES, int GROUPS>
 int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false>), dim3((unsigned)(grid * p.splits)), dim3(64 * WAVES),
-                     prompt::lds_bytes(DP, false), stream, p);
+  constexpr int keys = GROUPS * prompt::keys_of(DP, false), rows = 32 * WAVES / GROUPS;
+  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false, GROUPS>), dim3((unsigned)(grid * p.splits)),
+                     dim3(64 * WAVES), prompt::lds_bytes(DP, false, GROUPS), stream, p);
   if (p.splits > 1)
-    hipLaunchKernelGGL((prompt::prompt_merge<32 * WAVES, prompt::keys_of(DP, false), BF, false>),
-                       dim3((unsigned)(grid * WAVES)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((prompt::prompt_merge<rows, keys, BF, false>), dim3((unsigned)(grid * (rows / 32))), dim3(256), 0,
+                       stream, p);
   return dkv_check_launch("dkv_prompt_attention");
 }
 
-template <bool BF>
-int launch_dim(const PromptParams& p, int waves, int64_t grid, hipStream_t stream) {
-  // Eight waves share each tile's copies in LDS where there are tiles enough (16,384 tokens: 1.96 ms, four waves 1.99);
-  // head_dim 64 gains more from three waves a SIMD (fp16, six heads a KV head: 179 us, eight waves 207), and over 128
-  // the accumulators leave one.
-  if (p.D <= 64) return launch<64, BF, 4>(p, grid, stream);
-  if (p.D > 128) return launch<256, BF, 4>(p, grid, stream);
-  return waves == 8 ? launch<128, BF, 8>(p, grid, stream) : launch<128, BF, 4>(p, grid, stream);
-}
-
 struct Plan {
-  int waves, splits;
+  int waves, groups, splits;
   int64_t grid;  // workgroups of one part
+  int rows() const { return 32 * waves / groups; }
 };
 
+template <bool BF>
+int launch_dim(const PromptParams& p, const Plan& plan, hipStream_t stream) {
+  if (p.D > 128) return launch<256, BF, 4, 1>(p, plan.grid, stream);
+  if (p.D <= 64)
+    return plan.groups == 2 ? launch<64, BF, 8, 2>(p, plan.grid, stream) : launch<64, BF, 4, 1>(p, plan.grid, stream);
+  if (plan.groups == 2) return launch<128, BF, 8, 2>(p, plan.grid, stream);
+  return plan.waves == 8 ? launch<128, BF, 8, 1>(p, plan.grid, stream) : launch<128, BF, 4, 1>(p, plan.grid, stream);
+}
+
+// Eight waves share each tile's copies in LDS where there are tiles enough (16,384 tokens: 1.96 ms, four waves 1.99);
+// head_dim 64 gains more from three waves a SIMD (fp16, six heads a KV head: 179 us, eight waves 207), and over 128 the
+// accumulators leave one.  No more workgroups of 128 rows than CUs: eight waves in two groups.
 Plan plan_of(const dkv_prompt_attention_args& a) {
   const int64_t G = a.Hq / a.Hkv;
   auto grid_of = [&](int64_t bm) {
     if (!a.q_starts) return a.requests * ((a.q_tokens * G + bm - 1) / bm) * a.Hkv;
     return ((a.q_tokens * G + bm - 1) / bm + a.requests + 1) * a.Hkv;
   };
-  Plan plan;
-  plan.waves = a.D > 64 && a.D <= 128 && grid_of(256) >= 512 ? 8 : 4;
-  plan.grid = grid_of(32 * plan.waves);
-  plan.splits = prompt::splits_for(plan.grid, a.k_tokens, prompt::keys_of(a.D <= 128 ? 128 : 256, false));
+  Plan plan = {4, 1, 1, grid_of(128)};
+  if (a.D <= 128 && plan.grid <= 256)
+    plan.waves = 8, plan.groups = 2;
+  else if (a.D > 64 && a.D <= 128 && grid_of(256) >= 512)
+    plan.waves = 8, plan.grid = grid_of(256);
+  plan.splits = prompt::splits_for(plan.grid, a.k_tokens, plan.groups * prompt::keys_of(a.D <= 128 ? 128 : 256, false));
   return plan;
 }
 
@@ -63,7 +69,7 @@ int check_prompt(const dkv_prompt_attention_args& a) {
 extern "C" int64_t dkv_prompt_attention_workspace_bytes(const dkv_prompt_attention_args* args) {
   if (!args || check_prompt(*args) != DKV_OK) return 0;
   const Plan plan = plan_of(*args);
-  return prompt::record_bytes(plan.grid, plan.splits, 32 * plan.waves, args->D);
+  return prompt::record_bytes(plan.grid, plan.splits, plan.rows(), args->D);
 }
 
 extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream) {
@@ -99,11 +105,11 @@ extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void*
   p.splits = plan.splits;
   if (plan.splits > 1) {
     DKV_CHECK(a.workspace && ((uintptr_t)a.workspace & 15) == 0 &&
-                  a.workspace_bytes >= prompt::record_bytes(plan.grid, plan.splits, 32 * plan.waves, a.D),
+                  a.workspace_bytes >= prompt::record_bytes(plan.grid, plan.splits, plan.rows(), a.D),
               DKV_ERR_INVALID, "dkv_prompt_attention: workspace too small");
     p.records = (float*)a.workspace;
-    p.stats = p.records + plan.grid * plan.splits * 32 * plan.waves * a.D;
+    p.stats = p.records + plan.grid * plan.splits * plan.rows() * a.D;
   }
-  return a.dtype == kBF16 ? launch_dim<true>(p, plan.waves, plan.grid, (hipStream_t)stream)
-                          : launch_dim<false>(p, plan.waves, plan.grid, (hipStream_t)stream);
+  return a.dtype == kBF16 ? launch_dim<true>(p, plan, (hipStream_t)stream)
+                          : launch_dim<false>(p, plan, (hipStream_t)stream);
 }
