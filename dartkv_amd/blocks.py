@@ -214,7 +214,8 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     ``starts[r]`` to ``starts[r + 1]`` (``reserve_blocks``; None: one token each); the last is at position
     ``lengths[r] - 1``, so token i of n sees the first ``lengths[r] - n + 1 + i`` keys, and a row that sees none is
     0.  ``max_tokens``: no request has more new tokens in this call; where that is at most 64 rows (tokens times
-    query heads per KV head) the kernel for few rows does all of it.  Default: T (without starts 1).
+    query heads per KV head) the kernel for few rows does all of it, and the output rows of a request that has
+    more after all are undefined.  Default: T (without starts 1).
     ``table`` [requests, max_blocks] and ``lengths`` [requests] (int32), the codes and scales as ``append_blocks``
     writes them.  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
     makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request are 0 in
@@ -314,11 +315,13 @@ def _checked_attention(query, key_codes, value_codes, key_scale, value_scale, ta
 
 
 class BlockPlan(NamedTuple):
-    """Where a step's new tokens go: ``reserve_blocks``' slots and starts, and the most tokens of a request."""
+    """Where a step's new tokens go: ``reserve_blocks``' slots and starts, the most tokens of a request, and the
+    cache's step that they belong to."""
 
     slots: torch.Tensor
     starts: torch.Tensor
     max_tokens: int
+    step: int
 
 
 class BlockKVCache:
@@ -355,19 +358,28 @@ class BlockKVCache:
         self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
         self.state = torch.tensor([blocks, 0, 0, 0], dtype=torch.int32, device=device)
         self.nonfinite = torch.zeros(1, dtype=torch.int32, device=device)
+        self._step = 0
+
+    def _check_plan(self, plan: BlockPlan) -> None:
+        if plan.step != self._step:
+            raise ValueError("the plan is of an earlier reserve: the requests' lengths have moved on")
 
     def reserve(self, tokens: torch.Tensor, total: int, *, max_tokens: Optional[int] = None) -> BlockPlan:
-        """Room for ``tokens[r]`` new tokens of each request (``reserve_blocks``)."""
+        """Room for ``tokens[r]`` new tokens of each request (``reserve_blocks``).  ``max_tokens``: the most of
+        them, where the caller knows it; a request with more is left out of ``attention``."""
         slots, starts = reserve_blocks(self.table, self.lengths, self.free, self.state, tokens, total,
                                        block_size=self.block_size)
-        return BlockPlan(slots, starts, max(1, total if max_tokens is None else max_tokens))
+        self._step += 1
+        return BlockPlan(slots, starts, max(1, total if max_tokens is None else max_tokens), self._step)
 
     def release(self, tokens: Optional[torch.Tensor] = None) -> None:
         """Drop each request's last ``tokens[r]`` tokens, or everything (``release_blocks``)."""
         release_blocks(self.table, self.lengths, self.free, self.state, tokens, block_size=self.block_size)
+        self._step += 1
 
     def append(self, layer: int, keys: torch.Tensor, values: torch.Tensor, plan: BlockPlan) -> None:
         """The step's new ``keys`` and ``values`` [T, kv_heads, head_dim] of one layer (``append_blocks``)."""
+        self._check_plan(plan)
         append_blocks(keys, values, plan.slots, self.key_codes[layer], self.value_codes[layer], self.key_scale[layer],
                       self.value_scale[layer], nonfinite=self.nonfinite)
 
@@ -375,6 +387,7 @@ class BlockKVCache:
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of the step's ``query`` [T, heads, head_dim] over one layer's blocks (``block_attention``),
         after the layer's ``append`` and before the next ``reserve`` or ``release``."""
+        self._check_plan(plan)
         return block_attention(query, self.key_codes[layer], self.value_codes[layer], self.key_scale[layer],
                                self.value_scale[layer], self.table, self.lengths, plan.starts,
                                max_tokens=plan.max_tokens, scale=scale, out=out)

@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
     }
     before += uniform(__shfl(scan, 63, 64));
     base += 64;
+    if (base >= p.R) return;  // (lengths beyond what any pool holds)
     mine = work_of(bp, base + lane);
     scan = wave_scan(mine.units, lane);
   }
@@ -480,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
       while (!after) {
         before += uniform(__shfl(scan, 63, 64));
         base += 64;
+        if (base >= p.R) return;
         mine = work_of(bp, base + lane);
         scan = wave_scan(mine.units, lane);
         after = __ballot(mine.units > 0);

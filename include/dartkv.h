@@ -560,8 +560,8 @@ int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
  * one token each), the last of them at position lengths[r] - 1, so token i of n
  * sees the first lengths[r] - n + 1 + i keys.  A row that sees no key is 0.
  * fill: rows behind starts[requests] become 0 (0: they are left as they were).
- * max_tokens: no request has more new tokens (a request that has more than that
- * may be left out).  Bytes of blocks behind a request's length are not used; a
+ * max_tokens: no request has more new tokens (the rows of a request that has
+ * more are undefined).  Bytes of blocks behind a request's length are not used; a
  * table entry outside [0, blocks) makes the rows that see it NaN.  D a multiple
  * of 16 up to 256.  workspace (16-byte aligned):
  * dkv_block_attention_workspace_bytes of the same arguments (pointers are not

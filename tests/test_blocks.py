@@ -559,6 +559,54 @@ def test_check_reports_and_clears():
     cache.check()
 
 
+@pytest.mark.gpu
+def test_plans_of_earlier_steps_are_refused():
+    import dartkv_amd as dart
+    cache = dart.BlockKVCache(2, 8, 1, 64, block_size=16)
+    x = torch.ones(2, 1, 64, dtype=torch.bfloat16, device=DEV)
+    one = torch.ones(2, dtype=torch.int32, device=DEV)
+    plan = cache.reserve(one, 2)
+    cache.append(0, x, x, plan)
+    cache.append(0, x, x, plan)  # (again: the same tokens)
+    assert torch.equal(cache.attention(0, x, plan), x)
+    cache.release(one)
+    for call in (lambda: cache.append(0, x, x, plan), lambda: cache.attention(0, x, plan)):
+        with pytest.raises(ValueError, match="earlier"):
+            call()
+    new = cache.reserve(one, 2)
+    with pytest.raises(ValueError, match="earlier"):
+        cache.append(0, x, x, plan)
+    cache.append(0, x, x, new)
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_two_streams_at_once():
+    """Two captured calls that need workspaces, replayed on two streams at once, and eager calls beside them."""
+    import dartkv_amd as dart
+    calls = []
+    for seed in (1, 2):
+        cache = _cache([4000, 3000], 2, 128, 64, seed)
+        q = _query(2, 8, 128, torch.bfloat16, seed)
+        calls.append((q, cache, dart.block_attention(q, *cache)))
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for q, cache, _ in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(dart.block_attention(q, *cache))
+        graphs.append(graph)
+    for _ in range(10):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [dart.block_attention(q, *cache) for q, cache, _ in calls]
+        torch.cuda.synchronize()
+        for got, again, (_, _, want) in zip(outs, eager, calls):
+            assert torch.equal(got, want) and torch.equal(again, want)
+
+
 # ---- refusals ----
 
 @pytest.mark.gpu
