@@ -18,8 +18,14 @@
 // ds_read_b64_tr_b16: V stays in token order in LDS.
 //
 // LDS.  Rows of 2 DP bytes in chunks of 16, chunk c of row r at c ^ swizzle(r): sixteen consecutive rows' reads
-// of one chunk (K) and four consecutive rows' reads of four chunks (V) fall in different banks.  Two buffers of
-// 64 keys; the next tile's copies are in flight while a tile is computed (one barrier per tile).
+// of one chunk (K) and four consecutive rows' reads of four chunks (V) fall in different banks (no conflicts counted).
+// Two buffers of 64 keys (32 where registers are short); the next tile's copies are in flight while a tile is computed,
+// one barrier a tile.
+//
+// Bound and measured.  16,384 tokens of 32 query heads of 128, bf16: 1.96-2.0 ms, 1.1 PFLOP/s.  The matrix units are busy
+// 54 % of the cycles, at 1.65 GHz: the power limit holds the clock down as the kernel gets denser (1.77 GHz at 48 %; a
+// 16,384^3 matrix product reaches 1.37 PFLOP/s).  LDS 27 % busy.  A single short prompt is bound by its longest tile and
+// about 8 us of start and end.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
