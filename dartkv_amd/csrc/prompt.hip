@@ -32,9 +32,11 @@ int launch_dim(const PromptParams& p, const Plan& plan, hipStream_t stream) {
   return plan.waves == 8 ? launch<128, BF, 8, 1>(p, plan.grid, stream) : launch<128, BF, 4, 1>(p, plan.grid, stream);
 }
 
-// Eight waves share each tile's copies in LDS where there are tiles enough (16,384 tokens: 1.96 ms, four waves 1.99);
-// head_dim 64 gains more from three waves a SIMD (fp16, six heads a KV head: 179 us, eight waves 207), and over 128 the
-// accumulators leave one.  No more workgroups of 128 rows than CUs: eight waves in two groups.
+// Eight waves share each tile's copies in LDS for long sequences (one of 16,384 tokens: 1.99 ms, four waves 2.03); with
+// shorter ones two workgroups of four on a CU hide each other's start and end (16 of 64 to 4,096: 920 us, eight waves
+// 937; one of 6,464, six heads a KV head: 274 and 284).  head_dim 64 gains more from three waves a SIMD (fp16, six heads
+// a KV head: 179 us, eight waves 207), and over 128 the accumulators leave one.  No more workgroups of 128 rows than CUs:
+// eight waves in two groups (one of 1,024 tokens: 22.6 us, one group 25.2).
 Plan plan_of(const dkv_prompt_attention_args& a) {
   const int64_t G = a.Hq / a.Hkv;
   auto grid_of = [&](int64_t bm) {
@@ -44,7 +46,7 @@ Plan plan_of(const dkv_prompt_attention_args& a) {
   Plan plan = {4, 1, 1, grid_of(128)};
   if (a.D <= 128 && plan.grid <= 256)
     plan.waves = 8, plan.groups = 2;
-  else if (a.D > 64 && a.D <= 128 && grid_of(256) >= 512)
+  else if (a.D > 64 && a.D <= 128 && grid_of(256) >= 512 && (a.q_starts ? a.q_tokens / a.requests : a.q_tokens) >= 8192)
     plan.waves = 8, plan.grid = grid_of(256);
   plan.splits = prompt::splits_for(plan.grid, a.k_tokens, plan.groups * prompt::keys_of(a.D <= 128 ? 128 : 256, false));
   return plan;

@@ -542,6 +542,38 @@ def test_serving_loop(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompts_then_tokens(dtype):
+    """Packed prompts attended in 16 bits while they go into the blocks, then tokens over the blocks: the prompts'
+    results against 64 bits over what was given, the tokens' over the codes, which are within half a step of it."""
+    import dartkv_amd as dart
+    from tests.test_prompt_attention import _packed_check
+    H, G, D, lengths = 2, 3, 128, [70, 1, 333]
+    total = sum(lengths)
+    cache = dart.BlockKVCache(3, 16, H, D, block_size=64)
+    k, v = (torch.randn(total, H, D, generator=torch.Generator().manual_seed(i)).to(dtype).to(DEV) for i in (1, 2))
+    q = _query(total, H * G, D, dtype, 3)
+    plan = cache.reserve(torch.tensor(lengths, device=DEV), total)
+    cache.append(0, k, v, plan)
+    _packed_check(dart.prompt_attention(q, k, v, plan.starts), q, k, v, lengths, lengths, True, D ** -0.5, dtype)
+    view = [cache.key_codes[0], cache.value_codes[0], cache.key_scale[0], cache.value_scale[0], cache.table, cache.lengths]
+    at = 0
+    for r, n in enumerate(lengths):
+        for x, got in zip((k, v), _dense(view, r)):
+            x = x[at:at + n].double().cpu()
+            assert bool(((got - x).abs() <= torch.maximum(x.abs() * 2 ** -4, torch.tensor(2.0 ** -16))).all())
+        at += n
+    _check_attention(cache.attention(0, q, plan), q, view, lengths, dtype, chunk=True)
+    for step in range(3):
+        plan = cache.reserve(torch.ones(3, dtype=torch.int32, device=DEV), 3, max_tokens=1)
+        k, v = (torch.randn(3, H, D, generator=torch.Generator().manual_seed(9 + step + i)).to(dtype).to(DEV) for i in (0, 50))
+        q = _query(3, H * G, D, dtype, step)
+        cache.append(0, k, v, plan)
+        _check_attention(cache.attention(0, q, plan), q, view, [1] * 3, dtype)
+    cache.check()
+
+
+@pytest.mark.gpu
 def test_check_reports_and_clears():
     import dartkv_amd as dart
     cache = dart.BlockKVCache(2, 4, 1, 64, block_size=16)

@@ -178,10 +178,10 @@ def test_keys_that_a_row_does_not_see_do_not_reach_it(dtype, D, lengths, causal)
 def test_long_sequence_against_64_bits():
     """Many tiles with eight waves a workgroup: rows of the beginning, the middle and the end."""
     import dartkv_amd as dart
-    n, Hq, Hkv, D = 5003, 32, 8, 128
+    n, Hq, Hkv, D = 9003, 32, 8, 128
     q, k, v = (_rand((n, h, D), torch.bfloat16, h + i) for i, h in enumerate((Hq, Hkv, Hkv)))
     got = dart.prompt_attention(q, k, v, _starts([n]))
-    for i in (0, 1, 63, 64, 1000, 2047, 2500, 4095, 5002):
+    for i in (0, 1, 63, 64, 1000, 2047, 2500, 4095, 5002, 8191, 9002):
         s = torch.einsum("hgd,jhd->hgj", q[i].double().cpu().view(Hkv, 4, D), k[:i + 1].double().cpu()) / math.sqrt(D)
         p = torch.softmax(s, -1)
         o = torch.einsum("hgj,jhd->hgd", p, v[:i + 1].double().cpu()).reshape(Hq, D)
