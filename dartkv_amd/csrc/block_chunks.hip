@@ -31,7 +31,7 @@ template <int DP, bool BF, int WAVES, int GROUPS>
 void launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
   constexpr int keys = GROUPS * prompt::keys_of(DP, !BF), rows = 32 * WAVES / GROUPS;
   hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, true, GROUPS>), dim3((unsigned)(grid * p.splits)),
-                     dim3(64 * WAVES), prompt::lds_bytes(DP, !BF, GROUPS), stream, p);
+                     dim3(64 * WAVES), prompt::lds_bytes(DP, prompt::keys_of(DP, !BF), GROUPS), stream, p);
   if (p.splits > 1)
     hipLaunchKernelGGL((prompt::prompt_merge<rows, keys, BF, true>), dim3((unsigned)(grid * (rows / 32))), dim3(256), 0,
                        stream, p);

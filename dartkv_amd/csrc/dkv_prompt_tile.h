@@ -50,9 +50,10 @@ struct PromptParams {
   int64_t blocks;
   int32_t max_blocks, bs_shift;
   int32_t skip_rows;  // requests of at most this many rows are another kernel's
-  // A tile's keys in up to `splits` parts of at least kMinPart key tiles, where there are few tiles: each part leaves a
+  // A tile's keys in up to `splits` parts of at least kMinPart key tiles, where there are few workgroups: each leaves a
   // record, o [BM][D] and (m, l) [BM], that prompt_merge joins.
   int32_t splits;
+  int32_t pairs;  // two workgroups share a CU: the second half of a request's tiles are its shortest, shortest first
   float *records, *stats;
 };
 
@@ -75,7 +76,7 @@ typedef __attribute__((address_space(3))) void lds_void;
 // leave no registers for more.
 constexpr int keys_of(int DP, bool split) { return DP <= (split ? 64 : 128) ? 64 : 32; }
 // LDS of a workgroup: two buffers of keys and values, the blocks' scales, the careful pass's first keys.
-constexpr int lds_bytes(int DP, bool split, int groups) { return 4 * groups * keys_of(DP, split) * 2 * DP + 64 + 8 * DP; }
+constexpr int lds_bytes(int DP, int keys, int groups) { return 4 * groups * keys * 2 * DP + 64 + 8 * DP; }
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -157,10 +158,11 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
   const int64_t most = (int64_t)p.max_blocks << p.bs_shift;
   if (!p.q_starts) {
     const int rows = (int)p.q_tokens * p.G, tiles = (rows + BM - 1) / BM;
-    const int r = (int)(index / tiles);
-    if (r >= p.R) return t;
+    const bool across = p.pairs;  // every request's longest tiles first
+    if (index >= (int64_t)tiles * p.R) return t;
+    const int r = (int)(across ? index % p.R : index / tiles);
     const int nk = BLOCKS ? (int)clamped(p.lengths[r], 0, most) : (int)p.k_tokens;
-    t = {r, (int)(index - (int64_t)r * tiles), rows, (int)p.q_tokens, nk, 0, 0};
+    t = {r, (int)(across ? index / p.R : index - (int64_t)r * tiles), rows, (int)p.q_tokens, nk, 0, 0};
     return t;
   }
   int64_t before = 0;
@@ -355,11 +357,11 @@ struct BlockSource {
 };
 
 // GROUPS 2: half of the waves have a stage's first kKeys keys, the other half its second for the same rows, and their
-// sums are joined at the end: two waves a SIMD where a launch has no more workgroups than CUs.
-template <int DP, bool BF, int WAVES, bool BLOCKS, int GROUPS>
+// sums are joined at the end: two waves a SIMD where a launch has no more workgroups than CUs.  KEYS: keys of a tile.
+template <int DP, bool BF, int WAVES, bool BLOCKS, int GROUPS, int KEYS = keys_of(DP, BLOCKS && !BF)>
 __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1 ? 3 : DP <= 128 ? 2 : 1)
     prompt_tiles(PromptParams p) {
-  constexpr int BM = 32 * WAVES / GROUPS, KS = DP / 16, CB = DP / 32, kKeys = keys_of(DP, BLOCKS && !BF), T2 = kKeys / 32;
+  constexpr int BM = 32 * WAVES / GROUPS, KS = DP / 16, CB = DP / 32, kKeys = KEYS, T2 = kKeys / 32;
   constexpr int kStage = GROUPS * kKeys, kRowBytes = 2 * DP, kTileBytes = kStage * kRowBytes;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // K, V, K, V
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) % (WAVES / GROUPS), half = lane >> 5;
@@ -370,7 +372,10 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
   if (t.request < 0) return;
   t.request = uniform(t.request), t.tile = uniform(t.tile), t.rows = uniform(t.rows), t.nq = uniform(t.nq);
   t.nk = uniform(t.nk), t.q0 = uniform((uint32_t)t.q0), t.k0 = uniform((uint32_t)t.k0);
-  t.tile = (t.rows + BM - 1) / BM - 1 - t.tile;  // the longest tiles first
+  {
+    const int tiles = (t.rows + BM - 1) / BM, late = t.tile - (tiles + 1) / 2;
+    t.tile = p.pairs && late >= 0 ? late : tiles - 1 - t.tile;  // the longest tiles first
+  }
   const int nk = t.nk;
 
   // this lane's row, how many keys it sees, and its query in the products' operand layout
@@ -722,13 +727,19 @@ __global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
   }
 }
 
-// Parts for a launch of `grid` workgroups over at most `keys` keys: two on each of 256 CUs, where there would not be one
-// (32 heads x 1,024 tokens are 256 workgroups: 25 us, in two parts 26 and 15 for joining them).
+// Parts for a launch of `grid` workgroups over at most `keys` keys, where not every one of 256 CUs has a workgroup: the
+// least time in tiles, where a workgroup's start and end cost about as much as four and joining the parts as eight.
+// (Always two workgroups a CU is worse where one round becomes two or three: 2,000 tokens of 16 heads, all seeing all,
+// 252 workgroups, 40 us and 66; 300 tokens behind 7,892, head_dim 64, 50 and 71.)
 inline int splits_for(int64_t grid, int64_t keys, int tile_keys) {
-  const int64_t most = (keys + tile_keys * kMinPart - 1) / (tile_keys * kMinPart);
-  int64_t s = grid >= 256 ? 1 : (512 + grid - 1) / (grid < 1 ? 1 : grid);
-  s = s > 16 ? 16 : s;
-  return (int)(s > most ? (most < 1 ? 1 : most) : s);
+  const int64_t n = (keys + tile_keys - 1) / tile_keys;
+  int best = 1;
+  int64_t least = 0;
+  for (int s = 1; s <= 16 && grid < 256 && (s == 1 || n > (int64_t)(s - 1) * kMinPart); ++s) {
+    const int64_t cost = (grid * s + 255) / 256 * ((n + s - 1) / s + 4) + (s > 1 ? 8 : 0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  return best;
 }
 inline int64_t record_bytes(int64_t grid, int splits, int rows, int64_t D) {
   return splits > 1 ? grid * splits * rows * (D + 2) * 4 : 0;

@@ -6,11 +6,11 @@ using namespace dkv;
 
 namespace {
 
-template <int DP, bool BF, int WAVES, int GROUPS>
+template <int DP, bool BF, int WAVES, int GROUPS, int KEYS = prompt::keys_of(DP, false)>
 int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
-  constexpr int keys = GROUPS * prompt::keys_of(DP, false), rows = 32 * WAVES / GROUPS;
-  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false, GROUPS>), dim3((unsigned)(grid * p.splits)),
-                     dim3(64 * WAVES), prompt::lds_bytes(DP, false, GROUPS), stream, p);
+  constexpr int keys = GROUPS * KEYS, rows = 32 * WAVES / GROUPS;
+  hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false, GROUPS, KEYS>), dim3((unsigned)(grid * p.splits)),
+                     dim3(64 * WAVES), prompt::lds_bytes(DP, KEYS, GROUPS), stream, p);
   if (p.splits > 1)
     hipLaunchKernelGGL((prompt::prompt_merge<rows, keys, BF, false>), dim3((unsigned)(grid * (rows / 32))), dim3(256), 0,
                        stream, p);
@@ -19,6 +19,7 @@ int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
 
 struct Plan {
   int waves, groups, splits;
+  bool pairs;    // workgroups of 64 rows, two on a CU
   int64_t grid;  // workgroups of one part
   int rows() const { return 32 * waves / groups; }
 };
@@ -28,6 +29,7 @@ int launch_dim(const PromptParams& p, const Plan& plan, hipStream_t stream) {
   if (p.D > 128) return launch<256, BF, 4, 1>(p, plan.grid, stream);
   if (p.D <= 64)
     return plan.groups == 2 ? launch<64, BF, 8, 2>(p, plan.grid, stream) : launch<64, BF, 4, 1>(p, plan.grid, stream);
+  if (plan.pairs) return launch<128, BF, 4, 2, 32>(p, plan.grid, stream);
   if (plan.groups == 2) return launch<128, BF, 8, 2>(p, plan.grid, stream);
   return plan.waves == 8 ? launch<128, BF, 8, 1>(p, plan.grid, stream) : launch<128, BF, 4, 1>(p, plan.grid, stream);
 }
@@ -36,14 +38,20 @@ int launch_dim(const PromptParams& p, const Plan& plan, hipStream_t stream) {
 // shorter ones two workgroups of four on a CU hide each other's start and end (16 of 64 to 4,096: 920 us, eight waves
 // 937; one of 6,464, six heads a KV head: 274 and 284).  head_dim 64 gains more from three waves a SIMD (fp16, six heads
 // a KV head: 179 us, eight waves 207), and over 128 the accumulators leave one.  No more workgroups of 128 rows than CUs:
-// eight waves in two groups (one of 1,024 tokens: 22.6 us, one group 25.2).
+// eight waves in two groups (one of 1,024 tokens: 22.6 us, one group 25.2).  Of a causal triangle half of those workgroups
+// end early: workgroups of 64 rows and tiles of 32 keys, two on a CU, a long one with a short one (20.4 us; one of 512
+// tokens 16.0 -> 13.5, one of 2,048 with 16 heads 35 -> 32).  Where the tiles are about equally long the larger ones are
+// as good or better (1,024 tokens that all see all: 24.5, in pairs 27; 512 behind 7,680: 84 and 104).
 Plan plan_of(const dkv_prompt_attention_args& a) {
   const int64_t G = a.Hq / a.Hkv;
   auto grid_of = [&](int64_t bm) {
     if (!a.q_starts) return a.requests * ((a.q_tokens * G + bm - 1) / bm) * a.Hkv;
     return ((a.q_tokens * G + bm - 1) / bm + a.requests + 1) * a.Hkv;
   };
-  Plan plan = {4, 1, 1, grid_of(128)};
+  Plan plan = {4, 1, 1, false, grid_of(128)};
+  const bool triangle = a.causal && a.k_tokens <= 2 * a.q_tokens;
+  if (triangle && a.D > 64 && a.D <= 128 && plan.grid >= 128 && plan.grid <= 256)
+    return {4, 2, 1, true, grid_of(64)};
   if (a.D <= 128 && plan.grid <= 256)
     plan.waves = 8, plan.groups = 2;
   else if (a.D > 64 && a.D <= 128 && grid_of(256) >= 512 && (a.q_starts ? a.q_tokens / a.requests : a.q_tokens) >= 8192)
@@ -104,7 +112,7 @@ extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void*
   p.causal = a.causal ? 1 : 0, p.fill = a.fill && a.q_starts ? 1 : 0, p.skip_rows = 0;
   const Plan plan = plan_of(a);
   DKV_CHECK(plan.grid * 16 < (1ll << 31), DKV_ERR_INVALID, "dkv_prompt_attention: too many tokens");
-  p.splits = plan.splits;
+  p.splits = plan.splits, p.pairs = plan.pairs ? 1 : 0;
   if (plan.splits > 1) {
     DKV_CHECK(a.workspace && ((uintptr_t)a.workspace & 15) == 0 &&
                   a.workspace_bytes >= prompt::record_bytes(plan.grid, plan.splits, plan.rows(), a.D),

@@ -208,6 +208,34 @@ def test_few_queries_over_many_keys(dtype, D, qn, kn):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,Hkv,G,Q,T,D", [(3, 4, 4, 333, 333, 128), (2, 8, 4, 500, 500, 96), (1, 16, 1, 1300, 1300, 128),
+                                           (1, 8, 4, 501, 903, 72), (1, 4, 4, 999, 901, 128)])
+def test_batches_of_about_one_workgroup_a_cu(dtype, B, Hkv, G, Q, T, D):
+    """128 to 256 tiles of 128 rows, odd and even counts of them for each sequence, head_dims that are not powers of two."""
+    import dartkv_amd as dart
+    q, k, v = (_rand((B, h, n, D), dtype, h + n) for h, n in ((Hkv * G, Q), (Hkv, T), (Hkv, T)))
+    got = dart.prompt_attention(q, k, v)
+    for b in range(B):
+        o, w = _reference(*(t[b].transpose(0, 1) for t in (q, k, v)), True, 1 / math.sqrt(D))
+        _check(got[b].transpose(0, 1), o, w, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qn,kn", [([1, 0, 300, 77, 129], None), ([200, 130, 200], [200, 401, 160]), ([507], None)])
+def test_packed_of_about_one_workgroup_a_cu(qn, kn):
+    import dartkv_amd as dart
+    kn = kn or qn
+    dtype = torch.bfloat16
+    q = _rand((sum(qn) + 70, 32, 128), dtype, 1)
+    k, v = _rand((sum(kn) + 70, 8, 128), dtype, 2), _rand((sum(kn) + 70, 8, 128), dtype, 3)
+    k[sum(kn):], v[sum(kn):] = float("nan"), float("nan")
+    got = dart.prompt_attention(q, k, v, _starts(qn), _starts(kn))
+    _packed_check(got, q, k, v, qn, kn, True, 1 / math.sqrt(128), dtype)
+    assert bool((got[sum(qn):] == 0).all())
+
+
+@pytest.mark.gpu
 def test_out_and_rows_behind_the_last_sequence():
     import dartkv_amd as dart
     q, k, v = (_rand((90, h, 64), torch.bfloat16, h) for h in (4, 2, 2))
