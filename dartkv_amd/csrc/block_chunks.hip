@@ -15,7 +15,7 @@ struct Plan {
 
 // As for prompts; split weights (fp16, head_dim over 64) have the registers for four waves.
 Plan plan_of(const PromptParams& p, int64_t rows_bound, bool bf16) {
-  auto grid_of = [&](int64_t rows) { return ((rows_bound + rows - 1) / rows + p.R) * p.H; };
+  auto grid_of = [&](int64_t rows) { return prompt::tiles_of(rows_bound, p.R, rows) * p.H; };
   Plan plan = {4, 1, 1, grid_of(128)};
   if (p.D <= (bf16 ? 128 : 64) && plan.grid <= 256)
     plan.waves = 8, plan.groups = 2;
@@ -23,7 +23,7 @@ Plan plan_of(const PromptParams& p, int64_t rows_bound, bool bf16) {
     plan.waves = 8, plan.grid = grid_of(256);
   const int DP = p.D <= 64 ? 64 : p.D <= 128 ? 128 : 256;
   plan.splits = prompt::splits_for(plan.grid, (int64_t)p.max_blocks << p.bs_shift,
-                                   plan.groups * prompt::keys_of(DP, !bf16));
+                                   plan.groups * prompt::keys_of(DP, !bf16), p.R == 1, 6);
   return plan;
 }
 

@@ -728,19 +728,25 @@ __global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
 }
 
 // Parts for a launch of `grid` workgroups over at most `keys` keys, where not every one of 256 CUs has a workgroup: the
-// least time in tiles, where a workgroup's start and end cost about as much as four and joining the parts as eight.
+// least time in tiles, where a workgroup's start and end cost about as much as four and joining the parts as `join` (tiles of blocks, which
+// are converted, take longer).  `even`: equally long tiles, in whole rounds of the card; else about three quarters of the
+// longest's length, and the short fill the gaps that the long leave.
 // (Always two workgroups a CU is worse where one round becomes two or three: 2,000 tokens of 16 heads, all seeing all,
 // 252 workgroups, 40 us and 66; 300 tokens behind 7,892, head_dim 64, 50 and 71.)
-inline int splits_for(int64_t grid, int64_t keys, int tile_keys) {
+inline int splits_for(int64_t grid, int64_t keys, int tile_keys, bool even, int join) {
   const int64_t n = (keys + tile_keys - 1) / tile_keys;
   int best = 1;
   int64_t least = 0;
   for (int s = 1; s <= 16 && grid < 256 && (s == 1 || n > (int64_t)(s - 1) * kMinPart); ++s) {
-    const int64_t cost = (grid * s + 255) / 256 * ((n + s - 1) / s + 4) + (s > 1 ? 8 : 0);
+    // 256ths of a round
+    const int64_t fill = even ? (grid * s + 255) / 256 * 256 : grid * s < 342 ? 256 : grid * s * 3 / 4;
+    const int64_t cost = fill * ((n + s - 1) / s + 4) + (s > 1 ? 256 * join : 0);
     if (s == 1 || cost < least) best = s, least = cost;
   }
   return best;
 }
+// Tiles of `bm` rows of R sequences of `rows` rows together, at most.
+inline int64_t tiles_of(int64_t rows, int64_t R, int64_t bm) { return (rows + R * (bm - 1)) / bm; }
 inline int64_t record_bytes(int64_t grid, int splits, int rows, int64_t D) {
   return splits > 1 ? grid * splits * rows * (D + 2) * 4 : 0;
 }

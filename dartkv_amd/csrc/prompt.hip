@@ -46,7 +46,7 @@ Plan plan_of(const dkv_prompt_attention_args& a) {
   const int64_t G = a.Hq / a.Hkv;
   auto grid_of = [&](int64_t bm) {
     if (!a.q_starts) return a.requests * ((a.q_tokens * G + bm - 1) / bm) * a.Hkv;
-    return ((a.q_tokens * G + bm - 1) / bm + a.requests + 1) * a.Hkv;
+    return prompt::tiles_of(a.q_tokens * G, a.requests + (a.fill ? 1 : 0), bm) * a.Hkv;
   };
   Plan plan = {4, 1, 1, false, grid_of(128)};
   const bool triangle = a.causal && a.k_tokens <= 2 * a.q_tokens;
@@ -56,7 +56,8 @@ Plan plan_of(const dkv_prompt_attention_args& a) {
     plan.waves = 8, plan.groups = 2;
   else if (a.D > 64 && a.D <= 128 && grid_of(256) >= 512 && (a.q_starts ? a.q_tokens / a.requests : a.q_tokens) >= 8192)
     plan.waves = 8, plan.grid = grid_of(256);
-  plan.splits = prompt::splits_for(plan.grid, a.k_tokens, plan.groups * prompt::keys_of(a.D <= 128 ? 128 : 256, false));
+  plan.splits = prompt::splits_for(plan.grid, a.k_tokens, plan.groups * prompt::keys_of(a.D <= 128 ? 128 : 256, false),
+                                   !a.q_starts || a.requests == 1, 10);
   return plan;
 }
 
