@@ -24,7 +24,7 @@
 //
 // Bound and measured.  16,384 tokens of 32 query heads of 128, bf16: 1.96-2.0 ms, 1.1 PFLOP/s.  The matrix units are busy
 // 54 % of the cycles, at 1.65 GHz: the power limit holds the clock down as the kernel gets denser (1.77 GHz at 48 %; a
-// 16,384^3 matrix product reaches 1.37 PFLOP/s).  LDS 27 % busy.  A single short prompt is bound by its longest tile and
+// 16,384^3 matrix product reaches 1.37 PFLOP/s).  LDS 27 % busy.  A single short prompt is bound by its last tiles and
 // about 8 us of start and end.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -728,9 +728,9 @@ __global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
 }
 
 // Parts for a launch of `grid` workgroups over at most `keys` keys, where not every one of 256 CUs has a workgroup: the
-// least time in tiles, where a workgroup's start and end cost about as much as four and joining the parts as `join` (tiles of blocks, which
-// are converted, take longer).  `even`: equally long tiles, in whole rounds of the card; else about three quarters of the
-// longest's length, and the short fill the gaps that the long leave.
+// least time in tiles, where a workgroup's start and end cost about as much as four and joining the parts as `join`
+// (fewer for blocks, whose tiles are converted and take longer).  `even`: equally long tiles, in whole rounds of the
+// card; else about three quarters of the longest's length, and the short fill the gaps that the long leave.
 // (Always two workgroups a CU is worse where one round becomes two or three: 2,000 tokens of 16 heads, all seeing all,
 // 252 workgroups, 40 us and 66; 300 tokens behind 7,892, head_dim 64, 50 and 71.)
 inline int splits_for(int64_t grid, int64_t keys, int tile_keys, bool even, int join) {
