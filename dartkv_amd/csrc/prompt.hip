@@ -8,12 +8,14 @@ namespace {
 
 template <int DP, bool BF, int WAVES, int GROUPS, int KEYS = prompt::keys_of(DP, false)>
 int launch(const PromptParams& p, int64_t grid, hipStream_t stream) {
-  constexpr int keys = GROUPS * KEYS, rows = 32 * WAVES / GROUPS;
+  [[maybe_unused]] constexpr int keys = GROUPS * KEYS, rows = 32 * WAVES / GROUPS;
   hipLaunchKernelGGL((prompt::prompt_tiles<DP, BF, WAVES, false, GROUPS, KEYS>), dim3((unsigned)(grid * p.splits)),
                      dim3(64 * WAVES), prompt::lds_bytes(DP, KEYS, GROUPS), stream, p);
-  if (p.splits > 1)
-    hipLaunchKernelGGL((prompt::prompt_merge<rows, keys, BF, false>), dim3((unsigned)(grid * (rows / 32))), dim3(256), 0,
-                       stream, p);
+  if constexpr (KEYS == prompt::keys_of(DP, false)) {  // (pairs come in one part)
+    if (p.splits > 1)
+      hipLaunchKernelGGL((prompt::prompt_merge<rows, keys, BF, false>), dim3((unsigned)(grid * (rows / 32))), dim3(256),
+                         0, stream, p);
+  }
   return dkv_check_launch("dkv_prompt_attention");
 }
 
@@ -36,12 +38,13 @@ int launch_dim(const PromptParams& p, const Plan& plan, hipStream_t stream) {
 
 // Eight waves share each tile's copies in LDS for long sequences (one of 16,384 tokens: 1.99 ms, four waves 2.03); with
 // shorter ones two workgroups of four on a CU hide each other's start and end (16 of 64 to 4,096: 920 us, eight waves
-// 937; one of 6,464, six heads a KV head: 274 and 284).  head_dim 64 gains more from three waves a SIMD (fp16, six heads
-// a KV head: 179 us, eight waves 207), and over 128 the accumulators leave one.  No more workgroups of 128 rows than CUs:
-// eight waves in two groups (one of 1,024 tokens: 22.6 us, one group 25.2).  Of a causal triangle half of those workgroups
-// end early: workgroups of 64 rows and tiles of 32 keys, two on a CU, a long one with a short one (20.4 us; one of 512
-// tokens 16.0 -> 13.5, one of 2,048 with 16 heads 35 -> 32).  Where the tiles are about equally long the larger ones are
-// as good or better (1,024 tokens that all see all: 24.5, in pairs 27; 512 behind 7,680: 84 and 104).
+// 937; one of 6,464, six heads a KV head: 274 and 284).  head_dim 64 gains more from three waves a SIMD (fp16, six
+// heads a KV head: 179 us, eight waves 207), and over 128 the accumulators leave one.  No more workgroups of 128 rows
+// than CUs: eight waves in two groups (one of 1,024 tokens: 22.6 us, one group 25.2).  Of a causal triangle half of
+// those workgroups end early: workgroups of 64 rows and tiles of 32 keys, two on a CU, a long one with a short one
+// (20.4 us; one of 512 tokens 16.0 -> 13.5, one of 2,048 with 16 heads 35 -> 32).  Where the tiles are about equally
+// long the larger ones are as good or better (1,024 tokens that all see all: 24.5, in pairs 27; 512 behind 7,680: 84 and
+// 104).
 Plan plan_of(const dkv_prompt_attention_args& a) {
   const int64_t G = a.Hq / a.Hkv;
   auto grid_of = [&](int64_t bm) {
