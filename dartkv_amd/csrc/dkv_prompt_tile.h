@@ -8,7 +8,9 @@
 // One pass over the keys, 64 at a time, with a running maximum m and sum l (fp32) per row:
 //   s = c q.k (c = scale log2 e), p = 2^(s - m), l += p, o += p v, and o, l times 2^(m - m') when m grows.
 // m is only raised when a row's maximum exceeds it by more than 8 (2^8: p stays within bf16 and fp16, and l and
-// o are sums of the same p), so most tiles scale nothing.
+// o are sums of the same p), so most tiles scale nothing.  fp16 has 2^7 p in place of p, which cancels in o / l: up to
+// 2^15 of its 2^16, and normal from p = 2^-21 on (bare weights were subnormal under 2^-14 and 0 under 2^-25, while l had
+// them whole: beside a dominant key 2^20 times as heavy the others' sum was 3 % off).
 //
 // Matrix layout.  Both products are v_mfma_f32_32x32x16 with the query row in the column of the result:
 // S^T = K Q^T puts keys 8 (i / 4) + 4 half + i % 4 (i < 16) of 32 in lane (row, half)'s accumulators, and
@@ -551,12 +553,14 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
           a[ks & 1][cb] = x.whole;
         }
       };
+      float lift = -m;
+      if constexpr (!BF && !BLOCKS) lift = 7.f - m;
       auto weights = [&](int ks) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = 8 * (ks % 2) + 2 * i;
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at], p.c, -m));
-          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at + 1], p.c, -m));
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at], p.c, lift));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks / 2][at + 1], p.c, lift));
           l += x, l += y;
           const uint32_t pair = pack2<BF || BLOCKS>(x, y);
           pk[ks & 1][i] = pair;

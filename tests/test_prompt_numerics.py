@@ -1,0 +1,47 @@
+"""prompt_attention where its types' ranges and its parts show, against 64 bits.
+
+Bounds are test_prompt_attention's, u (W + |o|) with u half a step of the type, and what is said at each test.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests.test_prompt_attention import _check, _packed_check, _rand, _reference, _starts
+
+DEV = "cuda"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("drop", [12.5, 20.5, 26.5])
+def test_small_weights_beside_one_dominant_key_in_fp16(D, causal, drop):
+    """One key whose value is 0 has all the weight but 2^-drop for each other key, and the result is theirs alone.
+
+    The kernel rounds 2^7 p to fp16, p = 2^(s - m) with m at most 8 under the row's maximum, so p of the dominant key is at
+    least 1, as is the sum of weights.  2^7 p is normal from 2^-14 on (p from 2^-21): half a step u relative.  Under that
+    the step is 2^-24, so p is off by at most 2^-32: |error| <= u (W + |o|) + 2^-32 sum |v|.
+    """
+    import dartkv_amd as dart
+    n = 700
+    q = torch.zeros(n, 2, D)
+    q[..., 0] = 1.0
+    k = torch.zeros(n, 1, D)
+    k[0, 0, 0] = drop
+    v = (torch.randn(n, 1, D, generator=torch.Generator().manual_seed(D)) + 2) * 1000
+    v[0] = 0.0
+    q, k, v = (t.half().to(DEV) for t in (q, k, v))
+    got = dart.prompt_attention(q, k, v, _starts([n]), causal=causal, scale=math.log(2.0))
+    o, w = _reference(q, k, v, causal, math.log(2.0))
+    u = torch.finfo(torch.float16).eps / 2
+    bound = 1.01 * u * (w + o.abs()) + 1e-6 * w
+    # the result's own rounding, where it is subnormal in fp16
+    bound = bound + 2.0 ** -25
+    if drop > 21:
+        bound = bound + 2.0 ** -32 * v.double().abs().sum(0).cpu()
+    err = (got.double().cpu() - o).abs()
+    assert bool((err <= bound).all()), f"error is {float((err / bound).max()):.3f} of its bound"
