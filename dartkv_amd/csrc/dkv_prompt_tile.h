@@ -220,9 +220,10 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
   return t;
 }
 
-// A product adds 0 * v for a key that its row does not see, which is NaN where v is an infinity or a NaN.  Where a
-// tile's result is not finite, it is computed again with such values set to 0 in LDS, and what they do is added at
-// the end: a row sees the keys before its limit, so it sees one exactly if the channel's first one is before it.
+// A product adds 0 * v for a key that its row does not see, or whose weight is too small for its type, which is NaN where
+// v is an infinity or a NaN.  Where a tile's result is not finite, it is computed again with such values set to 0 in LDS,
+// and what they do is added at the end: a row sees the keys before its limit, so it sees one exactly if the channel's
+// first one is before it.
 // first[ch] is the first key with an infinity or NaN, first[DP + ch] with a negative infinity or NaN.
 template <int DP, int KEYS, bool BF, int THREADS>
 __device__ __forceinline__ void set_apart(char* lv, int j, int32_t* first) {
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
       if constexpr (BLOCKS)
         if (more) blocks.finish(lds + next, lds + next + kTileBytes, lscale + 8 * buf);
     }
-    if (careful || !p.causal) break;
+    if (careful) break;
     float zero = 0.f;
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb)

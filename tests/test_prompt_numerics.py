@@ -45,3 +45,21 @@ def test_small_weights_beside_one_dominant_key_in_fp16(D, causal, drop):
         bound = bound + 2.0 ** -32 * v.double().abs().sum(0).cpu()
     err = (got.double().cpu() - o).abs()
     assert bool((err <= bound).all()), f"error is {float((err / bound).max()):.3f} of its bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,drop", [(torch.bfloat16, 140.0), (torch.float16, 60.0)])
+@pytest.mark.parametrize("n", [40, 300])
+def test_an_infinite_value_under_a_small_weight(dtype, drop, n):
+    """Without the causal mask every row sees every key: a positive weight times an infinity is one, however small."""
+    import dartkv_amd as dart
+    q, k, v = (_rand((n, h, 64), dtype, h, 0.5) for h in (4, 2, 2))
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[17, 0, 0] = -drop
+    v[17, 0, 3], v[17, 0, 9] = float("inf"), float("-inf")
+    got = dart.prompt_attention(q, k, v, _starts([n]), causal=False, scale=math.log(2.0)).double().cpu()
+    assert bool((got[:, :2, 3] == math.inf).all()) and bool((got[:, :2, 9] == -math.inf).all())
+    v[17, 0, 3], v[17, 0, 9] = 0.0, 0.0
+    o, w = _reference(q, k, v, False, math.log(2.0))
+    got[:, :2, 3], got[:, :2, 9] = o[:, :2, 3], o[:, :2, 9]
+    _check(got, o, w, dtype)
