@@ -670,6 +670,9 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
     }
 }
 
+// A part's sum at the weight of its maximum: an infinity stays one however small that is.
+__device__ __forceinline__ float weighted(float x, float f) { return __builtin_isfinite(x) ? x * f : x; }
+
 // Joins the parts' records of a tile: a workgroup has 32 of its rows, a wave one at a time.
 template <int BM, int KEYS, bool BF, bool BLOCKS>
 __global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
@@ -711,15 +714,15 @@ __global__ void __launch_bounds__(256) prompt_merge(PromptParams p) {
       const float f0 = __builtin_amdgcn_exp2f(m - up);
       m = up, l *= f0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[c] *= f0;
+      for (int c = 0; c < 4; ++c) acc[c] = weighted(acc[c], f0);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         if (ml[x][1] == 0.f) continue;  // no key seen
-        // (not 0, so that an infinity among the part's values stays one)
-        const float f = fmaxf(__builtin_amdgcn_exp2f(ml[x][0] - up), 1.1754944e-38f);
+        const float f = __builtin_amdgcn_exp2f(ml[x][0] - up);
         l += ml[x][1] * f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) acc[2 * c] += v[x][c][0] * f, acc[2 * c + 1] += v[x][c][1] * f;
+        for (int c = 0; c < 2; ++c)
+          acc[2 * c] += weighted(v[x][c][0], f), acc[2 * c + 1] += weighted(v[x][c][1], f);
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -63,3 +63,26 @@ def test_an_infinite_value_under_a_small_weight(dtype, drop, n):
     o, w = _reference(q, k, v, False, math.log(2.0))
     got[:, :2, 3], got[:, :2, 9] = o[:, :2, 3], o[:, :2, 9]
     _check(got, o, w, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_large_values_in_a_part_without_weight(D):
+    """The keys come in parts; some parts' values are large and their weights 2^-400 of the dominant key's: they
+    add nothing, an infinity among them apart."""
+    import dartkv_amd as dart
+    nq, nk = 3, 5000
+    q, k, v = _rand((nq, 4, D), torch.bfloat16, 1, 0.1), _rand((nk, 2, D), torch.bfloat16, 2), _rand((nk, 2, D), torch.bfloat16, 3)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    k[:2048, :, 0] = -300.0
+    v[:2048] = 1e34
+    k[4800, :, 0] = 100.0
+    got = dart.prompt_attention(q, k, v, _starts([nq]), _starts([nk]), scale=math.log(2.0))
+    o, w = _reference(q, k, v, True, math.log(2.0))
+    _check(got, o, w, torch.bfloat16)
+    v[5, 0, 3] = float("inf")  # in the first part, which the last one outweighs
+    again = dart.prompt_attention(q, k, v, _starts([nq]), _starts([nk]), scale=math.log(2.0))
+    assert bool((again[:, :2, 3] == math.inf).all())
+    again[:, :2, 3] = got[:, :2, 3]
+    assert torch.equal(again, got)
