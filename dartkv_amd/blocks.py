@@ -218,8 +218,8 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     more after all are undefined.  Default: T (without starts 1).
     ``table`` [requests, max_blocks] and ``lengths`` [requests] (int32), the codes and scales as ``append_blocks``
     writes them.  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
-    makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request are 0 in
-    a new tensor and stay as they were in ``out``.
+    makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request and before
+    the first are 0 in a new tensor and stay as they were in ``out``.
 
     Statistics and sums are fp32.  Forward only: a query that requires gradients is refused outside
     torch.no_grad().

@@ -145,12 +145,13 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) block_decode(Bloc
   __shared__ int32_t first_nan[kThreads / 64][DP];
   int32_t* first = first_nan[threadIdx.x >> 6];
 
-  if (p.fill && p.q_starts) {  // rows behind the last request
-    int64_t end = p.q_starts[p.R];
-    end = end < 0 ? 0 : end;
-    for (int64_t t = end + worker; t < p.q_tokens; t += bp.workers)
+  if (p.fill && p.q_starts) {  // rows behind the last request, then those before the first
+    const int64_t end = clamped(p.q_starts[p.R], 0, p.q_tokens), begin = clamped(p.q_starts[0], 0, end);
+    for (int64_t i = end + worker; i < p.q_tokens + begin; i += bp.workers) {
+      const int64_t t = i < p.q_tokens ? i : i - p.q_tokens;
       for (int c = lane; c < p.G * p.D; c += 64)
         ((uint16_t*)p.o)[t * p.o_st + (h * p.G + c / p.D) * p.o_sh + c % p.D] = 0;
+    }
   }
 
   // all units, then the request that this wave's first lies in

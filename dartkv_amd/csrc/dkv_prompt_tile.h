@@ -44,7 +44,7 @@ struct PromptParams {
   int32_t R, H, G, D;
   int64_t q_tokens, k_tokens;  // rows of the packed tensors, or of each request
   float c;                     // scale * log2(e)
-  int32_t causal, fill;        // fill: rows behind the last request become 0
+  int32_t causal, fill;        // fill: rows behind the last request and before the first become 0
   // e4m3 blocks
   const uint8_t *kc, *vc;       // [blocks][H][bs][D]
   const float *kscale, *vscale;  // [blocks][H]
@@ -152,7 +152,8 @@ struct Tile {
 __device__ __forceinline__ int64_t clamped(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
 // The requests' tiles one after the other, those of more keys first (up to 64 requests; else in their order), found
-// by a wave's scan over the requests: the longest work begins first, and what begins last is short.
+// by a wave's scan over the requests: the longest work begins first, and what begins last is short.  Rows to fill are one
+// more request without keys, from the last request's end round to the first's start (`token_at`).
 template <int BM, bool BLOCKS>
 __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) {
   Tile t = {-1, 0, 0, 0, 0, 0, 0};
@@ -174,7 +175,7 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
     int64_t a = 0, b = 0, ka = 0, kb = 0;
     if (r < total) {  // (never outside the tensors, whatever the starts say)
       a = clamped(p.q_starts[r], 0, p.q_tokens);
-      b = r < p.R ? clamped(p.q_starts[r + 1], a, p.q_tokens) : p.q_tokens;
+      b = r < p.R ? clamped(p.q_starts[r + 1], a, p.q_tokens) : p.q_tokens + clamped(p.q_starts[0], 0, a);
       if (r < p.R) {
         if constexpr (BLOCKS) {
           kb = clamped(p.lengths[r], 0, most);
@@ -218,6 +219,12 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
     before += __builtin_amdgcn_readlane(sum, 63);
   }
   return t;
+}
+
+// The place of a request's token in the packed tensors (those of the rows to fill go round their end).
+__device__ __forceinline__ int64_t token_at(const PromptParams& p, const Tile& t, int token) {
+  const int64_t at = t.q0 + token;
+  return at < p.q_tokens ? at : at - p.q_tokens;
 }
 
 // A product adds 0 * v for a key that its row does not see, or whose weight is too small for its type, which is NaN where
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
   const int row = t.tile * BM + wave * 32 + (lane & 31);
   const bool real = row < t.rows;
   const int token = row / p.G, head = h * p.G + row % p.G;
-  const int64_t qb = p.q_starts ? 0 : t.request;
+  const int64_t qb = p.q_starts ? 0 : t.request, place = token_at(p, t, token);
   auto limit_of = [&](int tok) {
     int n = p.causal ? tok + 1 + nk - t.nq : nk;
     return n < 0 ? 0 : n > nk ? nk : n;
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
 
   u32x4 q[KS];
   {
-    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + (t.q0 + token) * p.q_st + head * p.q_sh);
+    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + place * p.q_st + head * p.q_sh);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int ch = 16 * ks + 8 * half;
@@ -658,7 +665,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* dst = (char*)p.o + 2 * (qb * p.o_sb + (t.q0 + token) * p.o_st + head * p.o_sh);
+  char* dst = (char*)p.o + 2 * (qb * p.o_sb + place * p.o_st + head * p.o_sh);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb)
 #pragma unroll

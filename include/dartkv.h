@@ -455,7 +455,8 @@ int64_t dkv_decode_scratch_bytes(void);
  * [requests + 1], ascending): packed sequences, request r's query tokens at
  * rows [q_starts[r], q_starts[r + 1]) of q_tokens, its keys likewise; sb is
  * not used.  Starts outside the tensors are clamped to them.  fill: output rows
- * behind q_starts[requests] become 0 (0: they are left as they were).
+ * behind q_starts[requests] and before q_starts[0] become 0 (0: they are left as
+ * they were).
  *
  * causal: the last query token sees all nk keys, token i of nq the first
  * i + 1 + nk - nq.  A row that sees no key is 0.  D a multiple of 8 up to 256;
@@ -559,7 +560,8 @@ int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
  * (bf16 or fp16), request r's at rows [starts[r], starts[r + 1]) (starts NULL:
  * one token each), the last of them at position lengths[r] - 1, so token i of n
  * sees the first lengths[r] - n + 1 + i keys.  A row that sees no key is 0.
- * fill: rows behind starts[requests] become 0 (0: they are left as they were).
+ * fill: rows behind starts[requests] and before starts[0] become 0 (0: they are
+ * left as they were).
  * max_tokens: no request has more new tokens (the rows of a request that has
  * more are undefined).  Bytes of blocks behind a request's length are not used; a
  * table entry outside [0, blocks) makes the rows that see it NaN.  D a multiple

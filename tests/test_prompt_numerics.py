@@ -86,3 +86,44 @@ def test_large_values_in_a_part_without_weight(D):
     assert bool((again[:, :2, 3] == math.inf).all())
     again[:, :2, 3] = got[:, :2, 3]
     assert torch.equal(again, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("first,lengths,behind", [(10, [30, 40], 20), (200, [1], 0), (1, [300, 0, 77], 130), (64, [0], 0),
+                                                  (7, [1200], 3)])
+def test_rows_before_the_first_sequence(D, first, lengths, behind):
+    """0 in a new tensor like the rows behind the last, untouched in a given one."""
+    import dartkv_amd as dart
+    total = first + sum(lengths) + behind
+    q, k, v = (_rand((total, h, D), torch.bfloat16, h) for h in (4, 2, 2))
+    starts = _starts(lengths) + first
+    held = torch.full_like(q, float("nan"))
+    del held  # (what a new tensor is likely to hold)
+    got = dart.prompt_attention(q, k, v, starts)
+    real = slice(first, first + sum(lengths))
+    assert bool((got[:first] == 0).all()) and bool((got[real.stop:] == 0).all())
+    _packed_check(got[real], q[real], k[real], v[real], lengths, lengths, True, 1 / math.sqrt(D), torch.bfloat16)
+    out = torch.full((total, 4, D), 7.0, dtype=torch.bfloat16, device=DEV)
+    dart.prompt_attention(q, k, v, starts, out=out)
+    assert torch.equal(out[real], got[real]) and bool((out[:first] == 7).all()) and bool((out[real.stop:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_before_the_first_request_of_a_block_cache(many):
+    import dartkv_amd as dart
+    from tests.test_blocks import _cache, _check_attention, _query
+    new, lengths, first, behind = ([70, 1, 33] if many else [2, 1, 3]), [100, 300, 40], 5, 4
+    cache = _cache(lengths, 2, 64, 32, 7)
+    total = first + sum(new) + behind
+    q = _query(total, 4, 64, torch.bfloat16, 7)
+    held = torch.full_like(q, float("nan"))
+    del held
+    got = dart.block_attention(q, *cache, _starts(new) + first, max_tokens=None if many else 3)
+    real = slice(first, first + sum(new))
+    assert bool((got[:first] == 0).all()) and bool((got[real.stop:] == 0).all())
+    _check_attention(got[real], q[real], cache, new, torch.bfloat16, chunk=many)
+    out = torch.full((total, 4, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    dart.block_attention(q, *cache, _starts(new) + first, max_tokens=None if many else 3, out=out)
+    assert torch.equal(out[real], got[real]) and bool((out[:first] == 7).all()) and bool((out[real.stop:] == 7).all())
