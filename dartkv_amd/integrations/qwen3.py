@@ -32,7 +32,7 @@ from torch import nn
 
 from .. import _lib
 from ..fused_attention import fused_dart_attention
-from ..prompt import MAX_PROMPT_HEAD_DIM, prompt_attention
+from ..prompt import MAX_PROMPT_HEAD_DIM, followed, prompt_attention
 from .huggingface import DartHFCache
 
 
@@ -121,16 +121,18 @@ def _can_prepare(attn: nn.Module, hidden_states: torch.Tensor, cos: torch.Tensor
     return _fused_qkv_weight(attn)
 
 
-def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, attention_mask, kwargs: dict) -> bool:
+def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, attention_mask,
+                    kwargs: dict) -> bool:
     """Whether the backend's attention of these tensors is causal attention of whole prompts: sdpa takes a missing
     mask for it where there are as many keys as queries."""
     return (getattr(attn, "dart_prompt_attention", False) and attention_mask is None
             and attn.config._attn_implementation == "sdpa" and query.device.type == "cuda"
             and query.shape[-2] == keys.shape[-2] and query.dtype in (torch.bfloat16, torch.float16)
-            and keys.dtype == query.dtype and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_PROMPT_HEAD_DIM
+            and keys.dtype == values.dtype == query.dtype
+            and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_PROMPT_HEAD_DIM
             and attn.sliding_window is None and not (attn.training and attn.attention_dropout)
             and kwargs.get("is_causal") in (None, True) and not kwargs.get("output_attentions")
-            and not (torch.is_grad_enabled() and (query.requires_grad or keys.requires_grad)))
+            and not followed(query, keys, values))
 
 
 class DartQwen3Attention:  # replaced by build_dart_qwen3_attention_class()
@@ -182,7 +184,7 @@ def build_dart_qwen3_attention_class():
                     query_states, cache.layer_for_attention(self.layer_idx), scale=self.scaling, fallback=True,
                 ).transpose(1, 2)
                 attn_weights = None
-            elif _can_run_prompt(self, query_states, key_states, attention_mask, kwargs):
+            elif _can_run_prompt(self, query_states, key_states, value_states, attention_mask, kwargs):
                 attn_output = prompt_attention(query_states, key_states, value_states, scale=self.scaling).transpose(1, 2)
                 attn_weights = None
             else:

@@ -21,9 +21,14 @@ from .attention import _workspace
 MAX_PROMPT_HEAD_DIM = 256
 
 
+def followed(*tensors: torch.Tensor) -> bool:
+    """Whether autograd would follow an operation on one of the tensors."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
 def no_gradients(name: str, *tensors: torch.Tensor) -> None:
     """Forward-only operators refuse tensors that autograd would follow."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if followed(*tensors):
         raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
 
 
