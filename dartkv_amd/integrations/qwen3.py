@@ -124,14 +124,18 @@ def _can_prepare(attn: nn.Module, hidden_states: torch.Tensor, cos: torch.Tensor
 def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, attention_mask,
                     kwargs: dict) -> bool:
     """Whether the backend's attention of these tensors is causal attention of whole prompts: sdpa takes a missing
-    mask for it where there are as many keys as queries."""
+    mask for it where there are as many keys as queries, unless ``is_causal``, the keyword or else the module's, says
+    otherwise."""
+    causal = kwargs.get("is_causal")
+    if causal is None:
+        causal = getattr(attn, "is_causal", True)
     return (getattr(attn, "dart_prompt_attention", False) and attention_mask is None
             and attn.config._attn_implementation == "sdpa" and query.device.type == "cuda"
             and query.shape[-2] == keys.shape[-2] and query.dtype in (torch.bfloat16, torch.float16)
             and keys.dtype == values.dtype == query.dtype
             and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_PROMPT_HEAD_DIM
             and attn.sliding_window is None and not (attn.training and attn.attention_dropout)
-            and kwargs.get("is_causal") in (None, True) and not kwargs.get("output_attentions")
+            and bool(causal) and not kwargs.get("output_attentions")
             and not followed(query, keys, values))
 
 

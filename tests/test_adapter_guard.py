@@ -75,3 +75,23 @@ def test_training_of_the_value_projection_alone(calls):
     model(ids, use_cache=False).logits.float().sum().backward()
     assert proj.grad is not None and bool((proj.grad != 0).any())
     assert not calls
+
+
+def test_attention_that_is_not_causal_keeps_the_backend():
+    assert not _runs(_attn(is_causal=False))
+    assert _runs(_attn(is_causal=False), is_causal=True)
+    assert not _runs(is_causal=False)
+
+
+@pytest.mark.gpu
+def test_a_module_that_is_not_causal_sees_all_keys(calls):
+    model = _model()
+    ids = torch.randint(0, 128, (2, 12), generator=torch.Generator().manual_seed(1)).to(DEV)
+    with torch.no_grad():
+        causal = model(ids, use_cache=False).logits
+        assert len(calls) == 2
+        for layer in model.model.layers:
+            layer.self_attn.is_causal = False
+        full = model(ids, use_cache=False).logits
+        assert len(calls) == 2
+    assert not torch.equal(causal[:, 0], full[:, 0])  # (the first token sees the others now)
