@@ -121,11 +121,18 @@ def _can_prepare(attn: nn.Module, hidden_states: torch.Tensor, cos: torch.Tensor
     return _fused_qkv_weight(attn)
 
 
+# Keywords that may reach the attention: they do not change what sdpa computes, or _can_run_prompt looks at them.
+_KNOWN_KEYWORDS = frozenset(("cache_position", "is_causal", "num_items_in_batch", "output_attentions",
+                             "output_hidden_states", "position_ids", "return_dict", "use_cache"))
+
+
 def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, attention_mask,
                     kwargs: dict) -> bool:
     """Whether the backend's attention of these tensors is causal attention of whole prompts: sdpa takes a missing
     mask for it where there are as many keys as queries, unless ``is_causal``, the keyword or else the module's, says
-    otherwise."""
+    otherwise, or another keyword (a bias on positions) does."""
+    if any(value is not None and name not in _KNOWN_KEYWORDS for name, value in kwargs.items()):
+        return False
     causal = kwargs.get("is_causal")
     if causal is None:
         causal = getattr(attn, "is_causal", True)

@@ -95,3 +95,10 @@ def test_a_module_that_is_not_causal_sees_all_keys(calls):
         full = model(ids, use_cache=False).logits
         assert len(calls) == 2
     assert not torch.equal(causal[:, 0], full[:, 0])  # (the first token sees the others now)
+
+
+def test_arguments_that_the_kernel_does_not_know_keep_the_backend():
+    assert not _runs(position_bias=torch.zeros(1))
+    assert not _runs(output_attentions=True)
+    assert _runs(position_bias=None, position_ids=torch.zeros(1), use_cache=True, output_attentions=False,
+                 num_items_in_batch=3)
