@@ -228,7 +228,7 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     scale = None if scale is None else float(scale)
     max_tokens = None if max_tokens is None else int(max_tokens)
     key = None
-    if starts is None or starts.dtype == torch.int32:
+    if starts is None or (isinstance(starts, torch.Tensor) and starts.dtype == torch.int32):
         key = ("attend", max_tokens, scale, fill,
                _lib.layouts(query, key_codes, value_codes, key_scale, value_scale, table, lengths,
                             *(() if starts is None else (starts,)), *(() if fill else (out,))), starts is None)

@@ -86,10 +86,12 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     packed = query_starts is not None
     if packed and key_starts is None:
         key_starts = query_starts
+    if not packed and key_starts is not None:
+        raise ValueError("key_starts needs query_starts")
     fill = out is None
     scale = None if scale is None else float(scale)
     key = None
-    if not packed or (query_starts.dtype == torch.int32 == key_starts.dtype):
+    if not packed or all(isinstance(t, torch.Tensor) and t.dtype == torch.int32 for t in (query_starts, key_starts)):
         key = ("prompt", bool(causal), scale, fill, packed,
                _lib.layouts(query, keys, values, *((query_starts, key_starts) if packed else ()),
                             *(() if fill else (out,))))
@@ -129,8 +131,6 @@ def _checked(query, keys, values, query_starts, key_starts, causal, scale, out):
     device = query.device
     if keys.device != device or values.device != device:
         raise ValueError("query, keys and values must be on the same device")
-    if key_starts is not None and not packed:
-        raise ValueError("key_starts needs query_starts")
     dims = 3 if packed else 4
     if query.dim() != dims or keys.dim() != dims or values.dim() != dims:
         raise ValueError("query, keys and values must be [T, H, D] with query_starts, [B, H, T, D] without")
