@@ -222,7 +222,7 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     the first are 0 in a new tensor and stay as they were in ``out``.
 
     Statistics and sums are fp32.  Forward only: a query that requires gradients is refused outside
-    torch.no_grad().
+    torch.no_grad(), forward-mode tangents always.
     """
     fill = out is None
     scale = None if scale is None else float(scale)

@@ -14,6 +14,7 @@ import math
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 from .attention import _workspace
@@ -22,14 +23,19 @@ MAX_PROMPT_HEAD_DIM = 256
 
 
 def followed(*tensors: torch.Tensor) -> bool:
-    """Whether autograd would follow an operation on one of the tensors."""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    """Whether autograd would follow an operation on one of the tensors, backward or (which no_grad leaves on) forward."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    # (the level is -1 outside forward_ad.dual_level(), where no tensor has a tangent)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None
+                                                                 for t in tensors)
 
 
 def no_gradients(name: str, *tensors: torch.Tensor) -> None:
     """Forward-only operators refuse tensors that autograd would follow."""
     if followed(*tensors):
-        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad() or detach its inputs")
+        raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad(), or detach its "
+                           "inputs (forward mode: unpack them)")
 
 
 def scale_factor(scale: Optional[float], head_dim: int, name: str) -> float:
@@ -81,7 +87,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     in a new tensor and stay as they were in ``out``.  Keys a row does not see do not change it, whatever they hold.
 
     Softmax statistics and sums are fp32; the weights are rounded to the tensors' type for the second product.
-    Forward only: tensors that require gradients are refused outside torch.no_grad().
+    Forward only: tensors that require gradients are refused outside torch.no_grad(), forward-mode tangents always.
     """
     packed = query_starts is not None
     if packed and key_starts is None:

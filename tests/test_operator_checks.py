@@ -19,3 +19,15 @@ def test_key_starts_alone_are_refused_every_time():
         dart.prompt_attention(q, q[:, :2], q[:, 2:])
     with pytest.raises(TypeError, match="starts"):
         dart.prompt_attention(q[0].transpose(0, 1), q[0].transpose(0, 1), q[0].transpose(0, 1), [0, 8])
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as forward
+    from dartkv_amd.prompt import no_gradients
+    x = torch.zeros(3)
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones(3))
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            no_gradients("prompt_attention", x, dual.view(3, 1))
+        no_gradients("prompt_attention", x)
+    no_gradients("prompt_attention", x)
