@@ -151,8 +151,9 @@ def append_blocks(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor,
     raise the scale, the codes before them are rounded to it.  Slots are used once each, a block's next to each
     other and ascending; -1 (and any slot outside the blocks) writes nothing.  NaN and infinities become NaN, do
     not count for the scale, and set ``nonfinite`` (an int32 scalar tensor) to 1.  head_dim: a multiple of 16 up to
-    256.
+    256.  Keys and values that require gradients are refused outside torch.no_grad(), forward-mode tangents always.
     """
+    no_gradients("append_blocks", keys, values)
     key = ("append", _lib.layouts(keys, values, slots, key_codes, value_codes, key_scale, value_scale))
     known = _lib.template(key)
     if known is None or (keys.data_ptr() | values.data_ptr()) % 16:

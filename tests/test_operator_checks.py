@@ -31,3 +31,20 @@ def test_forward_mode_tangents_are_refused():
             no_gradients("prompt_attention", x, dual.view(3, 1))
         no_gradients("prompt_attention", x)
     no_gradients("prompt_attention", x)
+
+
+@pytest.mark.gpu
+def test_appends_refuse_gradients():
+    import dartkv_amd as dart
+    pool = [torch.zeros(2, 1, 16, 32, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)] + \
+        [torch.ones(2, 1, device=DEV) for _ in range(2)]
+    x = torch.ones(3, 1, 32, dtype=torch.bfloat16, device=DEV)
+    grad = torch.ones_like(x).requires_grad_()
+    slots = torch.arange(3, device=DEV)
+    for _ in range(2):
+        for k, v in ((grad, x), (x, grad)):
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                dart.append_blocks(k, v, slots, *pool)
+        dart.append_blocks(x, x, slots, *pool)
+    with torch.no_grad():
+        dart.append_blocks(grad, grad, slots, *pool)
