@@ -15,6 +15,7 @@ captured in a HIP graph and replayed while the requests grow.  The reference has
 
 from __future__ import annotations
 
+import itertools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -315,9 +316,12 @@ def _checked_attention(query, key_codes, value_codes, key_scale, value_scale, ta
     return a, query, starts, query is given[0] and starts is given[1]
 
 
+_steps = itertools.count(1)  # one line of steps for all caches, so that none takes another's plan
+
+
 class BlockPlan(NamedTuple):
     """Where a step's new tokens go: ``reserve_blocks``' slots and starts, the most tokens of a request, and the
-    cache's step that they belong to."""
+    step of one cache that they belong to."""
 
     slots: torch.Tensor
     starts: torch.Tensor
@@ -359,24 +363,24 @@ class BlockKVCache:
         self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
         self.state = torch.tensor([blocks, 0, 0, 0], dtype=torch.int32, device=device)
         self.nonfinite = torch.zeros(1, dtype=torch.int32, device=device)
-        self._step = 0
+        self._step = next(_steps)
 
     def _check_plan(self, plan: BlockPlan) -> None:
         if plan.step != self._step:
-            raise ValueError("the plan is of an earlier reserve: the requests' lengths have moved on")
+            raise ValueError("the plan is of an earlier reserve, whose requests' lengths have moved on, or of another cache")
 
     def reserve(self, tokens: torch.Tensor, total: int, *, max_tokens: Optional[int] = None) -> BlockPlan:
         """Room for ``tokens[r]`` new tokens of each request (``reserve_blocks``).  ``max_tokens``: the most of
         them, where the caller knows it; a request with more is left out of ``attention``."""
         slots, starts = reserve_blocks(self.table, self.lengths, self.free, self.state, tokens, total,
                                        block_size=self.block_size)
-        self._step += 1
+        self._step = next(_steps)
         return BlockPlan(slots, starts, max(1, total if max_tokens is None else max_tokens), self._step)
 
     def release(self, tokens: Optional[torch.Tensor] = None) -> None:
         """Drop each request's last ``tokens[r]`` tokens, or everything (``release_blocks``)."""
         release_blocks(self.table, self.lengths, self.free, self.state, tokens, block_size=self.block_size)
-        self._step += 1
+        self._step = next(_steps)
 
     def append(self, layer: int, keys: torch.Tensor, values: torch.Tensor, plan: BlockPlan) -> None:
         """The step's new ``keys`` and ``values`` [T, kv_heads, head_dim] of one layer (``append_blocks``)."""

@@ -48,3 +48,17 @@ def test_appends_refuse_gradients():
         dart.append_blocks(x, x, slots, *pool)
     with torch.no_grad():
         dart.append_blocks(grad, grad, slots, *pool)
+
+
+@pytest.mark.gpu
+def test_plans_of_another_cache_are_refused():
+    import dartkv_amd as dart
+    one, other = (dart.BlockKVCache(2, 8, 1, 64, block_size=16) for _ in range(2))
+    x = torch.ones(2, 1, 64, dtype=torch.bfloat16, device=DEV)
+    tokens = torch.ones(2, dtype=torch.int32, device=DEV)
+    mine, others = one.reserve(tokens, 2), other.reserve(tokens, 2)
+    for call in (lambda: one.append(0, x, x, others), lambda: one.attention(0, x, others)):
+        with pytest.raises(ValueError, match="another cache"):
+            call()
+    one.append(0, x, x, mine)
+    assert torch.equal(one.attention(0, x, mine), x)
