@@ -48,11 +48,13 @@ def scale_factor(scale: Optional[float], head_dim: int, name: str) -> float:
 
 
 def int32_vector(t: torch.Tensor, what: str, device: torch.device) -> torch.Tensor:
-    """``t`` as a contiguous int32 vector on ``device``."""
+    """``t`` as a contiguous int32 vector on ``device``; what 31 bits do not hold becomes the nearest that they do."""
     if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{what} must be a one-dimensional int32 or int64 tensor")
     if t.device != device:
         raise ValueError(f"{what} must be on {device}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
     return t.to(torch.int32).contiguous()
 
 

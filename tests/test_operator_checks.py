@@ -62,3 +62,20 @@ def test_plans_of_another_cache_are_refused():
             call()
     one.append(0, x, x, mine)
     assert torch.equal(one.attention(0, x, mine), x)
+
+
+def test_counts_and_starts_past_31_bits_do_not_wrap():
+    from dartkv_amd.prompt import int32_vector
+    most = 2 ** 31 - 1
+    got = int32_vector(torch.tensor([0, 5, 2 ** 32 + 1, -2 ** 32 + 7, 2 ** 31, most]), "tokens", torch.device("cpu"))
+    assert got.dtype == torch.int32 and got.tolist() == [0, 5, most, -2 ** 31, most, most]
+
+
+@pytest.mark.gpu
+def test_a_count_past_31_bits_is_reported():
+    import dartkv_amd as dart
+    cache = dart.BlockKVCache(2, 8, 1, 64, block_size=16)
+    plan = cache.reserve(torch.tensor([2 ** 32 + 1, 1], device=DEV), 2)
+    assert plan.slots.tolist() == [-1, -1] and cache.lengths.tolist() == [0, 0]
+    with pytest.raises(RuntimeError, match="more new tokens than total"):
+        cache.check()
