@@ -673,7 +673,8 @@ extern "C" int dkv_block_attention(const dkv_block_attention_args* args, void* s
   if (bad != DKV_OK) return bad;
   DKV_CHECK(a.starts || a.tokens == a.requests, DKV_ERR_INVALID,
             "dkv_block_attention: without starts every request has one token");
-  DKV_CHECK(a.scale > 0 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_block_attention: scale must be positive and finite");
+  // (the fp32 factor must not be 0: a hidden key's logit would be -inf * 0)
+  DKV_CHECK(a.scale >= 1e-37 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_block_attention: scale must be in 1e-37 to 1e30");
   if (a.tokens == 0) return DKV_OK;
   DKV_CHECK(a.query && a.out && a.key_codes && a.value_codes && a.key_scale && a.value_scale && a.table && a.lengths,
             DKV_ERR_INVALID, "dkv_block_attention: NULL pointer");

@@ -93,7 +93,8 @@ extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void*
   if (rc != DKV_OK) return rc;
   DKV_CHECK((a.q_starts == nullptr) == (a.k_starts == nullptr), DKV_ERR_INVALID,
             "dkv_prompt_attention: query and key starts come together");
-  DKV_CHECK(a.scale > 0 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_prompt_attention: scale must be positive and finite");
+  // (the fp32 factor must not be 0: a hidden key's logit would be -inf * 0)
+  DKV_CHECK(a.scale >= 1e-37 && a.scale < 1e30, DKV_ERR_INVALID, "dkv_prompt_attention: scale must be in 1e-37 to 1e30");
   if (a.q_tokens == 0) return DKV_OK;
   DKV_CHECK(a.query && a.out && (a.k_tokens == 0 || (a.keys && a.values)), DKV_ERR_INVALID,
             "dkv_prompt_attention: NULL pointer");

@@ -42,8 +42,8 @@ def scale_factor(scale: Optional[float], head_dim: int, name: str) -> float:
     if scale is None:
         return 1.0 / math.sqrt(head_dim)
     scale = float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"{name}: scale must be positive and finite")
+    if not 1e-37 <= scale < 1e30:  # (its fp32 factor must not be 0: a hidden key's logit would be -inf * 0)
+        raise ValueError(f"{name}: scale must be positive, from 1e-37 to 1e30")
     return scale
 
 
@@ -84,9 +84,10 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
 
     ``causal``: the last query token of a sequence sees all its nk keys, token i of nq the first
     ``i + 1 + nk - nq``; a row that sees no key is 0.  bf16 and fp16, head_dim a multiple of 8 up to 256, any
-    strides (rows that are not 16-byte aligned are copied).  ``scale`` defaults to 1 / sqrt(D).  Returns a tensor
-    like ``query``, or ``out`` (contiguous rows of D).  Rows behind the last packed sequence and before the first are 0
-    in a new tensor and stay as they were in ``out``.  Keys a row does not see do not change it, whatever they hold.
+    strides (rows that are not 16-byte aligned are copied).  ``scale`` (1e-37 to 1e30) defaults to 1 / sqrt(D).
+    Returns a tensor like ``query``, or ``out`` (contiguous rows of D).  Rows behind the last packed sequence and before
+    the first are 0 in a new tensor and stay as they were in ``out``.  Keys a row does not see do not change it,
+    whatever they hold.
 
     Softmax statistics and sums are fp32; the weights are rounded to the tensors' type for the second product.
     Forward only: tensors that require gradients are refused outside torch.no_grad(), forward-mode tangents always.

@@ -459,7 +459,8 @@ int64_t dkv_decode_scratch_bytes(void);
  * they were).
  *
  * causal: the last query token sees all nk keys, token i of nq the first
- * i + 1 + nk - nq.  A row that sees no key is 0.  D a multiple of 8 up to 256;
+ * i + 1 + nk - nq.  A row that sees no key is 0.  scale from 1e-37 to 1e30 (not
+ * included).  D a multiple of 8 up to 256;
  * rows 16-byte aligned (out: 8).  Forward only.  workspace (16-byte aligned):
  * dkv_prompt_attention_workspace_bytes of the same arguments (pointers apart
  * from whether there are starts are not looked at), 0 where the keys are not
@@ -564,8 +565,8 @@ int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
  * left as they were).
  * max_tokens: no request has more new tokens (the rows of a request that has
  * more are undefined).  Bytes of blocks behind a request's length are not used; a
- * table entry outside [0, blocks) makes the rows that see it NaN.  D a multiple
- * of 16 up to 256.  workspace (16-byte aligned):
+ * table entry outside [0, blocks) makes the rows that see it NaN.  scale from
+ * 1e-37 to 1e30 (not included).  D a multiple of 16 up to 256.  workspace (16-byte aligned):
  * dkv_block_attention_workspace_bytes of the same arguments (pointers are not
  * looked at); its contents need not be kept.
  */

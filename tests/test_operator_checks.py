@@ -79,3 +79,22 @@ def test_a_count_past_31_bits_is_reported():
     assert plan.slots.tolist() == [-1, -1] and cache.lengths.tolist() == [0, 0]
     with pytest.raises(RuntimeError, match="more new tokens than total"):
         cache.check()
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-300, 1e-39])
+def test_scales_that_vanish_in_fp32_are_refused(scale):
+    """With a factor of 0 the masked logits would be -inf * 0."""
+    from dartkv_amd import _lib
+    from dartkv_amd.prompt import scale_factor
+    with pytest.raises(ValueError, match="scale"):
+        scale_factor(scale, 64, "prompt_attention")
+    assert scale_factor(1e-37, 64, "prompt_attention") == 1e-37
+    a = _lib.PromptAttentionArgs(query=256, keys=256, values=256, out=256, requests=1, Hq=4, Hkv=2, D=64, q_tokens=8,
+                                 k_tokens=8, dtype=2, scale=scale, causal=1)
+    b = _lib.BlockAttentionArgs(query=256, out=256, dtype=2, q_st=128, q_sh=32, o_st=128, o_sh=32, tokens=4, starts=256,
+                                table=256, lengths=256, requests=2, max_blocks=4, blocks=8, block_size=16, key_codes=256,
+                                value_codes=256, key_scale=256, value_scale=256, Hq=4, Hkv=2, D=32, scale=scale,
+                                max_tokens=4, workspace=256, workspace_bytes=1 << 40)
+    lib = _lib.load()
+    for entry, args in ((lib.dkv_prompt_attention, a), (lib.dkv_block_attention, b)):
+        assert entry(args, None) == 1 and "scale" in lib.dkv_last_error().decode()
