@@ -71,6 +71,14 @@ def aligned_rows(t: torch.Tensor, token_axis: int) -> torch.Tensor:
     return t
 
 
+def new_output(query: torch.Tensor) -> torch.Tensor:
+    """The output of a call without ``out``: of the query's layout where that has rows of D, else contiguous."""
+    out = torch.empty_like(query)
+    if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]):
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    return out
+
+
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                      query_starts: Optional[torch.Tensor] = None, key_starts: Optional[torch.Tensor] = None, *,
                      causal: bool = True, scale: Optional[float] = None,
@@ -109,7 +117,7 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
             and (fill or not out.data_ptr() % 8):
         no_gradients("prompt_attention", query, keys, values)
         if fill:
-            out = torch.empty_like(query)
+            out = new_output(query)
         a = _lib.PromptAttentionArgs.from_buffer_copy(known)
     else:
         a, query, keys, values, query_starts, key_starts, out, whole = _checked(query, keys, values, query_starts,
@@ -155,18 +163,15 @@ def _checked(query, keys, values, query_starts, key_starts, causal, scale, out):
     if not packed and query.shape[0] != keys.shape[0]:
         raise ValueError("query and keys must have one batch size")
     factor = scale_factor(scale, D, "prompt_attention")
-    fill, whole = out is None, True
+    fill = out is None
     if out is None:
-        out = torch.empty_like(query)
-        if out.stride(-1) != 1 or any(s % 4 for s in out.stride()[:-1]):  # (a query whose layout is not rows of D)
-            out = torch.empty(query.shape, dtype=query.dtype, device=device)
-            whole = False
+        out = new_output(query)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1 \
             or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
         raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
     given = (query, keys, values)
     query, keys, values = (aligned_rows(t, t_axis) for t in given)
-    whole = whole and all(a is b for a, b in zip(given, (query, keys, values)))
+    whole = all(a is b for a, b in zip(given, (query, keys, values)))
 
     a = _lib.PromptAttentionArgs()
     if packed:

@@ -176,7 +176,7 @@ def prompt_attention(query: Tensor, keys: Tensor, values: Tensor, query_starts: 
 
 @prompt_attention.register_fake
 def _(query, keys, values, query_starts=None, key_starts=None, causal=True, scale=None):
-    return torch.empty_like(query)
+    return _prompt.new_output(query)
 
 
 @torch.library.custom_op("dartkv::reserve_blocks", mutates_args=("table", "lengths", "free", "state"))
