@@ -216,6 +216,20 @@ def _(keys, values, slots, key_codes, value_codes, key_scale, value_scale):
     return None
 
 
+# (an operator of its own: torch's custom operators need every argument that they change)
+@torch.library.custom_op("dartkv::append_blocks_reported",
+                         mutates_args=("key_codes", "value_codes", "key_scale", "value_scale", "nonfinite"))
+def append_blocks_reported(keys: Tensor, values: Tensor, slots: Tensor, key_codes: Tensor, value_codes: Tensor,
+                           key_scale: Tensor, value_scale: Tensor, nonfinite: Tensor) -> None:
+    """``append_blocks``, and ``nonfinite`` (int32, one element) becomes 1 where a key or value is not finite."""
+    _blocks.append_blocks(keys, values, slots, key_codes, value_codes, key_scale, value_scale, nonfinite=nonfinite)
+
+
+@append_blocks_reported.register_fake
+def _(keys, values, slots, key_codes, value_codes, key_scale, value_scale, nonfinite):
+    return None
+
+
 @torch.library.custom_op("dartkv::block_attention", mutates_args=())
 def block_attention(query: Tensor, key_codes: Tensor, value_codes: Tensor, key_scale: Tensor, value_scale: Tensor,
                     table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None, max_tokens: Optional[int] = None,
@@ -230,6 +244,6 @@ def _(query, key_codes, value_codes, key_scale, value_scale, table, lengths, sta
     return query.new_empty(query.shape)
 
 
-__all__ = ["append_blocks", "block_attention", "cache_handle", "decode_attention", "dequantize_key_mixed",
-           "dequantize_rows", "prompt_attention", "quantize_key_mixed", "quantize_rows", "release_blocks",
-           "reserve_blocks"]
+__all__ = ["append_blocks", "append_blocks_reported", "block_attention", "cache_handle", "decode_attention",
+           "dequantize_key_mixed", "dequantize_rows", "prompt_attention", "quantize_key_mixed", "quantize_rows",
+           "release_blocks", "reserve_blocks"]
