@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .attention import _workspace
-from .prompt import aligned_rows, int32_vector, no_gradients, scale_factor
+from .prompt import aligned_rows, check_output, int32_vector, no_gradients, scale_factor
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 MAX_BLOCK_HEAD_DIM = 256
@@ -299,9 +299,8 @@ def _checked_attention(query, key_codes, value_codes, key_scale, value_scale, ta
         most = min(most, int(max_tokens))
     factor = scale_factor(scale, D, "block_attention")
     fill = out is None
-    if not fill and (out.shape != query.shape or out.dtype != query.dtype or out.device != device
-                     or out.stride(-1) != 1 or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1])):
-        raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
+    if not fill:
+        check_output(out, query)
     query = aligned_rows(query, 0)
     a = _lib.BlockAttentionArgs()
     a.dtype = _lib.dtype_code(query.dtype)

@@ -79,6 +79,15 @@ def new_output(query: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def check_output(out: torch.Tensor, query: torch.Tensor) -> None:
+    """Refuse an ``out`` that the kernels cannot write: each row of D has to lie by itself."""
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(-1) != 1 \
+            or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
+        raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
+    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError("out must have rows of its own for every token and head")
+
+
 def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
                      query_starts: Optional[torch.Tensor] = None, key_starts: Optional[torch.Tensor] = None, *,
                      causal: bool = True, scale: Optional[float] = None,
@@ -166,9 +175,8 @@ def _checked(query, keys, values, query_starts, key_starts, causal, scale, out):
     fill = out is None
     if out is None:
         out = new_output(query)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != device or out.stride(-1) != 1 \
-            or out.data_ptr() % 8 or any(s % 4 for s in out.stride()[:-1]):
-        raise ValueError("out must be a tensor of the query's shape, dtype and device, with 8-byte aligned rows of D")
+    else:
+        check_output(out, query)
     given = (query, keys, values)
     query, keys, values = (aligned_rows(t, t_axis) for t in given)
     whole = all(a is b for a, b in zip(given, (query, keys, values)))

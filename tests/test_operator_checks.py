@@ -98,3 +98,22 @@ def test_scales_that_vanish_in_fp32_are_refused(scale):
     lib = _lib.load()
     for entry, args in ((lib.dkv_prompt_attention, a), (lib.dkv_block_attention, b)):
         assert entry(args, None) == 1 and "scale" in lib.dkv_last_error().decode()
+
+
+@pytest.mark.gpu
+def test_outputs_whose_rows_share_memory_are_refused():
+    import dartkv_amd as dart
+    q = torch.zeros(6, 4, 64, dtype=torch.bfloat16, device=DEV)
+    starts = torch.tensor([0, 6], dtype=torch.int32, device=DEV)
+    codes = [torch.zeros(2, 2, 16, 64, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.ones(2, 2, device=DEV) for _ in range(2)]
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.full((1,), 6, dtype=torch.int32, device=DEV)
+    calls = (lambda out: dart.prompt_attention(q, q[:, :2], q[:, 2:], starts, out=out),
+             lambda out: dart.block_attention(q, *codes, *scales, table, lengths, starts, out=out))
+    for call in calls:
+        for out in (q.new_zeros(6, 1, 64).expand(-1, 4, -1), q.new_zeros(1, 4, 64).expand(6, -1, -1)):
+            with pytest.raises(ValueError, match="rows of its own"):
+                call(out)
+        call(torch.empty_like(q))
+    one = q.new_zeros(64).expand(1, 1, 64)  # (one row: its strides say nothing)
+    dart.prompt_attention(q[:1, :1], q[:1, :1], q[:1, :1], torch.tensor([0, 1], dtype=torch.int32, device=DEV), out=one)
