@@ -113,7 +113,9 @@ def release_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
                    tokens: Optional[torch.Tensor] = None, *, block_size: int) -> None:
     """Drop the last ``tokens[r]`` tokens of each request (None: all of them; more than it has: all it has) and
     return the blocks in which none is left to the free stack.  The exact inverse of ``reserve_blocks`` with the
-    same counts: rejected draft tokens are given back as they were taken."""
+    same counts: rejected draft tokens are given back as they were taken.  A block that keeps tokens keeps its scale:
+    where a dropped token had raised it, those that come later are as coarse as that left it, until the block begins
+    anew."""
     if tokens is not None and not isinstance(tokens, torch.Tensor):
         raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
     a, tokens = _tables_args("release", table, lengths, free, state, tokens, block_size)
@@ -219,12 +221,14 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     query heads per KV head) the kernel for few rows does all of it, and the output rows of a request that has
     more after all are undefined.  Default: T (without starts 1).
     ``table`` [requests, max_blocks] and ``lengths`` [requests] (int32), the codes and scales as ``append_blocks``
-    writes them.  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
-    makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request and before
-    the first are 0 in a new tensor and stay as they were in ``out``.
+    writes them: the scales have to be powers of two (of others the kernels use different parts; nothing checks that
+    on the device).  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
+    makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request and
+    before the first are 0 in a new tensor and stay as they were in ``out``.
 
-    Statistics and sums are fp32.  Forward only: a query that requires gradients is refused outside
-    torch.no_grad(), forward-mode tangents always.
+    Statistics and sums are fp32; the weights keep 16 bits for the second product, but for a bf16 query's requests of
+    more rows than the kernel for few takes, where they are rounded to bf16.  Forward only: a query that requires
+    gradients is refused outside torch.no_grad(), forward-mode tangents always.
     """
     fill = out is None
     scale = None if scale is None else float(scale)
@@ -334,6 +338,12 @@ class BlockKVCache:
     A step of a serving loop: ``plan = cache.reserve(tokens, total)`` once, then per layer ``cache.append(layer,
     keys, values, plan)`` and ``cache.attention(layer, query, plan)``.  ``release`` gives back a request's last
     tokens, or all of them.  Nothing synchronizes; ``check`` reads the status once and raises.
+
+    ``max_blocks``: the most blocks of a request (default: all).  Attention of chunks plans its parts and workspace for
+    requests of that length, so a bound that the program knows is worth giving.
+
+    A plan of an earlier step, or of another cache, is refused.  Replays of a captured step move the requests on
+    without this object's knowledge: after one, no plan made outside the graph before it may be used.
     """
 
     def __init__(self, requests: int, blocks: int, kv_heads: int, head_dim: int, *, layers: int = 1,
@@ -370,7 +380,8 @@ class BlockKVCache:
 
     def reserve(self, tokens: torch.Tensor, total: int, *, max_tokens: Optional[int] = None) -> BlockPlan:
         """Room for ``tokens[r]`` new tokens of each request (``reserve_blocks``).  ``max_tokens``: the most of
-        them, where the caller knows it; a request with more is left out of ``attention``."""
+        them, where the caller knows it (default ``total``); ``attention`` leaves the rows of a request with more
+        undefined.  A decode step without it also launches the kernel for chunks, which finds nothing to do."""
         slots, starts = reserve_blocks(self.table, self.lengths, self.free, self.state, tokens, total,
                                        block_size=self.block_size)
         self._step = next(_steps)

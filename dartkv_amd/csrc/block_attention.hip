@@ -4,9 +4,10 @@
 // kscale[block, head], v = code * vscale[block, head].
 //
 // Bound: the cache's bytes, 2 D per key and KV head; one wave reads 32 keys and values (64 D bytes) while it computes
-// the 32 before, eight waves a CU keep 64 KB in flight at head_dim 128.  64 requests of 2,048 to 32,768 tokens, 8 KV
-// heads of 128: 382 us, 5.9 TB/s (a copy reaches 4.8), and 7 to join the shares.  One request of 4,000: 8.5 us, the chain
-// of loads from the lengths to the keys, and 5.6.
+// the 32 before: eight waves a CU keep 64 KB in flight at head_dim 128, 32 KB at 64, and the four that fit at 256 64 KB.
+// 64 requests of 2,048 to 32,768 tokens, 8 KV heads of 128: 382 us, 5.9 TB/s (a copy reaches 4.7), and 7 to join the
+// shares.  64 requests of 16,000, the whole call: head_dim 64 198 us, 5.3 TB/s; 128 372 us, 5.6; 256 710 us, 5.9; 16 of
+// 8,000: 3.7, 4.8 and 4.5 TB/s.  One request of 4,000: 9 us, the chain of loads from the lengths to the keys, and 6.
 //
 // Work.  The requests' 32-key tiles are one line of units per KV head, cut into equal shares: a wave takes its
 // share, whatever requests it covers, so ragged lengths leave no wave waiting for another.  A wave writes the
@@ -602,7 +603,7 @@ void launch_decode(const BlockParams& bp, hipStream_t stream) {
     hipLaunchKernelGGL((block_merge<BF, true>), dim3((unsigned)rows), dim3(kThreads), 0, stream, bp);
 }
 
-// Waves of a KV head: two resident on each of 1,024 SIMDs, one round.
+// Waves of a KV head: two for each of 1,024 SIMDs, resident at once; head_dims over 128 leave one, and two rounds.
 int workers_for(int64_t H) {
   const int64_t w = (2048 + H - 1) / H;
   return (int)(w < 1 ? 1 : w);

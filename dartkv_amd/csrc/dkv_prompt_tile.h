@@ -1,5 +1,5 @@
 // Attention of a tile of query rows over a request's keys (gfx950, wave64): the kernel of prompt_attention
-// (16-bit keys and values, prompt.hip) and of block_attention's long chunks (e4m3 blocks, blocks_chunk.hip).
+// (16-bit keys and values, prompt.hip) and of block_attention's long chunks (e4m3 blocks, block_chunks.hip).
 //
 // Rows.  The query heads of a KV head are rows of one problem: row t * G + g is token t of head h * G + g, so a
 // tile of BM rows reads its keys once for all G heads, and a causal tile of 128 rows masks no more than 128 / G
@@ -24,10 +24,18 @@
 // Two buffers of 64 keys (32 where registers are short); the next tile's copies are in flight while a tile is computed,
 // one barrier a tile.
 //
-// Bound and measured.  16,384 tokens of 32 query heads of 128, bf16: 1.96-2.0 ms, 1.1 PFLOP/s.  The matrix units are busy
-// 54 % of the cycles, at 1.65 GHz: the power limit holds the clock down as the kernel gets denser (1.77 GHz at 48 %; a
-// 16,384^3 matrix product reaches 1.37 PFLOP/s).  LDS 27 % busy.  A single short prompt is bound by its last tiles and
-// about 8 us of start and end.
+// Fewer bits.  l sums p in fp32; for the second product p is rounded to the operands' type (prompts, and chunks under bf16
+// queries), half a step each.  In bf16 that takes the error from 1.6e-3 of the result's norm, which is the result's own
+// rounding, to 2.1e-3.  p in two bf16 parts, as chunks under fp16 queries have it, leaves 1.6e-3 and costs half of all
+// products again: 16,384 tokens 2,740 us in place of 1,980, 16 ragged prompts 977 and 752, 1,024 tokens 32.7 and 26.7.
+//
+// Bound and measured.  16,384 tokens of 32 query heads of 128, bf16: 1.95-2.01 ms, 1.1 PFLOP/s.  Matrix units busy 53 % of
+// the cycles, vector units 46 %, LDS 27 %, at 1.78-1.91 GHz (counters and times of the same launches); a 16,384^3 matrix
+// product keeps the matrix units busy 72 % at 1.81 GHz, 1.37 PFLOP/s.  So it is the exponentials and maxima between the
+// products that hold it, not the clock.  Ragged prompts of 64 to 4,096 tokens: 45 % busy, the vector units the same: about
+// 18 key tiles a workgroup, whose start and end cost about four.  A single short prompt is bound by its last tiles and
+// about 8 us of start and end.  Chunks over blocks: 35 % and 39 % busy at 2.1 GHz, as a stage's conversion into LDS stands
+// between two barriers.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

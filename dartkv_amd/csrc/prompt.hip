@@ -103,7 +103,7 @@ extern "C" int dkv_prompt_attention(const dkv_prompt_attention_args* args, void*
                     0 &&
                 (((uintptr_t)a.out | (uintptr_t)(2 * (a.o_sb | a.o_st | a.o_sh))) & 7) == 0,
             DKV_ERR_INVALID, "dkv_prompt_attention: rows must be 16-byte aligned (output rows 8-byte)");
-  // offsets within a tile of 64 keys are 31-bit
+  // offsets within a stage of up to 128 keys are 31-bit
   DKV_CHECK(a.k_st >= 0 && a.v_st >= 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23), DKV_ERR_INVALID,
             "dkv_prompt_attention: token strides of keys and values must be under 2^23 elements");
   PromptParams p = {};

@@ -23,7 +23,7 @@ MAX_PROMPT_HEAD_DIM = 256
 
 
 def followed(*tensors: torch.Tensor) -> bool:
-    """Whether autograd would follow an operation on one of the tensors, backward or (which no_grad leaves on) forward."""
+    """Whether autograd would follow an operation on a tensor, backward or (which no_grad leaves on) forward."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         return True
     # (the level is -1 outside forward_ad.dual_level(), where no tensor has a tangent)
@@ -106,7 +106,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
     the first are 0 in a new tensor and stay as they were in ``out``.  Keys a row does not see do not change it,
     whatever they hold.
 
-    Softmax statistics and sums are fp32; the weights are rounded to the tensors' type for the second product.
+    Softmax statistics and sums are fp32; the weights are rounded to the tensors' type for the second product (fp16:
+    with 2^7 of its range in hand, so that weights down to 2^-21 of the largest keep all its bits).
     Forward only: tensors that require gradients are refused outside torch.no_grad(), forward-mode tangents always.
     """
     packed = query_starts is not None

@@ -505,7 +505,8 @@ int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
  * their first places.  Stack entries that are taken become -1.
  * dkv_release_blocks drops the last tokens[r] of each request (all of them when
  * tokens is NULL, or more than it has) and returns the blocks that no token is
- * left in; it undoes a reserve of the same counts exactly.
+ * left in; it undoes a reserve of the same counts exactly (a block that keeps
+ * tokens keeps its scale).
  *
  * A call that cannot be met changes nothing but the status, where it sets 1
  * (too few free blocks), 2 (a request needs more than max_blocks), 4 (a
@@ -564,11 +565,12 @@ int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream);
  * fill: rows behind starts[requests] and before starts[0] become 0 (0: they are
  * left as they were).
  * max_tokens: no request has more new tokens (the rows of a request that has
- * more are undefined).  Bytes of blocks behind a request's length are not used; a
- * table entry outside [0, blocks) makes the rows that see it NaN.  scale from
- * 1e-37 to 1e30 (not included).  D a multiple of 16 up to 256.  workspace (16-byte aligned):
- * dkv_block_attention_workspace_bytes of the same arguments (pointers are not
- * looked at); its contents need not be kept.
+ * more are undefined).  Scales are powers of two, as dkv_append_blocks writes
+ * them; others give undefined results.  Bytes of blocks behind a request's
+ * length are not used; a table entry outside [0, blocks) makes the rows that see
+ * it NaN.  scale from 1e-37 to 1e30 (not included).  D a multiple of 16 up to
+ * 256.  workspace (16-byte aligned): dkv_block_attention_workspace_bytes of the
+ * same arguments (pointers are not looked at); its contents need not be kept.
  */
 typedef struct dkv_block_attention_args {
   const void* query;
