@@ -5,7 +5,7 @@
 //
 // Bound: the cache's bytes, 2 D per key and KV head; one wave reads 32 keys and values (64 D bytes) while it computes
 // the 32 before: eight waves a CU keep 64 KB in flight at head_dim 128, 32 KB at 64, and the four that fit at 256 64 KB.
-// 64 requests of 2,048 to 32,768 tokens, 8 KV heads of 128: 382 us, 5.9 TB/s (a copy reaches 4.7), and 7 to join the
+// 64 requests of 2,048 to 32,768 tokens, 8 KV heads of 128: 397 us, 5.7 TB/s (a copy reaches 4.7), and 7 to join the
 // shares.  64 requests of 16,000, the whole call: head_dim 64 198 us, 5.3 TB/s; 128 372 us, 5.6; 256 710 us, 5.9; 16 of
 // 8,000: 3.7, 4.8 and 4.5 TB/s.  One request of 4,000: 9 us, the chain of loads from the lengths to the keys, and 6.
 //

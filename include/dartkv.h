@@ -500,9 +500,9 @@ int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
  *
  * dkv_reserve_blocks gives request r tokens[r] new tokens behind its lengths[r]
  * and the blocks they need, from the top of the stack in the requests' order.
- * slots [total] (int64) becomes block * block_size + offset of every new token,
- * packed in the requests' order, and -1 behind the last; starts [requests + 1]
- * their first places.  Stack entries that are taken become -1.
+ * slots [total] (int64, 16-byte aligned) becomes block * block_size + offset of
+ * every new token, packed in the requests' order, and -1 behind the last; starts
+ * [requests + 1] their first places.  Stack entries that are taken become -1.
  * dkv_release_blocks drops the last tokens[r] of each request (all of them when
  * tokens is NULL, or more than it has) and returns the blocks that no token is
  * left in; it undoes a reserve of the same counts exactly (a block that keeps

@@ -130,3 +130,26 @@ def test_appends_of_many_tokens(dtype, H, D, bs, R, sizes):
     assert max(sizes) * R * H > 16384
     for got, w in zip(pool, want):
         _same_values(got, w)
+
+
+@pytest.mark.gpu
+def test_tables_of_the_most_requests():
+    """8,190 requests, whose prefix sums take 96 KiB of LDS; one more is refused."""
+    import dartkv_amd as dart
+    from tests.test_blocks import TableModel, _same_state
+    R, bs, most = 8190, 16, 3
+    rng = random.Random(1)
+    state, model = _state(R, R * most, most), TableModel(R, R * most, most, bs)
+    for _ in range(2):
+        counts = [rng.choice([0, 1, rng.randint(0, 20)]) for _ in range(R)]
+        total = sum(counts) + 5
+        slots, starts = dart.reserve_blocks(*state, torch.tensor(counts, dtype=torch.int32, device=DEV), total, block_size=bs)
+        want_slots, want_starts = model.reserve(counts, total)
+        assert slots.cpu().tolist() == want_slots and starts.cpu().tolist() == want_starts
+        _same_state(state, model)
+        drop = [rng.randint(0, 9) for _ in range(R)]
+        dart.release_blocks(*state, torch.tensor(drop, dtype=torch.int32, device=DEV), block_size=bs)
+        model.release(drop)
+        _same_state(state, model)
+    with pytest.raises(ValueError, match="8190"):
+        dart.release_blocks(*_state(R + 1, R, 1), block_size=bs)
