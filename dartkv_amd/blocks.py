@@ -224,7 +224,8 @@ def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: t
     writes them: the scales have to be powers of two (of others the kernels use different parts; nothing checks that
     on the device).  Bytes of a block behind its request's length are not used.  A table entry outside the blocks
     makes the rows that see it NaN.  Returns a tensor like ``query``, or ``out``; rows behind the last request and
-    before the first are 0 in a new tensor and stay as they were in ``out``.
+    before the first are 0 in a new tensor and stay as they were in ``out``.  ``scale`` (1e-37 to 1e30) defaults to
+    1 / sqrt(D).
 
     Statistics and sums are fp32; the weights keep 16 bits for the second product, but for a bf16 query's requests of
     more rows than the kernel for few takes, where they are rounded to bf16.  Forward only: a query that requires

@@ -161,7 +161,7 @@ __device__ __forceinline__ int64_t clamped(int64_t x, int64_t lo, int64_t hi) { 
 
 // The requests' tiles one after the other, those of more keys first (up to 64 requests; else in their order), found
 // by a wave's scan over the requests: the longest work begins first, and what begins last is short.  Rows to fill are one
-// more request without keys, from the last request's end round to the first's start (`token_at`).
+// more request without keys, from the last request's end round to the first's start.
 template <int BM, bool BLOCKS>
 __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) {
   Tile t = {-1, 0, 0, 0, 0, 0, 0};
@@ -229,10 +229,18 @@ __device__ __forceinline__ Tile find_tile(const PromptParams& p, int64_t index) 
   return t;
 }
 
-// The place of a request's token in the packed tensors (those of the rows to fill go round their end).
-__device__ __forceinline__ int64_t token_at(const PromptParams& p, const Tile& t, int token) {
-  const int64_t at = t.q0 + token;
-  return at < p.q_tokens ? at : at - p.q_tokens;
+// A tile of the rows to fill, which go round the end of the packed tensor: a way of its own, so that the kernel around it
+// keeps its registers (head_dim 256: 4 % of a prompt's time with the wrap in every tile's addresses).
+template <int BM>
+__device__ __forceinline__ void fill_tile(const PromptParams& p, const Tile& t, int h) {
+  const int pieces = p.D / 4;
+  for (int i = threadIdx.x; i < BM * pieces; i += blockDim.x) {
+    const int row = t.tile * BM + i / pieces;
+    if (row >= t.rows) return;
+    int64_t at = t.q0 + row / p.G;
+    if (at >= p.q_tokens) at -= p.q_tokens;
+    *(u32x2*)((uint16_t*)p.o + at * p.o_st + (h * p.G + row % p.G) * p.o_sh + i % pieces * 4) = (u32x2){0, 0};
+  }
 }
 
 // A product adds 0 * v for a key that its row does not see, or whose weight is too small for its type, which is NaN where
@@ -394,13 +402,17 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
     const int tiles = (t.rows + BM - 1) / BM, late = t.tile - (tiles + 1) / 2;
     t.tile = p.pairs && late >= 0 ? late : tiles - 1 - t.tile;  // the longest tiles first
   }
+  if (t.request == p.R) {
+    if (part == 0) fill_tile<BM>(p, t, h);
+    return;
+  }
   const int nk = t.nk;
 
   // this lane's row, how many keys it sees, and its query in the products' operand layout
   const int row = t.tile * BM + wave * 32 + (lane & 31);
   const bool real = row < t.rows;
   const int token = row / p.G, head = h * p.G + row % p.G;
-  const int64_t qb = p.q_starts ? 0 : t.request, place = token_at(p, t, token);
+  const int64_t qb = p.q_starts ? 0 : t.request;
   auto limit_of = [&](int tok) {
     int n = p.causal ? tok + 1 + nk - t.nq : nk;
     return n < 0 ? 0 : n > nk ? nk : n;
@@ -447,7 +459,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
 
   u32x4 q[KS];
   {
-    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + place * p.q_st + head * p.q_sh);
+    const char* src = (const char*)p.q + 2 * (qb * p.q_sb + (t.q0 + token) * p.q_st + head * p.q_sh);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int ch = 16 * ks + 8 * half;
@@ -673,7 +685,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 64 && !BLOCKS && GROUPS == 1
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* dst = (char*)p.o + 2 * (qb * p.o_sb + place * p.o_st + head * p.o_sh);
+  char* dst = (char*)p.o + 2 * (qb * p.o_sb + (t.q0 + token) * p.o_st + head * p.o_sh);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
