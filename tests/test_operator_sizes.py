@@ -153,3 +153,30 @@ def test_tables_of_the_most_requests():
         _same_state(state, model)
     with pytest.raises(ValueError, match="8190"):
         dart.release_blocks(*_state(R + 1, R, 1), block_size=bs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_single_tokens_of_many_requests(dtype):
+    import dartkv_amd as dart
+    rng = random.Random(5)
+    lengths = [rng.choice([1, 16, rng.randint(1, 60)]) for _ in range(2000)] + [3000, 1]
+    cache = _cache(lengths, 2, 64, 16, 9)
+    q = _query(len(lengths), 8, 64, dtype, 2)
+    _check_attention(dart.block_attention(q, *cache), q, cache, [1] * len(lengths), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunks_among_more_than_64_requests(dtype, D):
+    """The kernel for few rows takes the requests of up to 16 rows, the chunk kernel finds the others among all."""
+    import dartkv_amd as dart
+    rng = random.Random(6)
+    new = [rng.choice([0, 1, 1, 1, 4, 5, 40]) for _ in range(150)] + [100, 0, 1]
+    lengths = [max(1, n) + rng.randint(0, 70) for n in new]
+    cache = _cache(lengths, 2, D, 16, D)
+    q = _query(sum(new) + 3, 8, D, dtype, 3)
+    got = dart.block_attention(q, *cache, _starts(new))
+    _check_attention(got, q, cache, new, dtype, chunk=True)
+    assert bool((got[sum(new):] == 0).all())
