@@ -246,9 +246,9 @@ def _prepare_store(case, seed):
     starts = torch.tensor(_starts(new), dtype=torch.int32).cuda()
     wq, wk = _weights(case, seed)
     pools = {n: t[0] for n, t in _pools(case, seed, 1, blocks).items()}
-    slots, _ = _slots(state["table"], state["lengths"] - (starts[1:] - starts[:-1]), starts, total, bs)
+    slots, positions = _slots(state["table"], state["lengths"] - (starts[1:] - starts[:-1]), starts, total, bs)
     return {**state, **pools, "kind": "store", "q": q, "k": k, "v": v, "cos": cos, "sin": sin, "wq": wq, "wk": wk,
-            "next": case["pairs"] == "next", "starts": starts, "slots": slots}
+            "next": case["pairs"] == "next", "positions": positions.to(torch.int32), "slots": slots}
 
 
 def _forks(case):
@@ -344,8 +344,8 @@ def _run_own(state):
         grads = torch.autograd.grad(out, state["leaves"], state["given"]) if state["grad"] else ()
         return [*(t.detach() for t in out), *grads]
     if kind == "store":
-        q = dart.append_rotated_blocks(state["q"], state["k"], state["v"], state["cos"], state["sin"], state["slots"],
-                                       state["starts"], state["lengths"], *_pool_of(state), q_weight=state["wq"],
+        q = dart.append_rotated_blocks(state["q"], state["k"], state["v"], state["cos"], state["sin"],
+                                       state["positions"], state["slots"], *_pool_of(state), q_weight=state["wq"],
                                        k_weight=state["wk"], eps=EPS, interleaved=state["next"])
         return [q, *_pool_of(state)]
     if kind == "fork":
@@ -430,9 +430,7 @@ def _slots(table, before, starts, total, bs):
 
 
 def _store_plain(state):
-    starts = state["starts"]
-    slots, at = _slots(state["table"], state["lengths"] - (starts[1:] - starts[:-1]), starts, state["q"].shape[0],
-                       state["bs"])
+    slots, at = state["slots"], state["positions"].long()
     cos, sin = state["cos"][at], state["sin"][at]
     q = _turned(state["q"], state["wq"], cos, sin, state["next"]).to(state["q"].dtype)
     # (in 64 bits: a key next to the border of two codes, or of two scales, goes to its own side)
@@ -725,7 +723,7 @@ def work(case):
         touched = sum(-(-n // bs) - (n - m) // bs for n, m in zip(lengths, new))
         size = DTYPES[case["dtype"]].itemsize
         row = D * H * (2 * case["G"] * size + 2 * size + 2)
-        return {"bytes": tokens * (row + 4 * case["rotated"] + 8) + touched * 16 * H, "flops": tokens * D * H * 8 * (case["G"] + 2)}
+        return {"bytes": tokens * (row + 4 * case["rotated"] + 12) + touched * 16 * H, "flops": tokens * D * H * 8 * (case["G"] + 2)}
     layers = case["layers"]
     if kind == "fork":
         _, lengths, sources, _ = _forks(case)
