@@ -26,7 +26,7 @@ KEY_DENSE, KEY_UNIFORM, KEY_MIXED = 0, 1, 2
 VALUE_DENSE, VALUE_UNIFORM = 0, 1
 SELECT_MAGNITUDE, SELECT_VARIANCE, SELECT_GIVEN = 0, 1, 2
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}
 # element types the kernels read and write (sources, outputs, metadata)
@@ -163,7 +163,38 @@ class PromptAttentionArgs(ctypes.Structure):
 
 
 class BlockTablesArgs(ctypes.Structure):
-    _fields_ = _fields("table lengths free state tokens slots starts", "total requests max_blocks blocks block_size")
+    _fields_ = [
+        *_fields("table lengths free state tokens slots starts", "total requests max_blocks blocks block_size"),
+        *_fields("shares copies sources positions workspace", "workspace_bytes"),
+    ]
+
+
+class CopyBlocksArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("copies", "count layers blocks H block_size D"),
+        *_fields("key_codes value_codes key_scale value_scale", "key_stride value_stride key_scale_stride value_scale_stride"),
+    ]
+
+
+class RotateHeadsArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("query keys q_out k_out q_grad k_grad", "q_sb q_st q_sh k_sb k_st k_sh qo_sb qo_st qo_sh ko_sb ko_st ko_sh "
+                 "qg_sb qg_st qg_sh kg_sb kg_st kg_sh"),
+        *_fields("q_weight k_weight q_weight_grad k_weight_grad cos sin positions",
+                 "c_sb c_st table_rows wide_positions batch tokens Hq Hkv D half interleaved dtype weight_dtype angle_dtype"),
+        ("eps", ctypes.c_double), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [
+        *_fields("logits tokens logprobs entropy stats top_logprobs top_tokens", "stride rows vocab top dtype wide_tokens"),
+        *_fields("workspace", "workspace_bytes"),
+    ]
+
+
+class TokenLogprobsGrads(ctypes.Structure):
+    _fields_ = _fields("logprobs entropy top_logprobs out", "stride")
 
 
 class AppendBlocksArgs(ctypes.Structure):
@@ -191,6 +222,10 @@ EXPORTED = (
     "dkv_decode_scratch_bytes", "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize",
     "dkv_decode_route", "dkv_prompt_attention", "dkv_reserve_blocks", "dkv_release_blocks", "dkv_append_blocks",
     "dkv_block_attention", "dkv_block_attention_workspace_bytes", "dkv_prompt_attention_workspace_bytes",
+    "dkv_fork_blocks", "dkv_compact_blocks", "dkv_share_workspace_bytes", "dkv_copy_blocks",
+    "dkv_append_rotated_blocks", "dkv_rotate_heads", "dkv_rotate_heads_backward",
+    "dkv_rotate_heads_backward_workspace_bytes", "dkv_token_logprobs", "dkv_token_logprobs_backward",
+    "dkv_token_logprobs_workspace_bytes",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -238,12 +273,24 @@ def load() -> ctypes.CDLL:
         lib.dkv_prompt_attention_workspace_bytes.restype = i64
         lib.dkv_block_attention_workspace_bytes.argtypes = [ctypes.POINTER(BlockAttentionArgs)]
         lib.dkv_block_attention_workspace_bytes.restype = i64
+        for name, args in (("dkv_fork_blocks", BlockTablesArgs), ("dkv_compact_blocks", BlockTablesArgs),
+                           ("dkv_copy_blocks", CopyBlocksArgs), ("dkv_rotate_heads", RotateHeadsArgs),
+                           ("dkv_rotate_heads_backward", RotateHeadsArgs), ("dkv_token_logprobs", TokenLogprobsArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), vp]
+        lib.dkv_append_rotated_blocks.argtypes = [ctypes.POINTER(AppendBlocksArgs), ctypes.POINTER(RotateHeadsArgs), vp]
+        lib.dkv_token_logprobs_backward.argtypes = [ctypes.POINTER(TokenLogprobsArgs), ctypes.POINTER(TokenLogprobsGrads), vp]
+        for name, args in (("dkv_share_workspace_bytes", BlockTablesArgs),
+                           ("dkv_rotate_heads_backward_workspace_bytes", RotateHeadsArgs),
+                           ("dkv_token_logprobs_workspace_bytes", TokenLogprobsArgs)):
+            getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.POINTER(args)], i64
         for name in ("dkv_quantize_rows", "dkv_quantize_row_blocks", "dkv_quantize_value_rows", "dkv_quantize_key_pages",
                      "dkv_dequantize_rows",
                      "dkv_dequantize_mixed", "dkv_decode_attention", "dkv_decode_attention_noalloc",
                      "dkv_decode_prep", "dkv_copy_token_blocks", "dkv_materialize", "dkv_decode_route",
                      "dkv_prompt_attention", "dkv_reserve_blocks", "dkv_release_blocks", "dkv_append_blocks",
-                     "dkv_block_attention"):
+                     "dkv_block_attention", "dkv_fork_blocks", "dkv_compact_blocks", "dkv_copy_blocks",
+                     "dkv_append_rotated_blocks", "dkv_rotate_heads", "dkv_rotate_heads_backward", "dkv_token_logprobs",
+                     "dkv_token_logprobs_backward"):
             getattr(lib, name).restype = ctypes.c_int
         if lib.dkv_abi_version() != ABI_VERSION:
             raise RuntimeError("libdartkv_hip.so ABI version mismatch; rebuild it")

@@ -5,7 +5,11 @@ different lengths that begin and end at different times; here each holds blocks 
 pool, in e4m3 with one power-of-two scale per block and KV head:
 
 * ``reserve_blocks`` / ``release_blocks``: block tables and slot maps from the requests' lengths;
-* ``append_blocks``: new keys and values into their slots;
+* ``fork_blocks``: rows that become copies of others, by holding the same blocks (``shares``); a row that writes into a
+  block of others gets a copy of its own when it reserves, whose contents ``copy_blocks`` copies;
+* ``compact_blocks``: the blocks in use move to the lowest numbers;
+* ``append_blocks``: new keys and values into their slots, and ``append_rotated_blocks`` with the norm and the rotation
+  of queries and keys before;
 * ``block_attention``: attention of each request's newest tokens over its blocks;
 * ``BlockKVCache``: the tensors of all that for a model's layers, and the calls on them.
 
@@ -23,6 +27,7 @@ import torch
 from . import _lib
 from .attention import _workspace
 from .prompt import aligned_rows, check_output, int32_vector, no_gradients, scale_factor
+from .rotate import check_angles, check_weights, set_angles
 
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 MAX_BLOCK_HEAD_DIM = 256
@@ -30,7 +35,8 @@ MAX_REQUESTS = 8190
 CODE_DTYPE = torch.float8_e4m3fn
 
 _STATUS = ((1, "too few free blocks"), (2, "a request needs more than max_blocks blocks"),
-           (4, "a negative token count"), (8, "more new tokens than total"))
+           (4, "a negative token count"), (8, "more new tokens than total"),
+           (16, "a source that is not a request"))
 
 
 def _check_state(table, lengths, free, state, block_size) -> torch.device:
@@ -50,14 +56,26 @@ def _check_state(table, lengths, free, state, block_size) -> torch.device:
     return device
 
 
-def _tables_args(name, table, lengths, free, state, tokens, block_size):
+def _check_shares(shares, free) -> None:
+    if not isinstance(shares, torch.Tensor) or shares.dtype != torch.int32 or not shares.is_contiguous():
+        raise TypeError("shares must be a contiguous int32 tensor of 1 dimension(s)")
+    if shares.shape != free.shape or shares.device != free.device:
+        raise ValueError("shares must be [blocks], on the tables' device")
+
+
+def _tables_args(name, table, lengths, free, state, tokens, block_size, shares=None):
     """Checked arguments of a call on the tables' state, and the counts as an int32 vector."""
-    key = (name, block_size, _lib.layouts(table, lengths, free, state, *(() if tokens is None else (tokens,))))
+    key = (name, block_size, tokens is None, shares is None,
+           _lib.layouts(table, lengths, free, state, *(t for t in (tokens, shares) if t is not None)))
     known = _lib.template(key)
-    if known is None:
+    if known is None or (shares is not None and shares.data_ptr() % 16):
         device = _check_state(table, lengths, free, state, block_size)
+        if shares is not None:
+            _check_shares(shares, free)
         a = _lib.BlockTablesArgs()
         a.requests, a.max_blocks, a.blocks, a.block_size = table.shape[0], table.shape[1], free.shape[0], block_size
+        if shares is not None and name != "reserve":
+            a.workspace_bytes = _lib.load().dkv_share_workspace_bytes(a)
         if tokens is not None:
             checked = _counts(tokens, lengths, device)
             if checked is tokens:
@@ -70,7 +88,18 @@ def _tables_args(name, table, lengths, free, state, tokens, block_size):
     a.table, a.lengths, a.free, a.state = table.data_ptr(), lengths.data_ptr(), free.data_ptr(), state.data_ptr()
     if tokens is not None:
         a.tokens = tokens.data_ptr()
+    if shares is not None:
+        a.shares = shares.data_ptr()
     return a, tokens
+
+
+def _launch_shared(function, a, device, where) -> None:
+    """A call whose workspace is the calls' of its stream."""
+    stream = _lib.stream_ptr(device)
+    if a.workspace_bytes:
+        workspace = _workspace(device, a.workspace_bytes, stream)
+        a.workspace = workspace.data_ptr()
+    _lib.launch(function, a, device, where, stream)
 
 
 def _counts(tokens, lengths, device) -> torch.Tensor:
@@ -81,8 +110,10 @@ def _counts(tokens, lengths, device) -> torch.Tensor:
 
 
 def reserve_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, state: torch.Tensor,
-                   tokens: torch.Tensor, total: int, *, block_size: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Room for ``tokens[r]`` new tokens behind each request's ``lengths[r]``: returns (slots, starts).
+                   tokens: torch.Tensor, total: int, *, block_size: int, shares: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, ...]:
+    """Room for ``tokens[r]`` new tokens behind each request's ``lengths[r]``: returns (slots, starts), and with
+    ``shares`` (slots, starts, copies).
 
     ``table`` [requests, max_blocks], ``lengths`` [requests], ``free`` [blocks] and ``state`` [4] (int32, on the
     device) are the tables' state and are updated in place: ``free[:state[0]]`` is the stack of free blocks, of
@@ -91,35 +122,140 @@ def reserve_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     (int64) is block * block_size + offset of each packed token, -1 behind the last; ``starts`` [requests + 1]
     (int32) each request's first place.
 
+    ``shares`` [blocks] (int32), where requests were forked: a request that gets tokens in a block that others hold
+    takes a block for a copy of it first; of the writers of one call that are all its holders the last keeps it.
+    ``copies`` [requests, 3] (int32) holds (block, copy, tokens) of each, -1 behind the last: ``copy_blocks`` has to
+    make them before the tokens are appended.  ``positions`` [total] (int32) gets each packed token's position in its
+    request, -1 behind the last.
+
     Nothing is read back: a call that cannot be met (too few free blocks, more than max_blocks, a negative count,
     more tokens than total) changes nothing but ``state[1]``, and its slots are -1 and its starts 0, so that
     appends and attention of that call do nothing (``BlockKVCache.check`` raises).
     """
     if not isinstance(tokens, torch.Tensor):
         raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
-    a, tokens = _tables_args("reserve", table, lengths, free, state, tokens, block_size)
+    a, tokens = _tables_args("reserve", table, lengths, free, state, tokens, block_size, shares)
     total = int(total)
     if not 0 <= total < 1 << 31:
         raise ValueError("total must not be negative")
     device = table.device
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != (total,) or positions.device != device \
+                or not positions.is_contiguous() or positions.data_ptr() % 16:
+            raise ValueError("positions must be an aligned contiguous int32 [total] tensor on the tables' device")
+        a.positions = positions.data_ptr()
     slots = torch.empty(total, dtype=torch.int64, device=device)
     starts = torch.empty(a.requests + 1, dtype=torch.int32, device=device)
     a.slots, a.starts, a.total = slots.data_ptr(), starts.data_ptr(), total
+    if shares is None:
+        _lib.launch(_lib.load().dkv_reserve_blocks, a, device, "dkv_reserve_blocks")
+        return slots, starts
+    copies = torch.empty(a.requests, 3, dtype=torch.int32, device=device)
+    a.copies = copies.data_ptr()
     _lib.launch(_lib.load().dkv_reserve_blocks, a, device, "dkv_reserve_blocks")
-    return slots, starts
+    return slots, starts, copies
 
 
 def release_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, state: torch.Tensor,
-                   tokens: Optional[torch.Tensor] = None, *, block_size: int) -> None:
+                   tokens: Optional[torch.Tensor] = None, *, block_size: int,
+                   shares: Optional[torch.Tensor] = None) -> None:
     """Drop the last ``tokens[r]`` tokens of each request (None: all of them; more than it has: all it has) and
     return the blocks in which none is left to the free stack.  The exact inverse of ``reserve_blocks`` with the
     same counts: rejected draft tokens are given back as they were taken.  A block that keeps tokens keeps its scale:
     where a dropped token had raised it, those that come later are as coarse as that left it, until the block begins
-    anew."""
+    anew.
+
+    ``shares`` [blocks] (int32), where requests were forked: a block returns when no request holds it any more, and those
+    of a call return in the order of their numbers, the lowest on top of the stack."""
     if tokens is not None and not isinstance(tokens, torch.Tensor):
         raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
-    a, tokens = _tables_args("release", table, lengths, free, state, tokens, block_size)
-    _lib.launch(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
+    a, tokens = _tables_args("release", table, lengths, free, state, tokens, block_size, shares)
+    _launch_shared(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
+
+
+def fork_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, state: torch.Tensor,
+                shares: torch.Tensor, sources: torch.Tensor, tokens: Optional[torch.Tensor] = None, *,
+                block_size: int) -> None:
+    """Make request r a copy of what request ``sources[r]`` was before the call, or of its first ``tokens[r]`` tokens
+    (None, or more than it has: all); -1 leaves a request as it is.  All requests change at once, so beams go on from
+    each other in any order.  What they held before returns to the stack where no request holds it any more, the lowest
+    number on top.
+
+    No block is copied: both requests hold it, and ``shares`` [blocks] (int32, zeros at the start) counts the holders
+    beside one.  From then on every call on these tables has to be given ``shares``.  A source that is not a request, or
+    a negative count, leaves its request as it was and sets ``state[1]`` (``BlockKVCache.check`` raises)."""
+    if not isinstance(sources, torch.Tensor) or not (tokens is None or isinstance(tokens, torch.Tensor)):
+        raise TypeError("sources and tokens must be one-dimensional int32 or int64 tensors")
+    if not isinstance(shares, torch.Tensor):
+        raise TypeError("shares must be a contiguous int32 tensor of 1 dimension(s)")
+    a, tokens = _tables_args("fork", table, lengths, free, state, tokens, block_size, shares)
+    sources = int32_vector(sources, "sources", table.device)
+    if sources.numel() != lengths.numel():
+        raise ValueError("sources must hold one request per request")
+    a.sources = sources.data_ptr()
+    _launch_shared(_lib.load().dkv_fork_blocks, a, table.device, "dkv_fork_blocks")
+
+
+def compact_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, state: torch.Tensor,
+                   shares: Optional[torch.Tensor] = None, *, block_size: int) -> torch.Tensor:
+    """Move the blocks in use to the lowest numbers, so that the free ones are the highest and the pool behind them can
+    be used otherwise: of n used blocks those numbered n and above go to the free numbers below n, in ascending order.
+    Tables, stack and shares follow; returns the ``copies`` [blocks // 2, 3] (block, new number, block_size), -1 behind
+    the last, which ``copy_blocks`` has to make in every layer.  At most 2^20 blocks.  Slots given before are no longer
+    valid."""
+    a, _ = _tables_args("compact", table, lengths, free, state, None, block_size, shares)
+    a.workspace_bytes = _lib.load().dkv_share_workspace_bytes(a)
+    copies = torch.empty(a.blocks // 2, 3, dtype=torch.int32, device=table.device)
+    a.copies = copies.data_ptr()
+    _launch_shared(_lib.load().dkv_compact_blocks, a, table.device, "dkv_compact_blocks")
+    return copies
+
+
+def copy_blocks(copies: torch.Tensor, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scale: torch.Tensor,
+                value_scale: torch.Tensor) -> None:
+    """For each (block, target, tokens) of ``copies`` [n, 3] (int32): the block's first ``tokens`` tokens and its scales
+    to the block ``target``, in every layer of ``key_codes``, ``value_codes`` [layers, blocks, heads, block_size,
+    head_dim] (e4m3) and ``key_scale``, ``value_scale`` [layers, blocks, heads] (or without layers).  Entries with a
+    number outside the blocks are skipped.  No target may be another entry's source or target (the order of copies is
+    not defined, and nothing checks it on the device)."""
+    key = ("copy", _lib.layouts(copies, key_codes, value_codes, key_scale, value_scale))
+    a = _lib.template(key)
+    if a is None or (key_codes.data_ptr() | value_codes.data_ptr()) % 16:
+        a = _checked_copy(copies, key_codes, value_codes, key_scale, value_scale)
+        _lib.keep_template(key, a)
+    if a.count == 0:
+        return
+    a = _lib.CopyBlocksArgs.from_buffer_copy(a)
+    a.copies, a.key_codes, a.value_codes = copies.data_ptr(), key_codes.data_ptr(), value_codes.data_ptr()
+    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
+    _lib.launch(_lib.load().dkv_copy_blocks, a, copies.device, "dkv_copy_blocks")
+
+
+def _checked_copy(copies, key_codes, value_codes, key_scale, value_scale):
+    _lib.require_device(copies, key_codes, value_codes, key_scale, value_scale)
+    if copies.dtype != torch.int32 or copies.dim() != 2 or copies.shape[1] != 3 or not copies.is_contiguous():
+        raise TypeError("copies must be a contiguous int32 [n, 3] tensor")
+    pools = key_codes, value_codes, key_scale, value_scale
+    if key_codes.dim() == 4:
+        pools = [t.unsqueeze(0) for t in pools]
+    if any(t.dim() != dim for t, dim in zip(pools, (5, 5, 3, 3))) or len({t.shape[0] for t in pools}) != 1 \
+            or pools[0].shape[0] == 0:
+        raise ValueError("key_codes and value_codes must be [layers, blocks, heads, block_size, head_dim], key_scale and "
+                         "value_scale [layers, blocks, heads], or all without layers")
+    if pools[0].shape != pools[1].shape:
+        raise ValueError("key_codes and value_codes must have one shape")
+    _check_pool(*(t[0] for t in pools), copies.device)
+    layers, blocks, heads, block_size, D = pools[0].shape
+    if D == 0 or D % 16 or D > MAX_BLOCK_HEAD_DIM:
+        raise ValueError(f"head_dim must be a multiple of 16 up to {MAX_BLOCK_HEAD_DIM}")
+    if 2 * layers * heads >= 1 << 16:
+        raise ValueError("copy_blocks takes fewer than 2^15 heads of all layers together")
+    if any(t.data_ptr() % 16 or t.stride(0) % 16 for t in pools[:2]):
+        raise ValueError("key_codes and value_codes must have 16-byte aligned layers")
+    a = _lib.CopyBlocksArgs()
+    a.count, a.layers, a.blocks, a.H, a.block_size, a.D = copies.shape[0], layers, blocks, heads, block_size, D
+    a.key_stride, a.value_stride, a.key_scale_stride, a.value_scale_stride = (t.stride(0) for t in pools)
+    return a
 
 
 def _check_pool(key_codes, value_codes, key_scale, value_scale, device):
@@ -206,6 +342,81 @@ def _checked_append(keys, values, slots, key_codes, value_codes, key_scale, valu
     a.tokens, a.H, a.D = T, H, D
     a.blocks, a.block_size = key_codes.shape[0], key_codes.shape[2]
     return a, keys, values, slots, all(x is y for x, y in zip(given, (keys, values, slots)))
+
+
+def append_rotated_blocks(query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, key_codes: torch.Tensor,
+                          value_codes: torch.Tensor, key_scale: torch.Tensor, value_scale: torch.Tensor, *,
+                          q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                          eps: float = 1e-6, interleaved: bool = False,
+                          nonfinite: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rotate_heads`` of ``query`` [T, Hq, head_dim] and ``keys`` [T, heads, head_dim], and ``append_blocks`` of those
+    keys with ``values``, in one launch: returns the queries.
+
+    Arguments as there, with ``positions`` [T] (as ``reserve_blocks`` gives them, the same for all layers) and tables
+    ``cos``, ``sin`` [positions, angles], whose angles have to be a multiple of 8.  The keys are rounded to their type
+    before they become codes, as between the two calls.  Nothing has a gradient: tensors that require gradients are
+    refused outside torch.no_grad(), forward-mode tangents always."""
+    if not isinstance(positions, torch.Tensor):
+        raise TypeError("positions must be an int32 or int64 tensor")
+    given = [t for t in (query, keys, values, cos, sin, q_weight, k_weight) if t is not None]
+    no_gradients("append_rotated_blocks", *given)
+    tensors = (query, keys, values, cos, sin, positions, slots, key_codes, value_codes, key_scale, value_scale, q_weight,
+               k_weight)
+    key = ("append_rotated", float(eps), bool(interleaved), q_weight is None, k_weight is None,
+           _lib.layouts(*(t for t in tensors if t is not None)))
+    known = _lib.template(key)
+    if known is None or (query.data_ptr() | keys.data_ptr() | values.data_ptr() | cos.data_ptr() | sin.data_ptr()
+                         | _lib.ptr(q_weight) | _lib.ptr(k_weight)) % 16:
+        known, checked = _checked_rotated(*tensors, eps, interleaved)
+        if all(x is y for x, y in zip(tensors, checked)):
+            _lib.keep_template(key, known)
+        query, keys, values, cos, sin, positions, slots, *_, q_weight, k_weight = checked
+    device = query.device
+    if nonfinite is not None and (nonfinite.dtype != torch.int32 or nonfinite.numel() != 1
+                                  or nonfinite.device != device):
+        raise TypeError("nonfinite must be an int32 tensor of one element on the same device")
+    out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if query.shape[0] == 0:
+        return out
+    a, r = (type(x).from_buffer_copy(x) for x in known)
+    a.keys, a.values, a.slots = keys.data_ptr(), values.data_ptr(), slots.data_ptr()
+    a.key_codes, a.value_codes = key_codes.data_ptr(), value_codes.data_ptr()
+    a.key_scale, a.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
+    a.nonfinite = _lib.ptr(nonfinite)
+    r.query, r.q_out, r.cos, r.sin, r.positions = (t.data_ptr() for t in (query, out, cos, sin, positions))
+    r.q_weight, r.k_weight = _lib.ptr(q_weight), _lib.ptr(k_weight)
+    lib = _lib.load()
+    _lib.launch(lambda args, stream: lib.dkv_append_rotated_blocks(args, r, stream), a, device, "dkv_append_rotated_blocks")
+    return out
+
+
+def _checked_rotated(query, keys, values, cos, sin, positions, slots, key_codes, value_codes, key_scale, value_scale,
+                     q_weight, k_weight, eps, interleaved):
+    _lib.require_device(query, cos, sin, positions, q_weight, k_weight)
+    a, keys, values, slots, _ = _checked_append(keys, values, slots, key_codes, value_codes, key_scale, value_scale)
+    device, D = keys.device, a.D
+    if query.dtype != keys.dtype:
+        raise TypeError("query and keys must have one dtype")
+    if query.dim() != 3 or query.shape[0] != a.tokens or query.shape[1] == 0 or query.shape[2] != D:
+        raise ValueError("query must be [tokens, heads, head_dim], of the keys' tokens and head_dim")
+    if query.device != device:
+        raise ValueError("the tensors must be on the same device")
+    if cos.shape[-1] % 8:
+        raise ValueError("append_rotated_blocks takes angles in multiples of 8; else use rotate_heads and append_blocks")
+    if not 0 <= eps < 1e30:
+        raise ValueError("eps must not be negative")
+    q_weight, k_weight = check_weights(q_weight, k_weight, D, device)
+    cos, sin, positions, c_sb, c_st = check_angles(cos, sin, positions, (a.tokens,), D, device)
+    query = aligned_rows(query, 0)
+    r = _lib.RotateHeadsArgs()
+    r.batch, r.tokens, r.Hq, r.Hkv, r.D = 1, a.tokens, query.shape[1], a.H, D
+    r.q_st, r.q_sh, r.qo_st, r.qo_sh = query.stride(0), query.stride(1), query.shape[1] * D, D
+    r.dtype = a.dtype
+    r.weight_dtype = _lib.dtype_code(next((w.dtype for w in (q_weight, k_weight) if w is not None), query.dtype))
+    set_angles(r, cos, sin, positions, c_sb, c_st, interleaved, eps)
+    return (a, r), (query, keys, values, cos, sin, positions, slots, key_codes, value_codes, key_scale, value_scale,
+                    q_weight, k_weight)
 
 
 def block_attention(query: torch.Tensor, key_codes: torch.Tensor, value_codes: torch.Tensor, key_scale: torch.Tensor,
@@ -324,13 +535,14 @@ _steps = itertools.count(1)  # one line of steps for all caches, so that none ta
 
 
 class BlockPlan(NamedTuple):
-    """Where a step's new tokens go: ``reserve_blocks``' slots and starts, the most tokens of a request, and the
-    step of one cache that they belong to."""
+    """Where a step's new tokens go: ``reserve_blocks``' slots and starts, the most tokens of a request, the
+    step of one cache that they belong to, and the tokens' positions where they were asked for."""
 
     slots: torch.Tensor
     starts: torch.Tensor
     max_tokens: int
     step: int
+    positions: Optional[torch.Tensor] = None
 
 
 class BlockKVCache:
@@ -348,7 +560,7 @@ class BlockKVCache:
     """
 
     def __init__(self, requests: int, blocks: int, kv_heads: int, head_dim: int, *, layers: int = 1,
-                 block_size: int = 64, max_blocks: Optional[int] = None, device="cuda") -> None:
+                 block_size: int = 64, max_blocks: Optional[int] = None, sharing: bool = False, device="cuda") -> None:
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
         if min(requests, blocks, kv_heads, layers) < 1 or requests > MAX_REQUESTS:
@@ -372,6 +584,7 @@ class BlockKVCache:
         self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
         self.free = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
         self.state = torch.tensor([blocks, 0, 0, 0], dtype=torch.int32, device=device)
+        self.shares = torch.zeros(blocks, dtype=torch.int32, device=device) if sharing else None
         self.nonfinite = torch.zeros(1, dtype=torch.int32, device=device)
         self._step = next(_steps)
 
@@ -379,25 +592,68 @@ class BlockKVCache:
         if plan.step != self._step:
             raise ValueError("the plan is of an earlier reserve, whose requests' lengths have moved on, or of another cache")
 
-    def reserve(self, tokens: torch.Tensor, total: int, *, max_tokens: Optional[int] = None) -> BlockPlan:
+    @property
+    def _tables(self) -> Tuple[torch.Tensor, ...]:
+        return self.table, self.lengths, self.free, self.state
+
+    @property
+    def _pools(self) -> Tuple[torch.Tensor, ...]:
+        return self.key_codes, self.value_codes, self.key_scale, self.value_scale
+
+    def reserve(self, tokens: torch.Tensor, total: int, *, max_tokens: Optional[int] = None,
+                positions: bool = False) -> BlockPlan:
         """Room for ``tokens[r]`` new tokens of each request (``reserve_blocks``).  ``max_tokens``: the most of
         them, where the caller knows it (default ``total``); ``attention`` leaves the rows of a request with more
-        undefined.  A decode step without it also launches the kernel for chunks, which finds nothing to do."""
-        slots, starts = reserve_blocks(self.table, self.lengths, self.free, self.state, tokens, total,
-                                       block_size=self.block_size)
+        undefined.  A decode step without it also launches the kernel for chunks, which finds nothing to do.
+        ``positions``: the plan has the tokens' positions, for ``append_rotated``."""
+        places = torch.empty(int(total), dtype=torch.int32, device=self.table.device) if positions else None
+        slots, starts, *copies = reserve_blocks(*self._tables, tokens, total, block_size=self.block_size,
+                                                shares=self.shares, positions=places)
+        for more in copies:
+            copy_blocks(more, *self._pools)
         self._step = next(_steps)
-        return BlockPlan(slots, starts, max(1, total if max_tokens is None else max_tokens), self._step)
+        return BlockPlan(slots, starts, max(1, total if max_tokens is None else max_tokens), self._step, places)
 
     def release(self, tokens: Optional[torch.Tensor] = None) -> None:
         """Drop each request's last ``tokens[r]`` tokens, or everything (``release_blocks``)."""
-        release_blocks(self.table, self.lengths, self.free, self.state, tokens, block_size=self.block_size)
+        release_blocks(*self._tables, tokens, block_size=self.block_size, shares=self.shares)
         self._step = next(_steps)
+
+    def fork(self, sources: torch.Tensor, tokens: Optional[torch.Tensor] = None) -> None:
+        """Make each request r a copy of request ``sources[r]`` as it is now, or of its first ``tokens[r]`` tokens; -1
+        leaves it as it is (``fork_blocks``).  The cache has to be made with ``sharing``."""
+        if self.shares is None:
+            raise ValueError("the cache was made without sharing")
+        fork_blocks(*self._tables, self.shares, sources, tokens, block_size=self.block_size)
+        self._step = next(_steps)
+
+    def compact(self) -> torch.Tensor:
+        """Move the blocks in use to the lowest numbers, in all layers (``compact_blocks``): those from
+        ``blocks - state[0]`` on are free afterwards.  Returns the copies that were made."""
+        copies = compact_blocks(*self._tables, self.shares, block_size=self.block_size)
+        copy_blocks(copies, *self._pools)
+        self._step = next(_steps)
+        return copies
 
     def append(self, layer: int, keys: torch.Tensor, values: torch.Tensor, plan: BlockPlan) -> None:
         """The step's new ``keys`` and ``values`` [T, kv_heads, head_dim] of one layer (``append_blocks``)."""
         self._check_plan(plan)
         append_blocks(keys, values, plan.slots, self.key_codes[layer], self.value_codes[layer], self.key_scale[layer],
                       self.value_scale[layer], nonfinite=self.nonfinite)
+
+    def append_rotated(self, layer: int, query: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, cos: torch.Tensor,
+                       sin: torch.Tensor, plan: BlockPlan, *, q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       interleaved: bool = False) -> torch.Tensor:
+        """``append`` of keys that are normed and turned by their positions on the way, and the queries likewise: returns
+        these (``append_rotated_blocks``).  The plan has to be made with ``positions``."""
+        self._check_plan(plan)
+        if plan.positions is None:
+            raise ValueError("the plan has no positions; reserve with positions=True")
+        return append_rotated_blocks(query, keys, values, cos, sin, plan.positions, plan.slots, self.key_codes[layer],
+                                     self.value_codes[layer], self.key_scale[layer], self.value_scale[layer],
+                                     q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved,
+                                     nonfinite=self.nonfinite)
 
     def attention(self, layer: int, query: torch.Tensor, plan: BlockPlan, *, scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -419,4 +675,5 @@ class BlockKVCache:
             raise ValueError("append_blocks requires finite keys and values")
 
 
-__all__ = ["BlockKVCache", "BlockPlan", "append_blocks", "block_attention", "release_blocks", "reserve_blocks"]
+__all__ = ["BlockKVCache", "BlockPlan", "append_blocks", "append_rotated_blocks", "block_attention", "compact_blocks",
+           "copy_blocks", "fork_blocks", "release_blocks", "reserve_blocks"]

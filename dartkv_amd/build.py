@@ -22,7 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdartkv_hip.so")
 SOURCES = ["capi.hip", "quantize.hip", "decode.hip", "decode_fast.hip", "decode_uniform.hip", "decode_tiles.hip",
            "materialize.hip", "prep.hip", "copy.hip", "prompt.hip", "block_tables.hip", "block_append.hip",
-           "block_attention.hip", "block_chunks.hip"]
+           "block_attention.hip", "block_chunks.hip", "block_share.hip", "rotate.hip", "logprob.hip"]
 ARCH = os.environ.get("DKV_OFFLOAD_ARCH", "gfx950")
 
 
@@ -50,7 +50,7 @@ def command(output: str = LIB) -> list[str]:
 # Sources whose kernels must keep every value in registers: a spill to scratch
 # (private memory in HBM) would add memory traffic to the page and tile kernels' loops.
 NO_SCRATCH = {"decode_fast.hip", "decode_uniform.hip", "decode_tiles.hip", "prompt.hip", "block_attention.hip",
-              "block_chunks.hip"}
+              "block_chunks.hip", "block_append.hip", "rotate.hip", "logprob.hip"}
 
 
 def _run(cmd: list[str], verbose: bool) -> str:

@@ -1,4 +1,5 @@
-// New keys and values into the e4m3 blocks of a block cache (dkv_append_blocks).
+// New keys and values into the e4m3 blocks of a block cache (dkv_append_blocks), and the same for keys that are normed
+// and turned on their way, with their queries (dkv_append_rotated_blocks).
 //
 // A block of bs tokens of one KV head has one scale for its keys and one for its values, 2^e with e the least that
 // brings the largest magnitude so far under e4m3's 448 (e in [-120, 121], -120 for a block of zeros).  A token's code is
@@ -17,7 +18,7 @@
 #include <stdint.h>
 
 #include "dkv_capi_util.h"
-#include "dkv_device.h"
+#include "dkv_rotate.h"
 
 using namespace dkv;
 
@@ -37,6 +38,7 @@ struct AppendParams {
   uint32_t* nonfinite;
   int64_t T, blocks;
   int32_t H, D, shift, span, dtype;
+  uint32_t groups;  // workgroups of the launch
 };
 
 __device__ __forceinline__ int exponent_for(float amax) {
@@ -93,6 +95,12 @@ struct Raw {  // eight elements as they are
       }
     }
   }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    Words<SRC, 8> words;
+    words.set(x);
+#pragma unroll
+    for (int i = 0; i < 4 * kWords; ++i) w[i / 4][i % 4] = words.w[i];
+  }
   // The registers hold something unknown from here: what was made of them is not kept.
   __device__ __forceinline__ void forget() {
 #pragma unroll
@@ -126,20 +134,86 @@ __device__ __forceinline__ float magnitude(uint32_t top) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
 }
 
+enum Turn { kStays, kHalves, kNeighbours };  // which channels of a key turn with each other
+
+// Keys of a pass, as they go into the blocks: normed, turned by their tokens' angles and rounded to their type, as
+// rotate_heads gives them.  A lane has eight channels of its row, whose sums go over `lanes` lanes (a power of two; those
+// behind head_dim hold zeros); the partners of halves are in a lane of their own.
+template <int SRC, Turn TURN>
+struct KeyTurner {
+  const RotateParams& r;
+  int lane, lanes, ch;
+  bool turns, second;
+  float w[8];
+
+  __device__ __forceinline__ KeyTurner(const RotateParams* rotation, int lane, int lanes, int ch)
+      : r(*rotation), lane(lane), lanes(lanes), ch(ch) {
+    turns = ch < 2 * r.half, second = TURN == kHalves && ch >= r.half;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.f;
+    if (r.side[1].w && ch < r.D) load_any<8>(r.side[1].w, ch, r.w_dtype, w);
+  }
+  // `raw`: the row of token t (real: it is one).
+  __device__ __forceinline__ void turn(Raw<SRC>& raw, int64_t t, bool real) const {
+    float x[8], c[8], s[8];
+    raw.get(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+    const int64_t angles = real ? angles_at(r, (uint32_t)t) : kNoToken;
+    if (turns) {
+      const int at = TURN == kNeighbours ? ch / 2 : second ? ch - r.half : ch;
+      if constexpr (TURN == kNeighbours) {
+        float c4[4], s4[4];
+        load_angles<4>(r, angles, at, c4, s4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = c4[i / 2], s[i] = s4[i / 2];
+      } else {
+        load_angles<8>(r, angles, at, c, s);
+      }
+    }
+    const float f = r.side[1].w ? norm_factor(row_sum(sum_of_squares(x), lanes), r.inv_d, r.eps) : 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = angles == kNoToken ? 0.f : x[i] * (f * w[i]);
+    if constexpr (TURN == kNeighbours) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float a = x[i], b = x[i + 1];
+        x[i] = fmaf(a, c[i], -(b * s[i])), x[i + 1] = fmaf(b, c[i], a * s[i]);
+      }
+    } else {
+      const int partner = turns ? (second ? lane - r.half / 8 : lane + r.half / 8) : lane;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __shfl(x[i], partner, 64);
+        if (turns) x[i] = fmaf(x[i], c[i], second ? y * s[i] : -(y * s[i]));
+      }
+    }
+    raw.set(x);
+  }
+};
+
 template <int SRC>
-__global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
+struct KeyTurner<SRC, kStays> {
+  __device__ __forceinline__ KeyTurner(const RotateParams*, int, int, int) {}
+  __device__ __forceinline__ void turn(Raw<SRC>&, int64_t, bool) const {}
+};
+
+// Wave `unit`'s runs.
+template <int SRC, Turn TURN>
+__device__ __forceinline__ void append_runs(const AppendParams& p, const RotateParams* rotation, int64_t unit) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kinds = 2 * p.H;
   const int64_t first = unit / kinds * p.span;
   if (first >= p.T) return;
   const int kind = (int)(unit % kinds), which = kind & 1, h = kind >> 1;
   const int bs = 1 << p.shift;
-  const int lpr = p.D >> 3, rpp = 64 / lpr;  // lanes of a row, rows of a pass
+  const int lpr = TURN == kStays ? p.D >> 3 : rotation->lanes * 2, rpp = 64 / lpr;  // lanes of a row, rows of a pass
   const int my_row = lane / lpr, my_ch = (lane % lpr) * 8;
-  const bool active = my_row < rpp;
+  const bool active = my_row < rpp && (TURN == kStays || my_ch < p.D);
   const void* src = p.src[which];
   constexpr int kSize = SRC == kF32 ? 4 : 2;
+  const bool turned = TURN != kStays && which == 0;
+  const KeyTurner<SRC, TURN> turner(rotation, lane, lpr, my_ch);
   const uint32_t my_at = (uint32_t)((my_row * p.st[which] + my_ch) * kSize), my_code = my_row * p.D + my_ch;
 
   // the runs that begin among this wave's tokens
@@ -180,6 +254,11 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
       raw[i].zero();
       if (active && r < n) raw[i].load(base + i * pass + my_at);
     }
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < kHeld<SRC>; ++i)
+        if (i * rpp < n) turner.turn(raw[i], t + i * rpp + my_row, active && i * rpp + my_row < n);
+    }
 #pragma unroll
     for (int i = 0; i < kHeld<SRC>; ++i) {
       raw[i].largest(top);
@@ -187,11 +266,11 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
     }
     for (int row = kHeld<SRC> * rpp; row < n; row += rpp) {
       const int r = row + my_row;
-      if (active && r < n) {
-        Raw<SRC> more;
-        more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
-        more.largest(top);
-      }
+      Raw<SRC> more;
+      more.zero();
+      if (active && r < n) more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+      if (turned) turner.turn(more, t + r, active && r < n);
+      more.largest(top);
     }
     float amax = magnitude<SRC>(top);
     if (__any(!(amax < __builtin_inff()))) {  // the largest of the finite ones
@@ -200,15 +279,15 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
 #pragma unroll 1
       for (int row = 0; row < n; row += rpp) {
         const int r = row + my_row;
-        if (active && r < n) {
-          float x[8];
-          Raw<SRC> again;
-          again.load(base + (int64_t)row * p.st[which] * kSize + my_at);
-          again.get(x);
+        float x[8];
+        Raw<SRC> again;
+        again.zero();
+        if (active && r < n) again.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+        if (turned) turner.turn(again, t + r, active && r < n);
+        again.get(x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (fabsf(x[i]) < __builtin_inff()) amax = fmaxf(amax, fabsf(x[i]));
-        }
+        for (int i = 0; i < 8; ++i)
+          if (fabsf(x[i]) < __builtin_inff()) amax = fmaxf(amax, fabsf(x[i]));
       }
     }
     amax = wave_max(amax);
@@ -245,43 +324,55 @@ __global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
     }
     for (int row = kHeld<SRC> * rpp; row < n; row += rpp) {
       const int r = row + my_row;
-      if (active && r < n) {
-        float x[8];
-        Raw<SRC> more;
-        more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
-        more.get(x);
-        *(uint2*)(codes + row * p.D + my_code) = codes8(x, inv);
-      }
+      float x[8];
+      Raw<SRC> more;
+      more.zero();
+      if (active && r < n) more.load(base + (int64_t)row * p.st[which] * kSize + my_at);
+      if (turned) turner.turn(more, t + r, active && r < n);
+      more.get(x);
+      if (active && r < n) *(uint2*)(codes + row * p.D + my_code) = codes8(x, inv);
     }
     if (lane == 0 && (held == 0 || now != before)) *scale = now;
   }
 }
 
-}  // namespace
+template <int SRC>
+__global__ void __launch_bounds__(kThreads) block_append(AppendParams p) {
+  append_runs<SRC, kStays>(p, nullptr, (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+}
 
-extern "C" int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream) {
-  DKV_CHECK(args != nullptr, DKV_ERR_INVALID, "dkv_append_blocks: args is NULL");
-  const dkv_append_blocks_args& a = *args;
+// The workgroups of the append, then those of the queries' rows.
+template <int SRC, Turn TURN>
+__global__ void __launch_bounds__(kThreads) block_append_rotated(AppendParams p, RotateParams r) {
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x < p.groups)
+    append_runs<SRC, TURN>(p, &r, (int64_t)blockIdx.x * (kThreads / 64) + wave);
+  else
+    rotate_rows<SRC, 8, TURN == kNeighbours, 1>(r, r.side[0], (blockIdx.x - p.groups) * (kThreads / 64) + wave);
+}
+
+int append_params(const dkv_append_blocks_args& a, const char* where, AppendParams& p) {
   DKV_CHECK(a.dtype == kF32 || a.dtype == kF16 || a.dtype == kBF16, DKV_ERR_DTYPE,
-            "dkv_append_blocks: keys and values must be bf16, fp16 or fp32");
+            "%s: keys and values must be bf16, fp16 or fp32", where);
   DKV_CHECK(a.H >= 1 && a.H < (1 << 20) && a.D >= 16 && a.D <= 512 && a.D % 16 == 0, DKV_ERR_INVALID,
-            "dkv_append_blocks: head_dim must be a multiple of 16 up to 512");
+            "%s: head_dim must be a multiple of 16 up to 512", where);
   DKV_CHECK(a.block_size >= 16 && a.block_size <= 256 && (a.block_size & (a.block_size - 1)) == 0, DKV_ERR_INVALID,
-            "dkv_append_blocks: block_size must be 16, 32, 64, 128 or 256");
-  DKV_CHECK(a.tokens >= 0 && a.blocks >= 1, DKV_ERR_INVALID, "dkv_append_blocks: bad counts");
+            "%s: block_size must be 16, 32, 64, 128 or 256", where);
+  DKV_CHECK(a.tokens >= 0 && a.blocks >= 1, DKV_ERR_INVALID, "%s: bad counts", where);
+  p = {};
   if (a.tokens == 0) return DKV_OK;
   DKV_CHECK(a.keys && a.values && a.slots && a.key_codes && a.value_codes && a.key_scale && a.value_scale,
-            DKV_ERR_INVALID, "dkv_append_blocks: NULL pointer");
+            DKV_ERR_INVALID, "%s: NULL pointer", where);
   const int64_t esize = a.dtype == kF32 ? 4 : 2;
   DKV_CHECK((((uintptr_t)a.keys | (uintptr_t)a.values | (uintptr_t)(a.k_st * esize) | (uintptr_t)(a.k_sh * esize) |
               (uintptr_t)(a.v_st * esize) | (uintptr_t)(a.v_sh * esize) | (uintptr_t)a.key_codes |
               (uintptr_t)a.value_codes) & 15) == 0,
-            DKV_ERR_INVALID, "dkv_append_blocks: rows must be 16-byte aligned");
+            DKV_ERR_INVALID, "%s: rows must be 16-byte aligned", where);
   DKV_CHECK(a.k_st >= 0 && a.v_st >= 0 && a.k_st < (1 << 23) && a.v_st < (1 << 23), DKV_ERR_INVALID,
-            "dkv_append_blocks: token strides must be under 2^23 elements");
-  AppendParams p = {{a.keys, a.values}, {a.k_st, a.v_st}, {a.k_sh, a.v_sh}, {a.key_codes, a.value_codes},
-                    {a.key_scale, a.value_scale}, a.slots, a.nonfinite, a.tokens, a.blocks,
-                    (int32_t)a.H, (int32_t)a.D, __builtin_ctzll((uint64_t)a.block_size), 1, (int32_t)a.dtype};
+            "%s: token strides must be under 2^23 elements", where);
+  p = {{a.keys, a.values}, {a.k_st, a.v_st}, {a.k_sh, a.v_sh}, {a.key_codes, a.value_codes},
+       {a.key_scale, a.value_scale}, a.slots, a.nonfinite, a.tokens, a.blocks,
+       (int32_t)a.H, (int32_t)a.D, __builtin_ctzll((uint64_t)a.block_size), 1, (int32_t)a.dtype};
   // Few tokens: one wave for each of them; many: a wave looks through 64 for the runs that begin there.  16 x 5,354 tokens
   // of 8 heads: 103 us, a wave for each 424; 2,048 requests' single tokens: 31 us a wave for each, 112 through 64.  The
   // bound takes many tokens for prompts': single tokens of more requests than that, each a run, pay for it (4,096: 112
@@ -289,12 +380,60 @@ extern "C" int dkv_append_blocks(const dkv_append_blocks_args* args, void* strea
   p.span = a.tokens * a.H <= 16384 ? 1 : 64;
   const int64_t units = (a.tokens + p.span - 1) / p.span * 2 * a.H;
   const int64_t grid = (units + kThreads / 64 - 1) / (kThreads / 64);
-  DKV_CHECK(grid < (1ll << 31), DKV_ERR_INVALID, "dkv_append_blocks: too many tokens");
-  if (a.dtype == kF32)
-    hipLaunchKernelGGL(block_append<kF32>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
-  else if (a.dtype == kF16)
-    hipLaunchKernelGGL(block_append<kF16>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
+  DKV_CHECK(grid < (1ll << 31), DKV_ERR_INVALID, "%s: too many tokens", where);
+  p.groups = (uint32_t)grid;
+  return DKV_OK;
+}
+
+template <int SRC>
+void launch_rotated(const AppendParams& p, const RotateParams& r, bool next, hipStream_t stream) {
+  const dim3 grid(p.groups + r.side[0].groups), block(kThreads);
+  if (next)
+    hipLaunchKernelGGL((block_append_rotated<SRC, kNeighbours>), grid, block, 0, stream, p, r);
   else
-    hipLaunchKernelGGL(block_append<kBF16>, dim3((unsigned)grid), dim3(kThreads), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL((block_append_rotated<SRC, kHalves>), grid, block, 0, stream, p, r);
+}
+
+}  // namespace
+
+extern "C" int dkv_append_blocks(const dkv_append_blocks_args* args, void* stream) {
+  DKV_CHECK(args != nullptr, DKV_ERR_INVALID, "dkv_append_blocks: args is NULL");
+  AppendParams p;
+  const int rc = append_params(*args, "dkv_append_blocks", p);
+  if (rc != DKV_OK || p.T == 0) return rc;
+  const dim3 grid(p.groups);
+  if (p.dtype == kF32)
+    hipLaunchKernelGGL(block_append<kF32>, grid, dim3(kThreads), 0, (hipStream_t)stream, p);
+  else if (p.dtype == kF16)
+    hipLaunchKernelGGL(block_append<kF16>, grid, dim3(kThreads), 0, (hipStream_t)stream, p);
+  else
+    hipLaunchKernelGGL(block_append<kBF16>, grid, dim3(kThreads), 0, (hipStream_t)stream, p);
   return dkv_check_launch("dkv_append_blocks");
+}
+
+extern "C" int dkv_append_rotated_blocks(const dkv_append_blocks_args* args, const dkv_rotate_heads_args* rotation,
+                                         void* stream) {
+  const char* where = "dkv_append_rotated_blocks";
+  DKV_CHECK(args != nullptr && rotation != nullptr, DKV_ERR_INVALID, "%s: args is NULL", where);
+  const dkv_rotate_heads_args& a = *rotation;
+  AppendParams p;
+  int rc = append_params(*args, where, p);
+  if (rc != DKV_OK) return rc;
+  RotateParams r;
+  rc = rotate_params(a, where, r);
+  if (rc != DKV_OK) return rc;
+  DKV_CHECK(a.batch == 1 && a.tokens == args->tokens && a.Hkv == args->H && a.D == args->D && a.dtype == args->dtype,
+            DKV_ERR_INVALID, "%s: queries and keys must have the same tokens, head_dim and type", where);
+  DKV_CHECK(a.half % 8 == 0, DKV_ERR_UNSUPPORTED, "%s: turned channels must be a multiple of 16", where);
+  if (p.T == 0) return DKV_OK;
+  DKV_CHECK(a.query && a.q_out && a.positions && (a.half == 0 || (a.cos && a.sin)), DKV_ERR_INVALID, "%s: NULL pointer",
+            where);
+  DKV_CHECK((uint64_t)p.groups + r.side[0].groups < (1ull << 31), DKV_ERR_INVALID, "%s: too many tokens", where);
+  if (p.dtype == kF32)
+    launch_rotated<kF32>(p, r, a.interleaved != 0, (hipStream_t)stream);
+  else if (p.dtype == kF16)
+    launch_rotated<kF16>(p, r, a.interleaved != 0, (hipStream_t)stream);
+  else
+    launch_rotated<kBF16>(p, r, a.interleaved != 0, (hipStream_t)stream);
+  return dkv_check_launch(where);
 }

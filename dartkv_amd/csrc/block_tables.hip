@@ -13,17 +13,20 @@
 // writes its share of the slots and of the moved blocks, whose requests it finds in the sums by bisection; what all of
 // them read (lengths, the stack's count) is changed by the last workgroup to finish, which the ticket tells.  It needs
 // no fence: the others have only read what it changes, and nothing that they wrote is read (with fences a reserve of
-// 400,000 slots took 38 us).  Bound: latency, a load of the lengths, one of the blocks and the ticket's round trip after
+// 400,000 slots took 38 us).  With shares (blocks that several requests hold) a request that writes into a block of others
+// gets a copy of it first: of the writers of a block those whose rank among them, in the requests' order, is below the
+// block's shares; the last workgroup changes those entries and the shares.  Bound: latency, a load of the lengths, one of the blocks and the ticket's round trip after
 // each other.  256 requests, a token each: 4.2 us; 128 requests, 400,000 tokens: 10.6 us, their release 5.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "dkv_block_share.h"
 #include "dkv_capi_util.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRequests = 8190;  // 12 bytes each of 160 KiB of LDS
+constexpr int kMaxRequests = dkv::kMaxRequests;  // 12 bytes each of 160 KiB of LDS (16 with shares)
 constexpr int kSlots = 4;  // of a thread, where there are many
 
 struct TablesParams {
@@ -33,6 +36,7 @@ struct TablesParams {
   int32_t* starts;
   int64_t total, blocks;
   int32_t R, max_blocks, shift;
+  int32_t *shares, *copies, *positions;
 };
 
 enum : int32_t { kNoBlocks = 1, kRowFull = 2, kBadCount = 4, kBadTotal = 8 };
@@ -90,16 +94,81 @@ __device__ __forceinline__ int find(const Sum* sums, int R, uint32_t i) {
   return lo;
 }
 
-template <bool RESERVE, int SLOTS>  // SLOTS: of a thread
+// The blocks that requests have to copy: copied[r] is the shared block that request r writes into, or -1 where it does
+// not, or is the last of all its holders.
+__device__ __forceinline__ void find_copies(const TablesParams& p, int32_t* copied) {
+  static_assert((kMaxRequests + kThreads - 1) / kThreads <= 32, "a bit for each of a thread's requests");
+  __shared__ int32_t any;
+  if (threadIdx.x == 0) any = 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < p.R; r += kThreads) {
+    const int32_t length = p.lengths[r], column = length >> p.shift;
+    int32_t block = -1;
+    if (p.tokens[r] > 0 && length > 0 && (length & ((1 << p.shift) - 1)) != 0 && column < p.max_blocks) {
+      block = p.table[(int64_t)r * p.max_blocks + column];
+      if (block < 0 || block >= p.blocks || p.shares[block] <= 0) block = -1;
+    }
+    copied[r] = block;
+    if (block >= 0) any = 1;
+  }
+  __syncthreads();
+  if (!any) return;
+  uint32_t keeps = 0;
+  for (int r = threadIdx.x, i = 0; r < p.R; r += kThreads, ++i) {
+    const int32_t block = copied[r];
+    if (block < 0) continue;
+    int32_t rank = 0;
+    for (int q = 0; q < r; ++q) rank += copied[q] == block;
+    if (rank >= p.shares[block]) keeps |= 1u << i;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x, i = 0; r < p.R; r += kThreads, ++i)
+    if (keeps >> i & 1) copied[r] = -1;
+  __syncthreads();
+}
+
+// The copies, in the requests' order, and the entries and shares that they change.
+__device__ __forceinline__ void make_copies(const TablesParams& p, const Sum* sums, const int32_t* lens,
+                                            const int32_t* copied, int64_t count, bool fits) {
+  __shared__ int32_t wave_count[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int running = 0;
+  for (int base = 0; base < p.R; base += kThreads) {
+    const int r = base + tid;
+    const bool copy = fits && r < p.R && copied[r] >= 0;
+    const uint64_t mask = __ballot(copy);
+    int32_t* counts = wave_count[base / kThreads & 1];
+    if (lane == 0) counts[wave] = __builtin_popcountll(mask);
+    __syncthreads();
+    int before = running + __builtin_popcountll(mask & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += counts[w];
+      running += counts[w];
+    }
+    if (copy) {
+      const int32_t id = p.free[count - 1 - sums[r].blocks];
+      p.table[(int64_t)r * p.max_blocks + (lens[r] >> p.shift)] = id;
+      atomicSub(&p.shares[copied[r]], 1);
+      int32_t* entry = p.copies + 3 * (int64_t)before;
+      entry[0] = copied[r], entry[1] = id, entry[2] = lens[r] & ((1 << p.shift) - 1);
+    }
+  }
+  for (int i = 3 * running + tid; i < 3 * p.R; i += kThreads) p.copies[i] = -1;
+  __syncthreads();  // (the stack is read before it is cleared)
+}
+
+template <bool RESERVE, int SLOTS, bool SHARED>  // SLOTS: of a thread
 __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   extern __shared__ Sum sums[];                // [R + 1]: before each request
   int32_t* lens = (int32_t*)(sums + p.R + 1);  // [R]: the lengths before
+  int32_t* copied = lens + p.R;                // [R] (SHARED)
   __shared__ Sum wave_sum[2][4];
   __shared__ int32_t flags, last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) flags = 0;
   const int64_t count = p.state[0];
 
+  if constexpr (SHARED) find_copies(p, copied);
   Sum running = {0, 0};
   int32_t bad = 0;
   for (int base = 0; base < p.R; base += kThreads) {
@@ -107,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
     Sum x = {0, 0};
     if (r < p.R) {
       const Row row = row_of<RESERVE>(p, r, bad);
-      x = {(uint32_t)row.count, (uint32_t)row.moved};
+      x = {(uint32_t)row.count + (SHARED && copied[r] >= 0), (uint32_t)row.moved};
       lens[r] = row.length;
     }
     Sum sum = x;
@@ -146,27 +215,36 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
     const int mask = (1 << p.shift) - 1;
     for (int64_t at = me * SLOTS; at < p.total; at += all * SLOTS) {
       int64_t slot[SLOTS];
+      int32_t place[SLOTS];
       int r = fits && at < moved ? find<true>(sums, p.R, (uint32_t)at) : 0;
 #pragma unroll
       for (int i = 0; i < SLOTS; ++i) {
-        slot[i] = -1;
+        slot[i] = place[i] = -1;
         if (fits && at + i < moved) {
           if (i > 0)
             while (sums[r + 1].tokens <= at + i) ++r;
           const int64_t position = lens[r] + (at + i - sums[r].tokens);
           const int32_t block = (int32_t)(position >> p.shift), old = (int32_t)blocks_of(lens[r], p.shift);
-          const int32_t id = block < old ? p.table[(int64_t)r * p.max_blocks + block]
-                                         : p.free[count - 1 - ((int64_t)sums[r].blocks + block - old)];
-          slot[i] = ((int64_t)id << p.shift) + (position & mask);
+          const int copy = SHARED && copied[r] >= 0;  // (its tokens lie in block old - 1 and those behind it)
+          const int32_t id = block < old - copy ? p.table[(int64_t)r * p.max_blocks + block]
+                                                : p.free[count - 1 - ((int64_t)sums[r].blocks + block - (old - copy))];
+          slot[i] = ((int64_t)id << p.shift) + (position & mask), place[i] = (int32_t)position;
         }
       }
       if (SLOTS > 1 && at + SLOTS <= p.total) {
 #pragma unroll
         for (int i = 0; i + 1 < SLOTS; i += 2) *(longlong2*)(p.slots + at + i) = make_longlong2(slot[i], slot[i + 1]);
+        if constexpr (SLOTS == 4)
+          if (p.positions) *(int4*)(p.positions + at) = make_int4(place[0], place[1], place[2], place[3]);
       } else {
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i)
           if (at + i < p.total) p.slots[at + i] = slot[i];
+        if (p.positions) {
+#pragma unroll
+          for (int i = 0; i < SLOTS; ++i)
+            if (at + i < p.total) p.positions[at + i] = place[i];
+        }
       }
     }
   }
@@ -177,7 +255,8 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
       const int64_t j = i - sums[r].blocks, length = lens[r];
       const int64_t old = RESERVE ? blocks_of(length, p.shift)
                                   : blocks_of(length - (int64_t)(sums[r + 1].tokens - sums[r].tokens), p.shift);
-      int32_t* entry = p.table + (int64_t)r * p.max_blocks + old + j;
+      if (SHARED && copied[r] >= 0 && j == 0) continue;  // (others read that entry)
+      int32_t* entry = p.table + (int64_t)r * p.max_blocks + old + j - (SHARED && copied[r] >= 0);
       if constexpr (RESERVE) {
         *entry = p.free[count - 1 - i];
       } else {
@@ -195,6 +274,7 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
     __syncthreads();
     if (!last) return;
   }
+  if constexpr (SHARED) make_copies(p, sums, lens, copied, count, fits);
   if (fits) {
     for (int r = tid; r < p.R; r += kThreads) {
       const int32_t n = (int32_t)(sums[r + 1].tokens - sums[r].tokens);
@@ -211,16 +291,24 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
 }
 
 int check_tables(const dkv_block_tables_args& a, const char* where, TablesParams& p) {
-  DKV_CHECK(a.requests >= 1 && a.requests <= kMaxRequests, DKV_ERR_INVALID, "%s: requests must be in 1..%d", where,
-            kMaxRequests);
-  DKV_CHECK(a.block_size >= 16 && a.block_size <= 256 && (a.block_size & (a.block_size - 1)) == 0, DKV_ERR_INVALID,
-            "%s: block_size must be 16, 32, 64, 128 or 256", where);
-  DKV_CHECK(a.max_blocks >= 1 && a.max_blocks * a.block_size < (1ll << 31) && a.blocks >= 1 && a.blocks < (1ll << 31),
-            DKV_ERR_INVALID, "%s: bad block counts", where);
-  DKV_CHECK(a.table && a.lengths && a.free && a.state, DKV_ERR_INVALID, "%s: NULL pointer", where);
+  const int rc = dkv::check_block_tables(a, where);
+  if (rc != DKV_OK) return rc;
   p = {a.table, a.lengths, a.free, a.state, a.tokens, a.slots, a.starts, a.total, a.blocks,
-       (int32_t)a.requests, (int32_t)a.max_blocks, __builtin_ctzll((uint64_t)a.block_size)};
+       (int32_t)a.requests, (int32_t)a.max_blocks, __builtin_ctzll((uint64_t)a.block_size), a.shares, a.copies, a.positions};
   return DKV_OK;
+}
+
+template <bool SHARED>
+void launch_reserve(const TablesParams& p, hipStream_t stream) {
+  const int lds = (SHARED ? 16 : 12) * p.R + 8;
+  if (p.total <= 4 * kThreads) {
+    const int64_t groups = p.total > kThreads ? (p.total + kThreads - 1) / kThreads : 1;
+    hipLaunchKernelGGL((block_tables<true, 1, SHARED>), dim3((unsigned)groups), dim3(kThreads), lds, stream, p);
+  } else {
+    int64_t groups = (p.total + kSlots * kThreads - 1) / (kSlots * kThreads);
+    groups = groups > 512 ? 512 : groups;
+    hipLaunchKernelGGL((block_tables<true, kSlots, SHARED>), dim3((unsigned)groups), dim3(kThreads), lds, stream, p);
+  }
 }
 
 }  // namespace
@@ -233,15 +321,13 @@ extern "C" int dkv_reserve_blocks(const dkv_block_tables_args* args, void* strea
   DKV_CHECK(args->tokens && args->starts && (args->slots || args->total == 0), DKV_ERR_INVALID,
             "dkv_reserve_blocks: NULL pointer");
   DKV_CHECK(args->total >= 0 && args->total < (1ll << 31), DKV_ERR_INVALID, "dkv_reserve_blocks: bad total");
-  DKV_CHECK(((uintptr_t)args->slots & 15) == 0, DKV_ERR_INVALID, "dkv_reserve_blocks: slots must be 16-byte aligned");
-  const int lds = 12 * p.R + 8;
-  if (args->total <= 4 * kThreads) {
-    const int64_t groups = args->total > kThreads ? (args->total + kThreads - 1) / kThreads : 1;
-    hipLaunchKernelGGL((block_tables<true, 1>), dim3((unsigned)groups), dim3(kThreads), lds, (hipStream_t)stream, p);
+  DKV_CHECK((((uintptr_t)args->slots | (uintptr_t)args->positions) & 15) == 0, DKV_ERR_INVALID,
+            "dkv_reserve_blocks: slots and positions must be 16-byte aligned");
+  if (p.shares) {
+    DKV_CHECK(p.copies, DKV_ERR_INVALID, "dkv_reserve_blocks: NULL pointer");
+    launch_reserve<true>(p, (hipStream_t)stream);
   } else {
-    int64_t groups = (args->total + kSlots * kThreads - 1) / (kSlots * kThreads);
-    groups = groups > 512 ? 512 : groups;
-    hipLaunchKernelGGL((block_tables<true, kSlots>), dim3((unsigned)groups), dim3(kThreads), lds, (hipStream_t)stream, p);
+    launch_reserve<false>(p, (hipStream_t)stream);
   }
   return dkv_check_launch("dkv_reserve_blocks");
 }
@@ -251,8 +337,9 @@ extern "C" int dkv_release_blocks(const dkv_block_tables_args* args, void* strea
   TablesParams p;
   const int rc = check_tables(*args, "dkv_release_blocks", p);
   if (rc != DKV_OK) return rc;
+  if (args->shares) return dkv::release_shared(*args, (hipStream_t)stream);
   int64_t groups = (p.blocks + 4 * kThreads - 1) / (4 * kThreads);  // (at most that many blocks return)
   groups = groups > 16 ? 16 : groups;
-  hipLaunchKernelGGL((block_tables<false, 1>), dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8, (hipStream_t)stream, p);
+  hipLaunchKernelGGL((block_tables<false, 1, false>), dim3((unsigned)groups), dim3(kThreads), 12 * p.R + 8, (hipStream_t)stream, p);
   return dkv_check_launch("dkv_release_blocks");
 }

@@ -52,7 +52,7 @@ extern "C" {
 /* Thread-local description of the last error on this thread. */
 const char* dkv_last_error(void);
 
-/* ABI version (16); bumps when a struct or an entry point below changes. */
+/* ABI version (17); bumps when a struct or an entry point below changes. */
 int dkv_abi_version(void);
 
 /*
@@ -502,7 +502,8 @@ int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
  * and the blocks they need, from the top of the stack in the requests' order.
  * slots [total] (int64, 16-byte aligned) becomes block * block_size + offset of
  * every new token, packed in the requests' order, and -1 behind the last; starts
- * [requests + 1] their first places.  Stack entries that are taken become -1.
+ * [requests + 1] their first places; positions [total] (int32, 16-byte aligned,
+ * optional) their places within the requests, -1 where slots are.  Stack entries that are taken become -1.
  * dkv_release_blocks drops the last tokens[r] of each request (all of them when
  * tokens is NULL, or more than it has) and returns the blocks that no token is
  * left in; it undoes a reserve of the same counts exactly (a block that keeps
@@ -513,6 +514,20 @@ int dkv_prompt_attention(const dkv_prompt_attention_args* args, void* stream);
  * negative count) or 8 (more new tokens than total); a reserve's slots are
  * then -1 and its starts 0.  Calls on one state run in order: two streams must
  * not run them at once.  At most 8,190 requests.
+ *
+ * shares [blocks] (int32, optional): how many requests beside one hold each block
+ * (dkv_fork_blocks); 0 for a free one.  With it,
+ *   - dkv_reserve_blocks gives a request that gets tokens in a block others hold a
+ *     copy of that block, a new one from the stack before the request's other new
+ *     blocks; of the writers in one call that are all of a block's holders, the last
+ *     keeps it.  copies [requests][3] lists what dkv_copy_blocks has to copy before
+ *     the tokens are appended: block, its copy, tokens; (-1, -1, -1) behind the last.
+ *     (A block is known by the token behind the request's last: a request whose last
+ *     block is full writes to a new one.)
+ *   - dkv_release_blocks returns the blocks that no request holds any more, the
+ *     lowest number on top of the stack, and leaves a request alone (status 2) whose
+ *     length is more than max_blocks blocks hold; workspace:
+ *     dkv_share_workspace_bytes.
  */
 typedef struct dkv_block_tables_args {
   int32_t* table;
@@ -523,10 +538,59 @@ typedef struct dkv_block_tables_args {
   int64_t* slots;
   int32_t* starts;
   int64_t total, requests, max_blocks, blocks, block_size;
+  int32_t* shares;
+  int32_t* copies;
+  const int32_t* sources;
+  int32_t* positions;
+  void* workspace;
+  int64_t workspace_bytes;
 } dkv_block_tables_args;
 
 int dkv_reserve_blocks(const dkv_block_tables_args* args, void* stream);
 int dkv_release_blocks(const dkv_block_tables_args* args, void* stream);
+
+/*
+ * dkv_fork_blocks: request r with sources[r] >= 0 becomes a copy of what request
+ * sources[r] was before the call, of its first tokens[r] tokens (tokens NULL, or more
+ * than it has: all), all requests at once; -1 leaves it as it is.  Blocks are not
+ * copied but held by both (shares, required); what no request holds any more returns to
+ * the stack, the lowest number on top.  A request whose source is not one, or whose
+ * count is negative, stays as it was (status 16 or 4).  Uses table, lengths, free,
+ * state, shares, sources, tokens and workspace.
+ *
+ * dkv_compact_blocks: the blocks in use move to the lowest numbers, so that the free
+ * ones are the highest: with n in use, the used ones from n on go to the free ones below
+ * n, both in ascending order.  Tables and shares follow, the stack has the lowest
+ * number on top; copies [blocks / 2][3] lists (block, its new number, block_size) for
+ * dkv_copy_blocks, (-1, -1, -1) behind the last.  shares may be NULL.  A state whose stack
+ * is not one (its count or entries outside the blocks) is left alone (status 1).
+ *
+ * dkv_share_workspace_bytes: the workspace (16-byte aligned, its contents need not be
+ * kept) of a dkv_fork_blocks, a dkv_compact_blocks or a dkv_release_blocks with shares.
+ */
+int64_t dkv_share_workspace_bytes(const dkv_block_tables_args* args);
+int dkv_fork_blocks(const dkv_block_tables_args* args, void* stream);
+int dkv_compact_blocks(const dkv_block_tables_args* args, void* stream);
+
+/*
+ * The first copies[i][2] tokens of block copies[i][0], and its scales, to block
+ * copies[i][1], for each of `count` entries, in each of `layers` layers: key_codes,
+ * value_codes [layers][blocks][H][block_size][D] and key_scale, value_scale
+ * [layers][blocks][H], each with its stride between layers (elements).  Entries with a
+ * number outside the blocks are skipped.  No target may be another entry's source or
+ * target.  D a multiple of 16 up to 512.
+ */
+typedef struct dkv_copy_blocks_args {
+  const int32_t* copies;
+  int64_t count, layers, blocks, H, block_size, D;
+  uint8_t* key_codes;
+  uint8_t* value_codes;
+  float* key_scale;
+  float* value_scale;
+  int64_t key_stride, value_stride, key_scale_stride, value_scale_stride;
+} dkv_copy_blocks_args;
+
+int dkv_copy_blocks(const dkv_copy_blocks_args* args, void* stream);
 
 /*
  * New keys and values [tokens][H][D] (bf16, fp16 or fp32; element (t, h, d) at
@@ -594,6 +658,114 @@ typedef struct dkv_block_attention_args {
 
 int64_t dkv_block_attention_workspace_bytes(const dkv_block_attention_args* args);
 int dkv_block_attention(const dkv_block_attention_args* args, void* stream);
+
+/*
+ * RMS norm of each query and key head and its rotation by the token's position:
+ * x r w with r = 1 / sqrt(mean(x^2) + eps) over the head's D channels (a NULL weight:
+ * no norm), then of the first 2 * half channels the pairs (i, i + half), or with
+ * interleaved (2 i, 2 i + 1), turn: a' = a cos_i - b sin_i, b' = b cos_i + a sin_i.
+ * fp32 between the load and one rounding.
+ *
+ * query, keys and the outputs have bf16, fp16 or fp32 element (b, t, h, d) at
+ * base[b * sb + t * st + h * sh + d], rows of D (a multiple of 8 up to 256) and weights
+ * [D] 16-byte aligned.  cos, sin: rows of half angles.  positions NULL: token (b, t)'s at
+ * b * c_sb + t * c_st; else int32 (wide_positions: int64) [batch * tokens], the rows of a
+ * table of table_rows rows; a position behind it makes the turned channels NaN, a negative
+ * one is of no token: its rows are 0 and have no part in the gradients.  Rows of
+ * cos and sin start at multiples of 16 bytes where half is a multiple of 8 (of two
+ * elements where it is even).
+ *
+ * The backward call takes the gradients of the outputs as q_grad, k_grad, and writes
+ * those of the inputs to q_out, k_out, and of the weights to q_weight_grad, k_weight_grad
+ * (weight_dtype; NULL: not wanted).  Sums are made in one order, whatever runs beside.
+ * workspace (16-byte aligned): dkv_rotate_heads_backward_workspace_bytes, where a
+ * weight's gradient is wanted.
+ *
+ * Beside dkv_decode_prep, which does this for one layout of one new token of each
+ * sequence and rounds after each step as the Transformers modules do (reference
+ * src/dart/integrations/qwen3.py:48-53).
+ */
+typedef struct dkv_rotate_heads_args {
+  const void* query;
+  const void* keys;
+  void* q_out;
+  void* k_out;
+  const void* q_grad;
+  const void* k_grad;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, qo_sb, qo_st, qo_sh, ko_sb, ko_st, ko_sh;
+  int64_t qg_sb, qg_st, qg_sh, kg_sb, kg_st, kg_sh;
+  const void* q_weight;
+  const void* k_weight;
+  void* q_weight_grad;
+  void* k_weight_grad;
+  const void* cos;
+  const void* sin;
+  const void* positions;
+  int64_t c_sb, c_st, table_rows, wide_positions;
+  int64_t batch, tokens, Hq, Hkv, D, half, interleaved;
+  int64_t dtype, weight_dtype, angle_dtype;
+  double eps;
+  void* workspace;
+  int64_t workspace_bytes;
+} dkv_rotate_heads_args;
+
+int dkv_rotate_heads(const dkv_rotate_heads_args* args, void* stream);
+int64_t dkv_rotate_heads_backward_workspace_bytes(const dkv_rotate_heads_args* args);
+int dkv_rotate_heads_backward(const dkv_rotate_heads_args* args, void* stream);
+
+/*
+ * dkv_append_blocks of keys that are normed and turned on their way (rounded to their
+ * type, then to codes), and their queries, in one launch: of `rotation` it takes query,
+ * q_out and their strides, Hq, weights, angles, positions (required), half (a multiple of
+ * 8), eps and interleaved; batch is 1, and tokens, Hkv (args->H), D and dtype are the same
+ * in both.  keys and k_out of `rotation` are not used.
+ */
+int dkv_append_rotated_blocks(const dkv_append_blocks_args* args, const dkv_rotate_heads_args* rotation, void* stream);
+
+/*
+ * For each of `rows` rows of `vocab` logits (bf16, fp16 or fp32, `stride` elements
+ * apart): logprobs, the log probability of tokens[row] (int32; wide_tokens: int64; 0 for
+ * a negative one, NaN for one of vocab or more); entropy, in nats; and with top > 0 (up to
+ * 64) the most likely alternatives, top_tokens and top_logprobs [rows][top], in
+ * descending order, the lower number first among equals.
+ *
+ * -inf is a logit of probability 0.  A row of nothing else has log probabilities -inf and
+ * entropy 0 (and a gradient of 0).  A NaN or an infinity makes the row's log
+ * probabilities and entropy NaN; NaN logits are no alternatives (where too few others are,
+ * top_tokens are -1).
+ *
+ * stats [rows][2] (optional): the row's maximum and log2 of its sum, which the backward
+ * call needs.  workspace (16-byte aligned): dkv_token_logprobs_workspace_bytes.
+ *
+ * The backward call writes the gradient of the logits to grads.out (rows `stride` apart)
+ * from those of logprobs, entropy and top_logprobs (NULL: 0); of args it reads logits,
+ * tokens, stats, entropy and top_tokens.  No counterpart in the reference.
+ */
+typedef struct dkv_token_logprobs_args {
+  const void* logits;
+  const void* tokens;
+  float* logprobs;
+  float* entropy;
+  float* stats;
+  float* top_logprobs;
+  int64_t* top_tokens;
+  int64_t stride, rows, vocab, top, dtype, wide_tokens;
+  void* workspace;
+  int64_t workspace_bytes;
+} dkv_token_logprobs_args;
+
+typedef struct dkv_token_logprobs_grads {
+  const float* logprobs;
+  const float* entropy;
+  const float* top_logprobs;
+  void* out;
+  int64_t stride;
+} dkv_token_logprobs_grads;
+
+int64_t dkv_token_logprobs_workspace_bytes(const dkv_token_logprobs_args* args);
+int dkv_token_logprobs(const dkv_token_logprobs_args* args, void* stream);
+int dkv_token_logprobs_backward(const dkv_token_logprobs_args* args, const dkv_token_logprobs_grads* grads,
+                                void* stream);
 
 #ifdef __cplusplus
 }
