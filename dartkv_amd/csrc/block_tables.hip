@@ -118,7 +118,13 @@ __device__ __forceinline__ void find_copies(const TablesParams& p, int32_t* copi
     const int32_t block = copied[r];
     if (block < 0) continue;
     int32_t rank = 0;
-    for (int q = 0; q < r; ++q) rank += copied[q] == block;
+    int q = 0;
+#pragma unroll 4
+    for (; q + 4 <= r; q += 4) {
+      const int4 four = *(const int4*)(copied + q);
+      rank += (four.x == block) + (four.y == block) + (four.z == block) + (four.w == block);
+    }
+    for (; q < r; ++q) rank += copied[q] == block;
     if (rank >= p.shares[block]) keeps |= 1u << i;
   }
   __syncthreads();
@@ -159,9 +165,10 @@ __device__ __forceinline__ void make_copies(const TablesParams& p, const Sum* su
 
 template <bool RESERVE, int SLOTS, bool SHARED>  // SLOTS: of a thread
 __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
-  extern __shared__ Sum sums[];                // [R + 1]: before each request
+  extern __shared__ __attribute__((aligned(16))) Sum sums[];  // [R + 1]: before each request
   int32_t* lens = (int32_t*)(sums + p.R + 1);  // [R]: the lengths before
-  int32_t* copied = lens + p.R;                // [R] (SHARED)
+  int32_t* copied = lens + p.R;                // [R] (SHARED), 16-byte aligned
+  copied += -(2 * (p.R + 1) + p.R) & 3;
   __shared__ Sum wave_sum[2][4];
   __shared__ int32_t flags, last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -300,7 +307,7 @@ int check_tables(const dkv_block_tables_args& a, const char* where, TablesParams
 
 template <bool SHARED>
 void launch_reserve(const TablesParams& p, hipStream_t stream) {
-  const int lds = (SHARED ? 16 : 12) * p.R + 8;
+  const int lds = (SHARED ? 16 : 12) * p.R + (SHARED ? 24 : 8);
   if (p.total <= 4 * kThreads) {
     const int64_t groups = p.total > kThreads ? (p.total + kThreads - 1) / kThreads : 1;
     hipLaunchKernelGGL((block_tables<true, 1, SHARED>), dim3((unsigned)groups), dim3(kThreads), lds, stream, p);

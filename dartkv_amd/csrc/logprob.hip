@@ -17,6 +17,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "dkv_capi_util.h"
 #include "dkv_device.h"
 
@@ -26,7 +28,8 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
-constexpr int kDeep = 4;  // chunks of 16 bytes a thread has in flight
+constexpr int kPartChunks = 4;  // of a thread, in the smallest part of a row
+constexpr int kDeep = 2;  // chunks of 16 bytes a thread computes on, while as many are on their way
 constexpr float kLog2E = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 struct LogprobParams {
@@ -84,37 +87,56 @@ __device__ __forceinline__ uint64_t shuffle(uint64_t v, int lane) {
   return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)v, lane, 64);
 }
 
-// Keeps the larger of this lane's and lane ^ stride's, or the smaller.
-template <typename T>
-__device__ __forceinline__ T exchange(T v, T other, bool larger) {
-  return (v > other) == larger ? v : other;
+// Lane ^ STRIDE's value, without a way through LDS: permutations within four, mirrors and rotations within rows of 16, and
+// swaps of rows and halves.
+template <int STRIDE>
+__device__ __forceinline__ uint32_t across(uint32_t v, int lane) {
+  const auto dpp = [](uint32_t x, auto control) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(control)::value, 0xf, 0xf, true);
+  };
+  if constexpr (STRIDE == 1) return dpp(v, std::integral_constant<int, 0xb1>());
+  if constexpr (STRIDE == 2) return dpp(v, std::integral_constant<int, 0x4e>());
+  if constexpr (STRIDE == 4)  // lane ^ 7, then ^ 3
+    return dpp(dpp(v, std::integral_constant<int, 0x141>()), std::integral_constant<int, 0x1b>());
+  if constexpr (STRIDE == 8) return dpp(v, std::integral_constant<int, 0x128>());
+  if constexpr (STRIDE == 16) {
+    const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return lane & 16 ? both[0] : both[1];
+  }
+  if constexpr (STRIDE == 32) {
+    const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? both[0] : both[1];
+  }
+}
+template <int STRIDE>
+__device__ __forceinline__ uint64_t across(uint64_t v, int lane) {
+  return (uint64_t)across<STRIDE>((uint32_t)(v >> 32), lane) << 32 | across<STRIDE>((uint32_t)v, lane);
 }
 
-__device__ __forceinline__ uint64_t sort_lanes(uint64_t v, int lane) {  // the largest in lane 0
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1)
-      v = exchange(v, shuffle(v, lane ^ stride), ((lane & stride) == 0) == ((lane & size) == 0));
+// One step of a sorting network: the larger goes to the lower lane, in lanes with SIZE set to the higher one.
+template <int SIZE, int STRIDE, typename T>
+__device__ __forceinline__ T exchange(T v, int lane) {
+  const T other = across<STRIDE>(v, lane);
+  return (v > other) == (((lane & STRIDE) == 0) == ((lane & SIZE) == 0)) ? v : other;
+}
+
+template <int SIZE, int STRIDE, typename T>
+__device__ __forceinline__ T exchanges(T v, int lane) {
+  if constexpr (STRIDE > 0) return exchanges<SIZE, STRIDE / 2>(exchange<SIZE, STRIDE>(v, lane), lane);
   return v;
 }
 
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1)
-      v = exchange(v, (uint32_t)__shfl_xor((int)v, stride, 64), ((lane & stride) == 0) == ((lane & size) == 0));
+template <typename T, int SIZE = 2>
+__device__ __forceinline__ T sort_lanes(T v, int lane) {  // the largest in lane 0
+  v = exchanges<SIZE, SIZE / 2>(v, lane);
+  if constexpr (SIZE < 64) return sort_lanes<T, 2 * SIZE>(v, lane);
   return v;
 }
 
 // The 64 largest of two sorted lists, sorted.
 __device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b, int lane) {
   const uint64_t other = shuffle(b, 63 - lane);
-  uint64_t v = a > other ? a : other;
-#pragma unroll
-  for (int stride = 32; stride > 0; stride >>= 1) v = exchange(v, shuffle(v, lane ^ stride), (lane & stride) == 0);
-  return v;
+  return exchanges<64, 32>(a > other ? a : other, lane);
 }
 
 // What a wave keeps of the largest it has seen.
@@ -175,10 +197,83 @@ struct Chunk {  // 16 bytes of a row
       }
     }
   }
+  // Element `lane` of lane l's chunk (lanes from kElements on: something else).
+  __device__ __forceinline__ float of_lane(int l, int lane) const {
+    uint32_t u = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)w[i], l);
+      if ((DT == kF32 ? lane : lane >> 1) == i) u = word;
+    }
+    if (DT == kF32) return u2f(u);
+    const uint32_t half = lane & 1 ? u >> 16 : u & 0xffffu;
+    return DT == kBF16 ? u2f(half << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+  }
   __device__ __forceinline__ float get(int i) const {
     if (DT == kF32) return u2f(w[i]);
     if (DT == kBF16) return u2f(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+  }
+};
+
+// A row as a split's wave reads it: kDeep chunks of each lane at a time, a workgroup's chunks next to each other.
+template <int DT, int THREADS>  // THREADS: of a row's part
+struct Group {
+  static constexpr int E = Chunk<DT>::kElements;
+  Chunk<DT> chunk[kDeep];
+  bool whole;  // for the wave: nothing but the row
+  // The group of chunks c + i * THREADS (c: this lane's); what is not the row's or the split's is -inf.
+  __device__ __forceinline__ void load(const char* aligned, int64_t c, int lane, int64_t stop, int off, int64_t V) {
+    const int64_t first = c - lane, last = first + 63 + (kDeep - 1) * THREADS;
+    whole = first * E >= off && last < stop && (last + 1) * E - off <= V;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        const uint4 u = *(const uint4*)(aligned + (c + i * THREADS) * 16);
+        chunk[i].w[0] = u.x, chunk[i].w[1] = u.y, chunk[i].w[2] = u.z, chunk[i].w[3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
+        const bool in = c + i * THREADS < stop;
+        chunk[i].load(aligned, in ? c + i * THREADS : 0, off, in ? V : -1);
+      }
+    }
+  }
+  // The registers hold something unknown from here: what was made of them is not kept.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(chunk[i].w[j]));
+  }
+  __device__ __forceinline__ void largest(float (&top)[kDeep]) const {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      top[i] = chunk[i].get(0);
+#pragma unroll
+      for (int j = 1; j < E; ++j) top[i] = fmaxf(top[i], chunk[i].get(j));
+    }
+  }
+  __device__ __forceinline__ void add(Sums& a) const {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float z = (chunk[i].get(j) - a.m) * kLog2E, e = __builtin_amdgcn_exp2f(z);
+        a.s += e, a.t = fmaf(e, z, a.t);
+      }
+    }
+  }
+  __device__ __forceinline__ void add_careful(Sums& a) const {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float z = (chunk[i].get(j) - a.m) * kLog2E, e = __builtin_amdgcn_exp2f(z);
+        a.s += e, a.t = fmaf(e, finite(z), a.t);
+      }
+    }
   }
 };
 
@@ -213,13 +308,18 @@ __device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Sum
   }
 }
 
-template <int DT, bool TOP>
+// WAVES of a workgroup share a part of a row: all four, or each has a row of its own.
+template <int DT, bool TOP, int WAVES>
 __global__ void __launch_bounds__(kThreads) logprob_rows(LogprobParams p) {
   constexpr int E = Chunk<DT>::kElements;
   __shared__ Sums wave_sums[kWaves];
   __shared__ uint64_t buffers[TOP ? kWaves : 1][TOP ? 128 : 1];
-  const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t shared_bound;
+  constexpr int kPart = 64 * WAVES;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, thread = threadIdx.x & (kPart - 1);
+  const uint32_t part = WAVES == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
+  const uint32_t row = part / p.splits, split = part - row * p.splits;
+  if (WAVES == 1 && row >= p.rows) return;
   const char* base = p.logits + row * p.stride;
   const int off = (int)((uintptr_t)base & 15) / Chunk<DT>::kSize;
   const char* aligned = base - off * Chunk<DT>::kSize;
@@ -229,48 +329,80 @@ __global__ void __launch_bounds__(kThreads) logprob_rows(LogprobParams p) {
 
   Sums sums = {-FLT_MAX, 0.f, 0.f};
   Best best;
-  bool begun = false;
-  for (int64_t c0 = split * p.chunks + threadIdx.x; c0 - lane < stop; c0 += kDeep * kThreads) {
-    Chunk<DT> chunk[kDeep];
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-      // (behind the split's last chunk: nothing but -inf)
-      const int64_t c = c0 + i * kThreads;
-      chunk[i].load(aligned, c < stop ? c : 0, off, c < stop ? p.V : -1);
+  float seen = -INFINITY;  // the largest of this lane
+  int steps = 0, refresh = 1;
+  if constexpr (TOP) {
+    if (WAVES > 1) {
+      if (threadIdx.x == 0) shared_bound = 0;
+      __syncthreads();
     }
+  }
+  Group<DT, kPart> next;
+  int64_t c0 = split * p.chunks + thread;
+  if (c0 - lane < stop) next.load(aligned, c0, lane, stop, off, p.V);
+  for (; c0 - lane < stop; c0 += kDeep * kPart) {
+    Group<DT, kPart> group = next;
+    if (c0 - lane + kDeep * kPart < stop) next.load(aligned, c0 + kDeep * kPart, lane, stop, off, p.V);
     float top[kDeep], most = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-      top[i] = chunk[i].get(0);
-#pragma unroll
-      for (int j = 1; j < E; ++j) top[i] = fmaxf(top[i], chunk[i].get(j));
-      most = fmaxf(most, top[i]);
-    }
-    if (most > sums.m) raise(sums, most);
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float z = (chunk[i].get(j) - sums.m) * kLog2E, e = __builtin_amdgcn_exp2f(z);
-        sums.s += e, sums.t = fmaf(e, finite(z), sums.t);
-      }
-    }
     if constexpr (TOP) {
-      if (!begun) {  // at least top values are as large as the top-th largest of the lanes' maxima
-        begun = true;
-        const uint32_t sorted = sort_lanes(order_of(most), lane);
-        const uint32_t kth = (uint32_t)__shfl((int)sorted, p.top - 1, 64);
+      group.largest(top);
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) most = fmaxf(most, top[i]);
+    }
+    // m need not be the maximum while 2^z and its sum are far from infinity: it is raised when they are not.  The first
+    // step, ends of rows and steps with a -inf take the careful way, which raises it before.
+    Sums sum = sums;
+    bool careful = steps == 0 || !group.whole;
+    if (!careful) {
+      group.add(sum);
+      careful = !__all(sum.s < 0x1p100f && sum.t == sum.t);
+    }
+    if (careful) {
+      group.forget();
+      if constexpr (!TOP) {
+        group.largest(top);
+#pragma unroll
+        for (int i = 0; i < kDeep; ++i) most = fmaxf(most, top[i]);
+      }
+      if (most > sums.m) raise(sums, most);
+      group.add_careful(sums);
+    } else {
+      sums = sum;
+    }
+    ++steps;
+    if constexpr (TOP) {
+      seen = fmaxf(seen, most);
+      if (steps == refresh) {  // after 1, 2, 4, .. steps
+        // at least top values are as large as the top-th largest of the lanes' maxima, so the row's top-th is; each wave's
+        // bound serves the others
+        refresh *= 2;
+        const uint32_t sorted = sort_lanes(order_of(seen), lane);
+        uint32_t kth = (uint32_t)__builtin_amdgcn_readlane((int)sorted, p.top - 1);
+        if (WAVES > 1 && lane == 0) kth = max(kth, atomicMax(&shared_bound, kth));
+        kth = (uint32_t)__builtin_amdgcn_readfirstlane((int)kth);
         if (kth > kLowest) best.raise_bound(((uint64_t)kth << 32) - 1);
       }
+      if (__any(most >= best.least)) {
 #pragma unroll
-      for (int i = 0; i < kDeep; ++i) {
-        if (__any(top[i] >= best.least)) {
-          const int64_t first = (c0 + i * kThreads) * E - off;
-          const bool in = c0 + i * kThreads < stop;
+        for (int i = 0; i < kDeep; ++i) {
+          uint64_t lanes = __ballot(top[i] >= best.least);
+          const int64_t c = c0 + i * kPart;
+          if (__builtin_popcountll(lanes) > 4) {
 #pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const bool real = in && first + j >= 0 && first + j < p.V;
-            best.add(real ? key_of(chunk[i].get(j), (uint32_t)(first + j)) : 0, buffer, p.top, lane);
+            for (int j = 0; j < E; ++j) {
+              const int64_t index = c * E - off + j;
+              const bool real = c < stop && index >= 0 && index < p.V;
+              best.add(real ? key_of(group.chunk[i].get(j), (uint32_t)index) : 0, buffer, p.top, lane);
+            }
+          } else {
+            while (lanes) {  // lane j takes element j of that lane's chunk
+              const int l = __builtin_ctzll(lanes);
+              lanes &= lanes - 1;
+              const float x = group.chunk[i].of_lane(l, lane);
+              const int64_t from = c - lane + l, index = from * E - off + lane;
+              const bool real = lane < E && from < stop && index >= 0 && index < p.V;
+              best.add(real ? key_of(x, (uint32_t)index) : 0, buffer, p.top, lane);
+            }
           }
         }
       }
@@ -278,42 +410,58 @@ __global__ void __launch_bounds__(kThreads) logprob_rows(LogprobParams p) {
   }
   if constexpr (TOP) best.flush(buffer, p.top, lane);
   sums = wave_join(sums);
-  if constexpr (TOP) {
-    buffer[lane] = best.list;
-  }
-  if (lane == 0) wave_sums[wave] = sums;
-  __syncthreads();
-  if (wave != 0) return;
+  if constexpr (WAVES > 1) {
+    if constexpr (TOP) buffer[lane] = best.list;
+    if (lane == 0) wave_sums[wave] = sums;
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    sums = join(sums, wave_sums[w]);
-    if constexpr (TOP) best.list = merge_lists(best.list, buffers[w][lane], lane);
+    for (int w = 1; w < WAVES; ++w) {
+      sums = join(sums, wave_sums[w]);
+      if constexpr (TOP) best.list = merge_lists(best.list, buffers[w][lane], lane);
+    }
   }
   if (p.splits == 1) {
     finish<DT>(p, row, sums, best.list, lane);
   } else {
-    if (lane == 0) *(float4*)(p.records + 4 * (int64_t)blockIdx.x) = make_float4(sums.m, sums.s, sums.t, 0.f);
-    if (lane < p.top) p.lists[(int64_t)blockIdx.x * p.top + lane] = best.list;
+    if (lane == 0) *(float4*)(p.records + 4 * (int64_t)part) = make_float4(sums.m, sums.s, sums.t, 0.f);
+    if (lane < p.top) p.lists[(int64_t)part * p.top + lane] = best.list;
   }
 }
 
-// A wave joins the parts of a row.
-template <int DT>
-__global__ void __launch_bounds__(64) logprob_join(LogprobParams p) {
+// The parts of a row joined by the waves of a workgroup: each takes every WAVES-th part, then they meet in pairs.
+template <int DT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) logprob_join(LogprobParams p) {
+  __shared__ Sums wave_sums[WAVES];
+  __shared__ uint64_t lists[WAVES][64];
   const uint32_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t first = (int64_t)row * p.splits;
   Sums sums = {-FLT_MAX, 0.f, 0.f};
-  for (int i = lane; i < p.splits; i += 64) {
+  for (int i = threadIdx.x; i < p.splits; i += 64 * WAVES) {
     const float4 r = *(const float4*)(p.records + 4 * (first + i));
     sums = join(sums, {r.x, r.y, r.z});
   }
   uint64_t list = 0;
-  if (p.top) {
-    for (int i = 0; i < p.splits; ++i)
+  if (p.top)
+    for (int i = wave; i < p.splits; i += WAVES)
       list = merge_lists(list, lane < p.top ? p.lists[(first + i) * p.top + lane] : 0, lane);
+  sums = wave_join(sums);
+  if (lane == 0) wave_sums[wave] = sums;
+  if (p.top) {
+#pragma unroll
+    for (int half = WAVES / 2; half > 0; half /= 2) {
+      if (wave >= half && wave < 2 * half) lists[wave][lane] = list;
+      __syncthreads();
+      if (wave < half) list = merge_lists(list, lists[wave + half][lane], lane);
+    }
+  } else {
+    __syncthreads();
   }
-  finish<DT>(p, row, wave_join(sums), list, lane);
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) sums = join(sums, wave_sums[w]);
+  finish<DT>(p, row, sums, list, lane);
 }
 
 struct GradParams {
@@ -408,12 +556,14 @@ __global__ void __launch_bounds__(kThreads) logprob_backward(GradParams p) {
   }
 }
 
+constexpr int64_t kManyRows = 2048;  // from which on each has one wave
+
 // Parts of a row: enough workgroups for the card (eight a CU) where there are few rows, none smaller than one step of
 // its loop.
 int64_t parts_of(int64_t rows, int64_t V, int64_t dtype, int deep) {
   const int64_t E = dtype == kF32 ? 4 : 8, chunks = (V + 2 * E - 1) / E;
   const int64_t most = (chunks + (int64_t)deep * kThreads - 1) / ((int64_t)deep * kThreads);
-  const int64_t want = (2048 + rows - 1) / rows;
+  const int64_t want = (1024 + rows - 1) / rows;
   return want < most ? want : most;
 }
 
@@ -437,7 +587,7 @@ int check_logprobs(const dkv_token_logprobs_args& a, const char* where) {
 
 extern "C" int64_t dkv_token_logprobs_workspace_bytes(const dkv_token_logprobs_args* args) {
   if (!args || check_logprobs(*args, "dkv_token_logprobs") != DKV_OK || args->rows == 0) return 0;
-  const int64_t parts = parts_of(args->rows, args->vocab, args->dtype, kDeep);
+  const int64_t parts = parts_of(args->rows, args->vocab, args->dtype, kPartChunks);
   return parts == 1 ? 0 : args->rows * parts * (16 + 8 * args->top);
 }
 
@@ -458,7 +608,7 @@ extern "C" int dkv_token_logprobs(const dkv_token_logprobs_args* args, void* str
   p.top_logprobs = a.top_logprobs, p.top_tokens = a.top_tokens;
   p.stride = a.stride * esize, p.V = (int32_t)a.vocab, p.top = (int32_t)a.top, p.wide = a.wide_tokens != 0;
   p.rows = (uint32_t)a.rows;
-  const int64_t parts = parts_of(a.rows, a.vocab, a.dtype, kDeep);
+  const int64_t parts = parts_of(a.rows, a.vocab, a.dtype, kPartChunks);
   p.splits = (int32_t)parts, p.chunks = chunks_of(a.vocab, a.dtype, parts);
   if (parts > 1) {
     DKV_CHECK(a.workspace && ((uintptr_t)a.workspace & 15) == 0 &&
@@ -470,13 +620,19 @@ extern "C" int dkv_token_logprobs(const dkv_token_logprobs_args* args, void* str
   DKV_CHECK(a.rows * parts < (1ll << 31), DKV_ERR_INVALID, "%s: too many rows", where);
   const dim3 grid((unsigned)(a.rows * parts)), block(kThreads);
   const hipStream_t s = (hipStream_t)stream;
+  const bool alone = parts == 1 && a.rows >= kManyRows;
+  const dim3 fewer((unsigned)((a.rows + kWaves - 1) / kWaves));
 #define DKV_LOGPROBS(DT)                                                         \
   do {                                                                           \
-    if (p.top)                                                                   \
-      hipLaunchKernelGGL((logprob_rows<DT, true>), grid, block, 0, s, p);        \
+    if (alone && p.top)                                                          \
+      hipLaunchKernelGGL((logprob_rows<DT, true, 1>), fewer, block, 0, s, p);    \
+    else if (alone)                                                              \
+      hipLaunchKernelGGL((logprob_rows<DT, false, 1>), fewer, block, 0, s, p);   \
+    else if (p.top)                                                              \
+      hipLaunchKernelGGL((logprob_rows<DT, true, kWaves>), grid, block, 0, s, p);  \
     else                                                                         \
-      hipLaunchKernelGGL((logprob_rows<DT, false>), grid, block, 0, s, p);       \
-    if (parts > 1) hipLaunchKernelGGL(logprob_join<DT>, dim3((unsigned)a.rows), dim3(64), 0, s, p); \
+      hipLaunchKernelGGL((logprob_rows<DT, false, kWaves>), grid, block, 0, s, p); \
+    if (parts > 1) hipLaunchKernelGGL((logprob_join<DT, 8>), dim3((unsigned)a.rows), dim3(512), 0, s, p); \
   } while (0)
   if (a.dtype == kF32)
     DKV_LOGPROBS(kF32);

@@ -24,11 +24,11 @@ constexpr int kMaxDim = kMaxRotateDim;
 constexpr int kMaxGroups = 1024;  // workgroups of a backward pass, each with its sums of the weights' gradients
 
 
-template <int DT, int VEC, bool NEXT, int K>
+template <int DT, int VEC, bool NEXT, int K, int N>
 __global__ void __launch_bounds__(kThreads) rotate_heads(RotateParams p) {
   const bool keys = blockIdx.x >= p.side[0].groups;
   const uint32_t group = blockIdx.x - (keys ? p.side[0].groups : 0);
-  rotate_rows<DT, VEC, NEXT, K>(p, p.side[keys], group * kWaves + (threadIdx.x >> 6));
+  rotate_rows<DT, VEC, NEXT, K, N>(p, p.side[keys], group * kWaves + (threadIdx.x >> 6));
 }
 
 template <int DT, int VEC, bool NEXT, int K>
@@ -135,20 +135,28 @@ __global__ void __launch_bounds__(kThreads) rotate_backward(RotateParams p) {
   }
 }
 
-// The workgroups' sums of the weights' gradients: 16 channels a workgroup, 16 threads each.
-__global__ void __launch_bounds__(kThreads) rotate_weights(RotateParams p) {
+// The workgroups' sums of the weights' gradients: 16 channels a workgroup, 64 threads each, whose loads are all in flight.
+__global__ void __launch_bounds__(1024) rotate_weights(RotateParams p) {
   const RotateSide& side = p.side[blockIdx.y];
   const int column = threadIdx.x & 15, part = threadIdx.x >> 4, d = blockIdx.x * 16 + column;
-  __shared__ float sums[16][17];
+  __shared__ float sums[64][17];
   float sum = 0.f;
-  if (d < p.D && side.dw)
-    for (uint32_t g = part; g < side.groups; g += 16) sum += side.sums[(int64_t)g * p.D + d];
+  if (d < p.D && side.dw) {
+    float x[kMaxGroups / 64];
+#pragma unroll
+    for (int i = 0; i < kMaxGroups / 64; ++i) {
+      const uint32_t g = part + 64 * i;
+      x[i] = g < side.groups ? side.sums[(int64_t)g * p.D + d] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxGroups / 64; ++i) sum += x[i];
+  }
   sums[part][column] = sum;
   __syncthreads();
   if (part == 0 && d < p.D && side.dw) {
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += sums[i][column];
+    for (int i = 0; i < 64; ++i) sum += sums[i][column];
     dev_store(side.dw, d, sum, p.w_dtype);
   }
 }
@@ -171,11 +179,17 @@ void launch_rotate(const RotateParams& p, bool next, bool backward, hipStream_t 
       hipLaunchKernelGGL((rotate_backward<DT, VEC, true, K>), grid, block, 0, stream, p);
     else
       hipLaunchKernelGGL((rotate_backward<DT, VEC, false, K>), grid, block, 0, stream, p);
-  } else {
+  } else if (p.steps == 1) {
     if (next)
-      hipLaunchKernelGGL((rotate_heads<DT, VEC, true, K>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, true, K, 1>), grid, block, 0, stream, p);
     else
-      hipLaunchKernelGGL((rotate_heads<DT, VEC, false, K>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, false, K, 1>), grid, block, 0, stream, p);
+  } else {
+    constexpr int N = kRotateSteps;
+    if (next)
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, true, K, N>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((rotate_heads<DT, VEC, false, K, N>), grid, block, 0, stream, p);
   }
 }
 
@@ -197,15 +211,16 @@ int run_rotate(const dkv_rotate_heads_args& a, bool backward, const char* where,
   DKV_CHECK(a.query && a.keys && a.q_out && a.k_out && (a.half == 0 || (a.cos && a.sin)) &&
                 (!backward || (a.q_grad && a.k_grad)),
             DKV_ERR_INVALID, "%s: NULL pointer", where);
+  const RotateShape s = rotate_shape(a.D, a.half);
   if (backward) {
+    p.steps = 1;
     for (int i = 0; i < 2; ++i) {
-      const uint32_t groups = p.side[i].groups;
       p.side[i].groups = (uint32_t)backward_groups(a, i);
-      const int32_t steps = (int32_t)((groups + p.side[i].groups - 1) / p.side[i].groups);
+      const int64_t per_turn = (int64_t)p.side[i].groups * kWaves << s.rows_shift;
+      const int32_t steps = (int32_t)((p.side[i].rows + per_turn - 1) / per_turn);
       p.steps = steps > p.steps ? steps : p.steps;
     }
   }
-  const RotateShape s = rotate_shape(a.D, a.half);
   const bool weights = backward && (a.q_weight_grad || a.k_weight_grad);
   if (weights) {
     DKV_CHECK((!a.q_weight_grad || a.q_weight) && (!a.k_weight_grad || a.k_weight), DKV_ERR_INVALID,
@@ -225,11 +240,24 @@ int run_rotate(const dkv_rotate_heads_args& a, bool backward, const char* where,
   else
     launch_vec<kBF16>(p, s.vec, next, backward, stream);
   if (weights)
-    hipLaunchKernelGGL(rotate_weights, dim3((unsigned)((a.D + 15) / 16), 2), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(rotate_weights, dim3((unsigned)((a.D + 15) / 16), 2), dim3(1024), 0, stream, p);
   return dkv_check_launch(where);
 }
 
 }  // namespace
+
+namespace dkv {
+
+void launch_rotate_heads(const RotateParams& p, int dtype, int vec, bool next, hipStream_t stream) {
+  if (dtype == kF32)
+    launch_vec<kF32>(p, vec, next, false, stream);
+  else if (dtype == kF16)
+    launch_vec<kF16>(p, vec, next, false, stream);
+  else
+    launch_vec<kBF16>(p, vec, next, false, stream);
+}
+
+}  // namespace dkv
 
 extern "C" int64_t dkv_rotate_heads_backward_workspace_bytes(const dkv_rotate_heads_args* args) {
   if (!args || check_rotate(*args, "dkv_rotate_heads_backward") != DKV_OK) return 0;
