@@ -21,25 +21,33 @@ from typing import Optional
 
 import torch
 
+from ..logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .huggingface import DartHFCache
 
 
 class GraphDecodeStep:
     """Greedy decode steps over ``cache``: ``input_ids`` [B, 1] and ``position_ids`` [1, 1] (device int64)
-    are read and advanced in place; ``logits`` holds the last step's [B, vocab] logits."""
+    are read and advanced in place; ``logits`` holds the last step's [B, vocab] logits.
+
+    ``top_logprobs``: ``logprobs`` holds the last step's ``TokenLogprobs`` of the generated tokens, with that many
+    alternatives (``token_logprobs``, within the captured step)."""
 
     def __init__(self, model: torch.nn.Module, cache: DartHFCache, input_ids: torch.Tensor,
-                 position_ids: torch.Tensor, *, use_graph: bool = True) -> None:
+                 position_ids: torch.Tensor, *, use_graph: bool = True, top_logprobs: Optional[int] = None) -> None:
         if input_ids.ndim != 2 or input_ids.shape[1] != 1 or input_ids.device.type != "cuda":
             raise ValueError("input_ids must be a [B, 1] device tensor")
         if position_ids.shape != (1, 1) or position_ids.device != input_ids.device:
             raise ValueError("position_ids must be a [1, 1] tensor on the input's device")
+        if top_logprobs is not None and not 0 <= top_logprobs <= MAX_TOP:
+            raise ValueError(f"top_logprobs must be from 0 to {MAX_TOP}")
         self.model = model
         self.cache = cache
         self.input_ids = input_ids
         self.position_ids = position_ids
         self.use_graph = use_graph
         self.logits: Optional[torch.Tensor] = None
+        self.top_logprobs = top_logprobs
+        self.logprobs: Optional[TokenLogprobs] = None
         self.captures = 0
         self.eager_steps = 0
         self.replays = 0
@@ -54,7 +62,15 @@ class GraphDecodeStep:
         if self.logits is None:
             self.logits = torch.empty_like(last)
         self.logits.copy_(last)
-        self.input_ids.copy_(last.argmax(-1, keepdim=True))
+        chosen = last.argmax(-1, keepdim=True)
+        if self.top_logprobs is not None:
+            with torch.no_grad():
+                out = token_logprobs(last, chosen.squeeze(-1), top=self.top_logprobs)
+            if self.logprobs is None:
+                self.logprobs = TokenLogprobs(*(torch.empty_like(t) for t in out))
+            for kept, t in zip(self.logprobs, out):
+                kept.copy_(t)
+        self.input_ids.copy_(chosen)
         self.position_ids.add_(1)
 
     def step(self) -> torch.Tensor:

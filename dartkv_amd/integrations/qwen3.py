@@ -11,6 +11,10 @@ that the model's backend would run as plain causal attention without a mask
 (``sdpa``, bf16 or fp16, no gradients, no sliding window) on
 ``prompt_attention`` instead; every other call keeps the backend.
 
+``attach_dart_fused_attention(model, rotate_heads=True)`` runs the norms of queries and
+keys and the rotary embedding on ``rotate_heads`` (one pass, one rounding, with
+gradients) in every call that does not run on the preparation kernel below.
+
 The forward accepts the cache under both keyword names Transformers has used
 (``past_key_values`` in 5.x, ``past_key_value`` in 4.x).
 
@@ -33,6 +37,7 @@ from torch import nn
 from .. import _lib
 from ..fused_attention import fused_dart_attention
 from ..prompt import MAX_PROMPT_HEAD_DIM, followed, prompt_attention
+from ..rotate import DTYPES, MAX_ROTATE_HEAD_DIM, rotate_heads
 from .huggingface import DartHFCache
 
 
@@ -146,6 +151,26 @@ def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, va
             and not followed(query, keys, values))
 
 
+def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tensor, cos: torch.Tensor,
+                sin: torch.Tensor) -> bool:
+    """Whether the norms and the rotation of these projections [B, T, H, D] are what ``rotate_heads`` computes."""
+    norms = (attn.q_norm, attn.k_norm)
+    return (getattr(attn, "dart_rotate_heads", False) and query.device.type == "cuda"
+            and all(type(n) is modules.Qwen3RMSNorm for n in norms)
+            and norms[0].variance_epsilon == norms[1].variance_epsilon
+            and query.dtype == keys.dtype and query.dtype in DTYPES and cos.dtype in DTYPES and sin.dtype == cos.dtype
+            and norms[0].weight.dtype == norms[1].weight.dtype and norms[0].weight.dtype in DTYPES
+            and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_ROTATE_HEAD_DIM
+            and cos.dim() == 3 and cos.shape == sin.shape and cos.shape[0] in (1, query.shape[0])
+            and cos.shape[1:] == (query.shape[1], attn.head_dim) and not followed(cos, sin)
+            and not _has_tangent(query, keys, norms[0].weight, norms[1].weight))
+
+
+def _has_tangent(*tensors: torch.Tensor) -> bool:
+    with torch.no_grad():
+        return followed(*tensors)
+
+
 class DartQwen3Attention:  # replaced by build_dart_qwen3_attention_class()
     """Placeholder; the real class subclasses the installed Qwen3Attention."""
 
@@ -175,11 +200,19 @@ def build_dart_qwen3_attention_class():
                 attn_output = attn_output.reshape(*input_shape, -1).contiguous()
                 return self.o_proj(attn_output), None
             hidden_shape = (*input_shape, -1, self.head_dim)
-            query_states = self.q_norm(self.q_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
-            key_states = self.k_norm(self.k_proj(hidden_states).view(hidden_shape)).transpose(1, 2)
+            query_states = self.q_proj(hidden_states).view(hidden_shape)
+            key_states = self.k_proj(hidden_states).view(hidden_shape)
             value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
-
-            query_states, key_states = modules.apply_rotary_pos_emb(query_states, key_states, cos, sin)
+            if _can_rotate(self, modules, query_states, key_states, cos, sin):
+                half = self.head_dim // 2  # (cos and sin hold the angles twice)
+                query_states, key_states = rotate_heads(
+                    query_states.transpose(1, 2), key_states.transpose(1, 2), cos[..., :half], sin[..., :half],
+                    q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.variance_epsilon,
+                )
+            else:
+                query_states = self.q_norm(query_states).transpose(1, 2)
+                key_states = self.k_norm(key_states).transpose(1, 2)
+                query_states, key_states = modules.apply_rotary_pos_emb(query_states, key_states, cos, sin)
 
             use_dart_decode = isinstance(cache, DartHFCache)
             if cache is not None:
@@ -221,9 +254,11 @@ def build_dart_qwen3_attention_class():
     return _DartQwen3Attention
 
 
-def attach_dart_fused_attention(model: nn.Module, *, prompt_attention: bool = False) -> nn.Module:
+def attach_dart_fused_attention(model: nn.Module, *, prompt_attention: bool = False,
+                                rotate_heads: bool = False) -> nn.Module:
     """Replace every Qwen3 self-attention module with the Dart adapter.  ``prompt_attention``: run prefills on the
-    HIP prompt kernel where it computes what the backend would (results differ by roundings)."""
+    HIP prompt kernel where it computes what the backend would; ``rotate_heads``: run the norms of queries and keys and
+    the rotary embedding on the HIP kernel for them (results differ by roundings)."""
     attention_class = build_dart_qwen3_attention_class()
     layers = getattr(getattr(model, "model", None), "layers", None)
     if layers is None:
@@ -238,6 +273,7 @@ def attach_dart_fused_attention(model: nn.Module, *, prompt_attention: bool = Fa
         replacement.train(original.training)
         _share_qkv_storage(replacement)
         replacement.dart_prompt_attention = prompt_attention
+        replacement.dart_rotate_heads = rotate_heads
         layer.self_attn = replacement
     return model
 

@@ -97,6 +97,38 @@ def _backward(logits, tokens, moments, entropy, top_tokens, grads):
     return out
 
 
+def _rows(logits, tokens):
+    """[rows, V] logits and [rows] tokens."""
+    rows = logits.reshape(-1, logits.shape[-1])
+    return rows if rows.stride(1) == 1 else rows.contiguous(), tokens.reshape(-1).contiguous()
+
+
+def with_moments(logits, tokens, top):
+    """``TokenLogprobs``' four, and the rows' moments [.., 2], which ``gradient`` takes."""
+    _checked(logits, tokens, top)
+    shape = tokens.shape
+    logprobs, entropy, top_logprobs, top_tokens, moments = _forward(*_rows(logits, tokens), top, True)
+    return (logprobs.view(shape), entropy.view(shape), top_logprobs.view(*shape, top), top_tokens.view(*shape, top),
+            moments.view(*shape, 2))
+
+
+def gradient(logprobs, entropy, top_logprobs, logits, tokens, moments, row_entropy, top_tokens):
+    """The gradient of logits [.., V] from those of their results; the rest as ``with_moments`` gave it."""
+    top = top_tokens.shape[-1]
+    _checked(logits, tokens, top)
+    shape = tuple(tokens.shape)
+    given = (logprobs, shape), (entropy, shape), (row_entropy, shape), (top_logprobs, (*shape, top)), \
+        (top_tokens, (*shape, top)), (moments, (*shape, 2))
+    if any(tuple(t.shape) != s or t.device != logits.device for t, s in given) or top_tokens.dtype != torch.int64:
+        raise ValueError("the results' gradients, moments and alternatives must be those of the logits")
+    rows, flat = _rows(logits, tokens)
+    n = flat.numel()
+    moments, row_entropy = (t.to(torch.float32).contiguous() for t in (moments, row_entropy))
+    out = _backward(rows, flat, moments, row_entropy, top_tokens.contiguous().view(n, top),
+                    (logprobs, entropy, top_logprobs))
+    return out.view(logits.shape)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top):
@@ -127,11 +159,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     """
     top = int(top)
     _checked(logits, tokens, top)
-    shape, V = tokens.shape, logits.shape[-1]
-    rows = logits.reshape(-1, V)
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
-    flat = tokens.reshape(-1).contiguous()
+    shape = tokens.shape
+    rows, flat = _rows(logits, tokens)
     if followed(logits):
         no_tangents("token_logprobs", logits)
         out = _TokenLogprobs.apply(rows, flat, top)

@@ -30,7 +30,7 @@ def no_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
         raise RuntimeError(f"{name} has no forward-mode derivative; unpack its inputs")
 
 
-def _output(like: torch.Tensor) -> torch.Tensor:
+def new_rows(like: torch.Tensor) -> torch.Tensor:
     """A tensor like ``like``, in its layout where that has rows of the last dimension, else contiguous."""
     out = torch.empty_like(like)
     if out.stride(-1) != 1 or any(s * out.element_size() % 16 for s in out.stride()[:-1]):
@@ -146,10 +146,10 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
     if known is not None and not (query.data_ptr() | keys.data_ptr() | cos.data_ptr() | sin.data_ptr()
                                   | _lib.ptr(q_weight) | _lib.ptr(k_weight)) % 16:
         a, tensors = _lib.RotateHeadsArgs.from_buffer_copy(known), given
-        q_out, k_out = _output(query), _output(keys)
+        q_out, k_out = new_rows(query), new_rows(keys)
     else:
         a, *tensors = _checked(*given, eps, interleaved)
-        q_out, k_out = _output(query), _output(keys)
+        q_out, k_out = new_rows(query), new_rows(keys)
         _strides(a, "qo", q_out), _strides(a, "ko", k_out)
         if all(x is y for x, y in zip(given, tensors)):
             _lib.keep_template(key, a)
@@ -161,13 +161,13 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
     return q_out, k_out, a, tensors
 
 
-def _backward(a, tensors, q_grad, k_grad, wanted):
+def _backward(a, tensors, q_grad, k_grad, wanted, like=None):
     """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no)."""
     query, keys, cos, sin, positions, q_weight, k_weight = tensors
     a = _lib.RotateHeadsArgs.from_buffer_copy(a)
     t_axis = 0 if query.dim() == 3 else 2
     q_grad, k_grad = aligned_rows(q_grad.to(query.dtype), t_axis), aligned_rows(k_grad.to(keys.dtype), t_axis)
-    dq, dk = _output(query), _output(keys)
+    dq, dk = (new_rows(t) for t in like or (query, keys))
     weights = [w.new_empty(w.shape) if w is not None and want else None
                for w, want in zip((q_weight, k_weight), wanted)]
     if not a.tokens or not a.batch:
@@ -184,6 +184,15 @@ def _backward(a, tensors, q_grad, k_grad, wanted):
         a.workspace = workspace.data_ptr()
     _lib.launch(_lib.load().dkv_rotate_heads_backward, a, query.device, "dkv_rotate_heads_backward", stream)
     return dq, dk, *weights
+
+
+def gradients(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved):
+    """Gradients of query, keys, q_weight and k_weight (None without one) from those of the outputs."""
+    a, *tensors = _checked(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+    if q_grad.shape != query.shape or k_grad.shape != keys.shape:
+        raise ValueError("q_grad and k_grad must have the shapes of query and keys")
+    _lib.require_device(q_grad, k_grad)
+    return _backward(a, tensors, q_grad, k_grad, (True, True), (query, keys))
 
 
 class _RotateHeads(torch.autograd.Function):

@@ -7,8 +7,9 @@ fake implementation gives output shapes and dtypes without touching the GPU
 runs the same C ABI call as the Python API beside it
 (``quantization.quantize``, ``QuantizedTensor.dequantize``,
 ``mixed.quantize_key_mixed``, ``MixedQuantizedKey.dequantize``,
-``attention.decode_attention``, ``prompt.prompt_attention`` and the operators of
-``blocks``); there is no second implementation.
+``attention.decode_attention``, ``prompt.prompt_attention``, ``rotate.rotate_heads``,
+``logprobs.token_logprobs`` and the operators of ``blocks``); there is no second
+implementation.
 
 ``decode_attention`` reads a ``DartKVCache``, which is not a tensor: the
 operator takes an integer handle from ``cache_handle(cache)``, valid while the
@@ -27,9 +28,11 @@ import torch
 
 from . import attention as _attention
 from . import blocks as _blocks
+from . import logprobs as _logprobs
 from . import mixed as _mixed
 from . import prompt as _prompt
 from . import quantization as _quantization
+from . import rotate as _rotate
 from .cache import DartKVCache
 
 Tensor = torch.Tensor
@@ -244,6 +247,180 @@ def _(query, key_codes, value_codes, key_scale, value_scale, table, lengths, sta
     return query.new_empty(query.shape)
 
 
-__all__ = ["append_blocks", "append_blocks_reported", "block_attention", "cache_handle", "decode_attention",
-           "dequantize_key_mixed", "dequantize_rows", "prompt_attention", "quantize_key_mixed", "quantize_rows",
-           "release_blocks", "reserve_blocks"]
+# (operators of their own, as an operator's results are the same in number whatever its arguments)
+@torch.library.custom_op("dartkv::reserve_shared_blocks", mutates_args=("table", "lengths", "free", "state", "shares"))
+def reserve_shared_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, shares: Tensor, tokens: Tensor,
+                          total: int, block_size: int) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``reserve_blocks`` of tables with forked requests: slots, starts, copies to be made, and positions."""
+    positions = torch.empty(total, dtype=torch.int32, device=table.device)
+    slots, starts, copies = _blocks.reserve_blocks(table, lengths, free, state, tokens, total, block_size=block_size,
+                                                   shares=shares, positions=positions)
+    return slots, starts, copies, positions
+
+
+@reserve_shared_blocks.register_fake
+def _(table, lengths, free, state, shares, tokens, total, block_size):
+    return (lengths.new_empty((total,), dtype=torch.int64), lengths.new_empty((lengths.shape[0] + 1,)),
+            lengths.new_empty((lengths.shape[0], 3)), lengths.new_empty((total,)))
+
+
+@torch.library.custom_op("dartkv::release_shared_blocks", mutates_args=("table", "lengths", "free", "state", "shares"))
+def release_shared_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, shares: Tensor,
+                          tokens: Optional[Tensor], block_size: int) -> None:
+    """``release_blocks`` of tables with forked requests."""
+    _blocks.release_blocks(table, lengths, free, state, tokens, block_size=block_size, shares=shares)
+
+
+@release_shared_blocks.register_fake
+def _(table, lengths, free, state, shares, tokens, block_size):
+    return None
+
+
+@torch.library.custom_op("dartkv::fork_blocks", mutates_args=("table", "lengths", "free", "state", "shares"))
+def fork_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, shares: Tensor, sources: Tensor,
+                tokens: Optional[Tensor], block_size: int) -> None:
+    """Requests become copies of others (-1: stay), of their first ``tokens`` (None: all)."""
+    _blocks.fork_blocks(table, lengths, free, state, shares, sources, tokens, block_size=block_size)
+
+
+@fork_blocks.register_fake
+def _(table, lengths, free, state, shares, sources, tokens, block_size):
+    return None
+
+
+@torch.library.custom_op("dartkv::compact_blocks", mutates_args=("table", "lengths", "free", "state", "shares"))
+def compact_blocks(table: Tensor, lengths: Tensor, free: Tensor, state: Tensor, shares: Tensor,
+                   block_size: int) -> Tensor:
+    """The blocks in use move to the lowest numbers; the copies [blocks // 2, 3] that have to be made."""
+    return _blocks.compact_blocks(table, lengths, free, state, shares, block_size=block_size)
+
+
+@compact_blocks.register_fake
+def _(table, lengths, free, state, shares, block_size):
+    return lengths.new_empty((free.shape[0] // 2, 3))
+
+
+@torch.library.custom_op("dartkv::copy_blocks", mutates_args=("key_codes", "value_codes", "key_scale", "value_scale"))
+def copy_blocks(copies: Tensor, key_codes: Tensor, value_codes: Tensor, key_scale: Tensor, value_scale: Tensor) -> None:
+    """Blocks' first tokens and scales to other blocks, in every layer."""
+    _blocks.copy_blocks(copies, key_codes, value_codes, key_scale, value_scale)
+
+
+@copy_blocks.register_fake
+def _(copies, key_codes, value_codes, key_scale, value_scale):
+    return None
+
+
+@torch.library.custom_op("dartkv::append_rotated_blocks",
+                         mutates_args=("key_codes", "value_codes", "key_scale", "value_scale", "nonfinite"))
+def append_rotated_blocks(query: Tensor, keys: Tensor, values: Tensor, cos: Tensor, sin: Tensor, positions: Tensor,
+                          slots: Tensor, key_codes: Tensor, value_codes: Tensor, key_scale: Tensor,
+                          value_scale: Tensor, nonfinite: Tensor, q_weight: Optional[Tensor] = None,
+                          k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tensor:
+    """The rotated queries; keys, normed and rotated, and values go into their slots."""
+    return _blocks.append_rotated_blocks(query, keys, values, cos, sin, positions, slots, key_codes, value_codes,
+                                         key_scale, value_scale, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                         interleaved=interleaved, nonfinite=nonfinite)
+
+
+@append_rotated_blocks.register_fake
+def _(query, keys, values, cos, sin, positions, slots, key_codes, value_codes, key_scale, value_scale, nonfinite,
+      q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    return query.new_empty(query.shape)
+
+
+# ---- norm and rotation, log probabilities: with gradients (no reference counterpart) ----
+
+@torch.library.custom_op("dartkv::rotate_heads", mutates_args=())
+def rotate_heads(query: Tensor, keys: Tensor, cos: Tensor, sin: Tensor, positions: Optional[Tensor] = None,
+                 q_weight: Optional[Tensor] = None, k_weight: Optional[Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    """RMS norm of each head and its rotation by the token's position."""
+    with torch.no_grad():
+        return _rotate.rotate_heads(query, keys, cos, sin, positions, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                    interleaved=interleaved)
+
+
+@rotate_heads.register_fake
+def _(query, keys, cos, sin, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    return _rotate.new_rows(query), _rotate.new_rows(keys)
+
+
+@torch.library.custom_op("dartkv::rotate_heads_backward", mutates_args=())
+def rotate_heads_backward(q_grad: Tensor, k_grad: Tensor, query: Tensor, keys: Tensor, cos: Tensor, sin: Tensor,
+                          positions: Optional[Tensor], q_weight: Optional[Tensor], k_weight: Optional[Tensor],
+                          eps: float, interleaved: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Gradients of query, keys and the weights (empty where there is no weight)."""
+    dq, dk, *weights = _rotate.gradients(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weight, eps,
+                                         interleaved)
+    return dq, dk, *(query.new_empty(0) if w is None else w for w in weights)
+
+
+@rotate_heads_backward.register_fake
+def _(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved):
+    return (_rotate.new_rows(query), _rotate.new_rows(keys),
+            *(query.new_empty(0) if w is None else w.new_empty(w.shape) for w in (q_weight, k_weight)))
+
+
+def _rotate_setup(ctx, inputs, output):
+    query, keys, cos, sin, positions, q_weight, k_weight, ctx.eps, ctx.interleaved = inputs
+    ctx.save_for_backward(query, keys, cos, sin, positions, q_weight, k_weight)
+
+
+def _rotate_backward(ctx, q_grad, k_grad):
+    query, keys, cos, sin, positions, q_weight, k_weight = ctx.saved_tensors
+    dq, dk, dwq, dwk = torch.ops.dartkv.rotate_heads_backward(q_grad, k_grad, query, keys, cos, sin, positions, q_weight,
+                                                              k_weight, ctx.eps, ctx.interleaved)
+    return dq, dk, None, None, None, None if q_weight is None else dwq, None if k_weight is None else dwk, None, None
+
+
+rotate_heads.register_autograd(_rotate_backward, setup_context=_rotate_setup)
+
+
+@torch.library.custom_op("dartkv::token_logprobs", mutates_args=())
+def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """``TokenLogprobs``' four, and each row's maximum and log2 of its sum, which the gradient needs."""
+    return _logprobs.with_moments(logits, tokens, top)
+
+
+@token_logprobs.register_fake
+def _(logits, tokens, top=0):
+    shape = tuple(tokens.shape)
+    f32 = dict(dtype=torch.float32)
+    return (logits.new_empty(shape, **f32), logits.new_empty(shape, **f32), logits.new_empty((*shape, top), **f32),
+            logits.new_empty((*shape, top), dtype=torch.int64), logits.new_empty((*shape, 2), **f32))
+
+
+@torch.library.custom_op("dartkv::token_logprobs_backward", mutates_args=())
+def token_logprobs_backward(logprobs: Tensor, entropy: Tensor, top_logprobs: Tensor, logits: Tensor, tokens: Tensor,
+                            moments: Tensor, row_entropy: Tensor, top_tokens: Tensor) -> Tensor:
+    """The gradient of the logits from those of the log probabilities, the entropy and the alternatives."""
+    return _logprobs.gradient(logprobs, entropy, top_logprobs, logits, tokens, moments, row_entropy, top_tokens)
+
+
+@token_logprobs_backward.register_fake
+def _(logprobs, entropy, top_logprobs, logits, tokens, moments, row_entropy, top_tokens):
+    return logits.new_empty(logits.shape)
+
+
+def _logprobs_setup(ctx, inputs, output):
+    logits, tokens, _ = inputs
+    _, entropy, _, top_tokens, moments = output
+    ctx.save_for_backward(logits, tokens, moments, entropy, top_tokens)
+    ctx.mark_non_differentiable(top_tokens, moments)
+
+
+def _logprobs_backward(ctx, logprobs, entropy, top_logprobs, _, __):
+    logits, tokens, moments, row_entropy, top_tokens = ctx.saved_tensors
+    return torch.ops.dartkv.token_logprobs_backward(logprobs, entropy, top_logprobs, logits, tokens, moments, row_entropy,
+                                                    top_tokens), None, None
+
+
+token_logprobs.register_autograd(_logprobs_backward, setup_context=_logprobs_setup)
+
+
+__all__ = ["append_blocks", "append_blocks_reported", "append_rotated_blocks", "block_attention", "cache_handle",
+           "compact_blocks", "copy_blocks", "decode_attention", "dequantize_key_mixed", "dequantize_rows", "fork_blocks",
+           "prompt_attention", "quantize_key_mixed", "quantize_rows", "release_blocks", "release_shared_blocks",
+           "reserve_blocks", "reserve_shared_blocks", "rotate_heads", "rotate_heads_backward", "token_logprobs",
+           "token_logprobs_backward"]
