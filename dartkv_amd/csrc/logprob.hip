@@ -563,8 +563,9 @@ __global__ void __launch_bounds__(kThreads) logprob_backward(GradParams p) {
   }
 }
 
-// Rows from which on each has one wave in place of four: 4,096 x 32,003 with twenty alternatives 114 us in place of 137,
-// 65,536 x 1,000 70 and 240, 2,048 x 32,000 with five 41 and 48 (1,024: the card is not full).
+// Rows from which on each has one wave in place of four: 4,096 x 32,003 with twenty alternatives 91 us in place of 120,
+// 65,536 x 1,000 42 and 113, 2,048 x 32,000 with five 45 and 45; 1,024 x 151,936, which leave the card half empty, 98 and
+// 58.
 constexpr int64_t kManyRows = 2048;
 
 // Parts of a row: enough workgroups for the card (four a CU) where there are few rows, none smaller than kPartChunks steps

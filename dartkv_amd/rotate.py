@@ -138,7 +138,8 @@ def _point(a, query, keys, cos, sin, positions, q_weight, k_weight) -> None:
 
 
 def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved):
-    """The outputs, and what a backward pass takes of the call."""
+    """The outputs, and what a backward pass takes of the call: its arguments, its tensors with aligned rows, and what
+    the arguments are kept by (None where rows had to be copied)."""
     given = (query, keys, cos, sin, positions, q_weight, k_weight)
     key = ("rotate", eps, interleaved, tuple(t is None for t in given),
            _lib.layouts(*(t for t in given if t is not None)))
@@ -154,32 +155,45 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
         if all(x is y for x, y in zip(given, tensors)):
             _lib.keep_template(key, a)
             a = _lib.RotateHeadsArgs.from_buffer_copy(a)
+        else:
+            key = None
     if a.tokens and a.batch:
         _point(a, *tensors)
         a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
         _lib.launch(_lib.load().dkv_rotate_heads, a, query.device, "dkv_rotate_heads")
-    return q_out, k_out, a, tensors
+    return q_out, k_out, a, tensors, key
 
 
-def _backward(a, tensors, q_grad, k_grad, wanted, like=None):
-    """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no)."""
+def _backward(a, tensors, q_grad, k_grad, wanted, like=None, key=None):
+    """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no).  ``key``: what the
+    arguments are kept by, beside the gradients' layouts."""
     query, keys, cos, sin, positions, q_weight, k_weight = tensors
-    a = _lib.RotateHeadsArgs.from_buffer_copy(a)
-    t_axis = 0 if query.dim() == 3 else 2
-    q_grad, k_grad = aligned_rows(q_grad.to(query.dtype), t_axis), aligned_rows(k_grad.to(keys.dtype), t_axis)
     dq, dk = (new_rows(t) for t in like or (query, keys))
     weights = [w.new_empty(w.shape) if w is not None and want else None
                for w, want in zip((q_weight, k_weight), wanted)]
     if not a.tokens or not a.batch:
         return dq, dk, *(w if w is None else w.zero_() for w in weights)
-    for name, t in (("qg", q_grad), ("kg", k_grad), ("qo", dq), ("ko", dk)):
-        _strides(a, name, t)
+    if key is not None:
+        key = ("rotate_backward", key, wanted, _lib.layouts(q_grad, k_grad))
+    known = None if key is None else _lib.template(key)
+    if known is None or (q_grad.data_ptr() | k_grad.data_ptr()) % 16:
+        t_axis = 0 if query.dim() == 3 else 2
+        given = q_grad, k_grad
+        q_grad, k_grad = aligned_rows(q_grad.to(query.dtype), t_axis), aligned_rows(k_grad.to(keys.dtype), t_axis)
+        known = _lib.RotateHeadsArgs.from_buffer_copy(a)
+        for name, t in (("qg", q_grad), ("kg", k_grad), ("qo", dq), ("ko", dk)):
+            _strides(known, name, t)
+        known.workspace_bytes = 0
+        if any(w is not None for w in weights):
+            known.workspace_bytes = _lib.load().dkv_rotate_heads_backward_workspace_bytes(known)
+        if key is not None and q_grad is given[0] and k_grad is given[1]:
+            _lib.keep_template(key, known)
+    a = _lib.RotateHeadsArgs.from_buffer_copy(known)
     _point(a, *tensors)
     a.q_grad, a.k_grad, a.q_out, a.k_out = q_grad.data_ptr(), k_grad.data_ptr(), dq.data_ptr(), dk.data_ptr()
     a.q_weight_grad, a.k_weight_grad = _lib.ptr(weights[0]), _lib.ptr(weights[1])
     stream = _lib.stream_ptr(query.device)
-    if any(w is not None for w in weights):
-        a.workspace_bytes = _lib.load().dkv_rotate_heads_backward_workspace_bytes(a)
+    if a.workspace_bytes:
         workspace = _workspace(query.device, a.workspace_bytes, stream)
         a.workspace = workspace.data_ptr()
     _lib.launch(_lib.load().dkv_rotate_heads_backward, a, query.device, "dkv_rotate_heads_backward", stream)
@@ -198,7 +212,7 @@ def gradients(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weig
 class _RotateHeads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, keys, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        q_out, k_out, ctx.args, tensors = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+        q_out, k_out, ctx.args, tensors, ctx.key = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved)
         ctx.save_for_backward(*tensors)
         return q_out, k_out
 
@@ -206,7 +220,7 @@ class _RotateHeads(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, q_grad, k_grad):
         need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = _backward(ctx.args, ctx.saved_tensors, q_grad, k_grad, need[2:4])
+        dq, dk, dwq, dwk = _backward(ctx.args, ctx.saved_tensors, q_grad, k_grad, need[2:4], key=ctx.key)
         return dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None
 
 
