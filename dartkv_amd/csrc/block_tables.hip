@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = dkv::kMaxRequests;  // 12 bytes each of 160 KiB of LDS (16 with shares)
+constexpr int kFewWriters = 512;  // requests whose ranks are counted one by one
 constexpr int kSlots = 4;  // of a thread, where there are many
 
 struct TablesParams {
@@ -94,9 +95,30 @@ __device__ __forceinline__ int find(const Sum* sums, int R, uint32_t i) {
   return lo;
 }
 
+// Sorts `n` keys in LDS, the least first.  Each merge first compares mirrored places, then those `stride` apart, always
+// the lesser to the lower place; what lies behind the last would be larger than all, so pairs with it are left out.
+__device__ __forceinline__ void sort_keys(uint64_t* keys, int n) {
+  for (int size = 1; 1 << (size - 1) < n; ++size) {
+    for (int stride = size; stride > 0; --stride) {
+      // pair i of the step: the lower place is in the first half of its group of 2^stride
+      const int half = 1 << (stride - 1), pairs = (n >> stride) * half + half;
+      for (int i = threadIdx.x; i < pairs; i += kThreads) {
+        const int group = i >> (stride - 1) << stride, at = i & (half - 1), low = group + at;
+        const int high = stride == size ? group + 2 * half - 1 - at : low + half;
+        if (high >= n) continue;
+        const uint64_t a = keys[low], b = keys[high];
+        if (a > b) keys[low] = b, keys[high] = a;
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // The blocks that requests have to copy: copied[r] is the shared block that request r writes into, or -1 where it does
-// not, or is the last of all its holders.
-__device__ __forceinline__ void find_copies(const TablesParams& p, int32_t* copied) {
+// not, or is the last of all its holders.  `keys`: LDS of 8 bytes a request.  Many writers' ranks come from sorting them by
+// block and request (8,190 requests: a reserve of 395 us in place of 1,600 where each looks at all before it, 1,024: 51 and
+// 56; 256 do that in 4).
+__device__ __forceinline__ void find_copies(const TablesParams& p, int32_t* copied, uint64_t* keys) {
   static_assert((kMaxRequests + kThreads - 1) / kThreads <= 32, "a bit for each of a thread's requests");
   __shared__ int32_t any;
   if (threadIdx.x == 0) any = 0;
@@ -109,10 +131,30 @@ __device__ __forceinline__ void find_copies(const TablesParams& p, int32_t* copi
       if (block < 0 || block >= p.blocks || p.shares[block] <= 0) block = -1;
     }
     copied[r] = block;
+    keys[r] = block >= 0 ? (uint64_t)(uint32_t)block << 32 | (uint32_t)r : ~0ull;
     if (block >= 0) any = 1;
   }
   __syncthreads();
   if (!any) return;
+  if (p.R > kFewWriters) {
+    sort_keys(keys, p.R);
+    for (int i = threadIdx.x; i < p.R; i += kThreads) {
+      const uint64_t key = keys[i];
+      if (key == ~0ull) break;
+      const uint32_t block = (uint32_t)(key >> 32);
+      int lo = 0, hi = i;  // the block's first writer
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if ((uint32_t)(keys[mid] >> 32) < block)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      if (i - lo >= p.shares[block]) copied[(uint32_t)key] = -1;
+    }
+    __syncthreads();
+    return;
+  }
   uint32_t keeps = 0;
   for (int r = threadIdx.x, i = 0; r < p.R; r += kThreads, ++i) {
     const int32_t block = copied[r];
@@ -175,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) block_tables(TablesParams p) {
   if (tid == 0) flags = 0;
   const int64_t count = p.state[0];
 
-  if constexpr (SHARED) find_copies(p, copied);
+  if constexpr (SHARED) find_copies(p, copied, (uint64_t*)sums);
   Sum running = {0, 0};
   int32_t bad = 0;
   for (int base = 0; base < p.R; base += kThreads) {
