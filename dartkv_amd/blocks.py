@@ -248,8 +248,6 @@ def _checked_copy(copies, key_codes, value_codes, key_scale, value_scale):
     layers, blocks, heads, block_size, D = pools[0].shape
     if D == 0 or D % 16 or D > MAX_BLOCK_HEAD_DIM:
         raise ValueError(f"head_dim must be a multiple of 16 up to {MAX_BLOCK_HEAD_DIM}")
-    if 2 * layers * heads >= 1 << 16:
-        raise ValueError("copy_blocks takes fewer than 2^15 heads of all layers together")
     if any(t.data_ptr() % 16 or t.stride(0) % 16 for t in pools[:2]):
         raise ValueError("key_codes and value_codes must have 16-byte aligned layers")
     a = _lib.CopyBlocksArgs()

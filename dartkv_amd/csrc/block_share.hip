@@ -444,20 +444,22 @@ struct CopyParams {
   int64_t stride[2], scale_stride[2];  // of a layer
   int64_t count, blocks;
   int32_t H, bs, D, heads;
+  uint32_t across;
 };
 
-// p.heads KV heads' keys or values of a layer for each workgroup of y, entries x, x + X, .. of 64 X at a time: a lane looks
-// at each.
+// Workgroup x + p.across * y: p.heads KV heads' keys or values of a layer for each y, entries x, x + p.across, .. of
+// 64 p.across at a time: a lane looks at each.
 __global__ void __launch_bounds__(kThreads) block_copy(CopyParams p) {
   const int lane = threadIdx.x & 63;
   const uint32_t pieces = (p.H + p.heads - 1) / p.heads;
-  const uint32_t piece = blockIdx.y % pieces, rest = blockIdx.y / pieces, which = rest & 1, layer = rest >> 1;
+  const uint32_t y = blockIdx.x / p.across, x = blockIdx.x - y * p.across;
+  const uint32_t piece = y % pieces, rest = y / pieces, which = rest & 1, layer = rest >> 1;
   const int first = piece * p.heads, heads = p.H - first < p.heads ? p.H - first : p.heads;
   const int64_t part = (int64_t)p.bs * p.D;
   uint8_t* codes = p.codes[which] + layer * p.stride[which] + first * part;
   float* scale = p.scale[which] + layer * p.scale_stride[which] + first;
-  for (int64_t base = blockIdx.x; base < p.count; base += 64ll * gridDim.x) {
-    const int64_t mine = base + (int64_t)lane * gridDim.x;
+  for (int64_t base = x; base < p.count; base += 64ll * p.across) {
+    const int64_t mine = base + (int64_t)lane * p.across;
     int32_t from = -1, to = -1, tokens = 0;
     if (mine < p.count) from = p.copies[3 * mine], to = p.copies[3 * mine + 1], tokens = p.copies[3 * mine + 2];
     uint64_t real = __ballot(from >= 0 && from < p.blocks && to >= 0 && to < p.blocks && from != to);
@@ -472,17 +474,17 @@ __global__ void __launch_bounds__(kThreads) block_copy(CopyParams p) {
       if ((int)threadIdx.x < heads) scale[target * p.H + threadIdx.x] = scale[source * p.H + threadIdx.x];
       constexpr int kDeep = 8;
       for (uint32_t i = threadIdx.x; i < all; i += kDeep * kThreads) {
-        u32x4 x[kDeep];
+        u32x4 data[kDeep];
         uint32_t at[kDeep];
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
           const uint32_t u = i + k * kThreads, h = u / units;
           at[k] = h * (uint32_t)part + (u - h * units) * 16;
-          if (u < all) x[k] = *(const u32x4*)(src + at[k]);
+          if (u < all) data[k] = *(const u32x4*)(src + at[k]);
         }
 #pragma unroll
         for (int k = 0; k < kDeep; ++k)
-          if (i + k * kThreads < all) *(u32x4*)(dst + at[k]) = x[k];
+          if (i + k * kThreads < all) *(u32x4*)(dst + at[k]) = data[k];
       }
     }
   }
@@ -596,7 +598,7 @@ extern "C" int dkv_copy_blocks(const dkv_copy_blocks_args* args, void* stream) {
   DKV_CHECK(a.D >= 16 && a.D <= 512 && a.D % 16 == 0, DKV_ERR_INVALID,
             "dkv_copy_blocks: head_dim must be a multiple of 16 up to 512");
   DKV_CHECK(a.count >= 0 && a.layers >= 1 && a.blocks >= 1 && a.blocks < (1ll << 31) && a.H >= 1 &&
-                2 * a.layers * a.H < 65536,
+                a.layers < (1 << 20) && a.H < (1 << 20) && 2 * a.layers * a.H < (1ll << 30),
             DKV_ERR_INVALID, "dkv_copy_blocks: bad counts");
   if (a.count == 0) return DKV_OK;
   DKV_CHECK(a.copies && a.key_codes && a.value_codes && a.key_scale && a.value_scale, DKV_ERR_INVALID,
@@ -605,13 +607,14 @@ extern "C" int dkv_copy_blocks(const dkv_copy_blocks_args* args, void* stream) {
             DKV_ERR_INVALID, "dkv_copy_blocks: codes must be 16-byte aligned");
   CopyParams p = {a.copies, {a.key_codes, a.value_codes}, {a.key_scale, a.value_scale}, {a.key_stride, a.value_stride},
                   {a.key_scale_stride, a.value_scale_stride}, a.count, a.blocks, (int32_t)a.H, (int32_t)a.block_size,
-                  (int32_t)a.D, 1};
+                  (int32_t)a.D, 1, 1};
   // 32 KiB of a whole block for a workgroup (at most kThreads heads, whose scales its threads copy)
   const int64_t heads = 32768 / (a.block_size * a.D);
   p.heads = (int32_t)(heads < 1 ? 1 : heads > a.H ? a.H : heads);
   const int64_t y = 2 * a.layers * ((a.H + p.heads - 1) / p.heads);
   int64_t x = 65536 / y < 1 ? 1 : 65536 / y;
   x = x > a.count ? a.count : x;
-  hipLaunchKernelGGL(block_copy, dim3((unsigned)x, (unsigned)y), dim3(kThreads), 0, (hipStream_t)stream, p);
+  p.across = (uint32_t)x;
+  hipLaunchKernelGGL(block_copy, dim3((unsigned)(x * y)), dim3(kThreads), 0, (hipStream_t)stream, p);
   return dkv_check_launch("dkv_copy_blocks");
 }

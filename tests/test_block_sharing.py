@@ -364,6 +364,20 @@ def test_many_copies_of_many_heads():
 
 
 @pytest.mark.gpu
+def test_copies_of_very_many_heads():
+    """More heads of all layers than a launch's second dimension counts."""
+    import dartkv_amd as dart
+    layers, H = 260, 140
+    codes = [torch.randint(0, 120, (layers, 3, H, 16, 16), device=DEV, dtype=torch.uint8) for _ in range(2)]
+    scales = [torch.rand(layers, 3, H, device=DEV) for _ in range(2)]
+    want = [t.clone() for t in (*codes, *scales)]
+    for t in want:
+        t[:, 1] = t[:, 2]
+    dart.copy_blocks(torch.tensor([[2, 1, 16]], dtype=torch.int32, device=DEV), *(t.view(E4M3) for t in codes), *scales)
+    assert all(torch.equal(a, b) for a, b in zip((*codes, *scales), want))
+
+
+@pytest.mark.gpu
 def test_a_captured_step_of_beams():
     """fork, reserve and copy, replayed while the beams grow: the same state as eager calls leave."""
     import dartkv_amd as dart
@@ -494,7 +508,7 @@ def test_refusals_of_the_c_entries():
     copy = dict(copies=256, count=3, layers=2, blocks=8, H=2, block_size=16, D=16, key_codes=256, value_codes=256, key_scale=256,
                 value_scale=256, key_stride=4096, value_stride=4096, key_scale_stride=16, value_scale_stride=16)
     for change in (dict(block_size=20), dict(D=24), dict(D=528), dict(count=-1), dict(layers=0), dict(H=0), dict(blocks=0),
-                   dict(layers=1 << 10, H=32), dict(copies=0), dict(key_codes=0), dict(value_scale=0), dict(key_codes=264),
+                   dict(layers=1 << 20), dict(layers=1 << 19, H=1 << 19), dict(copies=0), dict(key_codes=0), dict(value_scale=0), dict(key_codes=264),
                    dict(value_stride=4100)):
         assert lib.dkv_copy_blocks(_lib.CopyBlocksArgs(**{**copy, **change}), None) != 0, change
     assert lib.dkv_copy_blocks(_lib.CopyBlocksArgs(**{**copy, "count": 0}), None) == 0 and lib.dkv_copy_blocks(None, None) == 1

@@ -137,6 +137,27 @@ def test_the_formulas_against_differences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,Hq,Hkv,D,turned,interleaved", [(3301, 33, 7, 128, 128, False), (8201, 3, 1, 72, 36, True),
+                                                           (4801, 3, 1, 40, 18, False), (3301, 40, 1, 64, 32, False)])
+def test_many_rows(T, Hq, Hkv, D, turned, interleaved, dtype):
+    """Waves that make several rows a lane; tokens change between their rows, some of which are no token's."""
+    import dartkv_amd as dart
+    q, k = inputs(T, Hq, Hkv, D, dtype, T)
+    cos, sin = angles(77, turned // 2, torch.float32, T)
+    gen = torch.Generator().manual_seed(T)
+    positions = torch.randint(0, 77, (T,), generator=gen)
+    none = torch.rand(T, generator=gen) < 0.1
+    w = 1 + torch.randn(D, generator=gen) / 2
+    out = dart.rotate_heads(q.to(DEV), k.to(DEV), cos.to(DEV), sin.to(DEV), torch.where(none, -1, positions).to(DEV),
+                            q_weight=w.to(DEV), k_weight=w.to(DEV), interleaved=interleaved)
+    for got, x in zip(out, (q, k)):
+        want, size = reference(x.double(), w.double(), cos.double()[positions], sin.double()[positions], interleaved)
+        assert not got[none.to(DEV)].any()
+        close(got[~none.to(DEV)], want[~none], size[~none], 2.0 ** -18)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_gradients_against_differences_of_the_operator(interleaved):
     """Along one direction in fp32: the quotient is off by the sums' roundings over h, and by what the quotient in 64
@@ -275,7 +296,7 @@ def test_rows_of_zeros_of_large_and_of_infinite_values():
 def test_more_rows_than_a_backward_pass_has_workgroups():
     """Each workgroup goes over its rows in turns; the weights' gradient is the same every time."""
     import dartkv_amd as dart
-    T, H, D = 1500, 33, 64
+    T, H, D = 3000, 33, 64
     q, k = (t.to(DEV) for t in inputs(T, H, 1, D, torch.bfloat16, 15))
     cos, sin = (t.to(DEV) for t in angles(T, 32, torch.float32, 16))
     w = (torch.rand(D) + 0.5).to(DEV)

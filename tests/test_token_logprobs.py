@@ -72,7 +72,7 @@ def rows(T, V, dtype, seed, spread=3.0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("T,V,top", [(1, 1, 1), (3, 2, 2), (2, 63, 63), (5, 64, 64), (1, 1000, 5), (7, 4097, 20),
                                      (2, 8191, 64), (1, 32768, 1), (64, 32001, 20), (3, 151936, 64), (300, 1537, 3),
-                                     (2100, 333, 7), (1, 151936, 0), (9, 2055, 0)])
+                                     (2100, 333, 7), (1, 151936, 0), (9, 2055, 0), (2049, 9001, 33), (2300, 4500, 0)])
 def test_against_64_bits(T, V, top, dtype):
     import dartkv_amd as dart
     x, tokens = rows(T, V, dtype, V + T)
@@ -96,6 +96,13 @@ def test_orders_that_a_selection_finds_hard(kind, dtype):
         logits = x.repeat(T // 2, 1)
         tokens = torch.arange(T) * 31 % V
         check(dart.token_logprobs(logits.to(DEV), tokens.to(DEV), top=33), logits, tokens, 33)
+    # a wave for each of very many rows
+    T = 2200
+    logits, tokens = x.repeat(T // 2, 1).to(DEV), torch.tensor([31, 62]).repeat(T // 2).to(DEV)
+    out = dart.token_logprobs(logits, tokens, top=33)
+    check(dart.TokenLogprobs(*(t[:8] for t in out)), x.repeat(4, 1), tokens[:8], 33)
+    # (rows of an odd size begin at eight offsets, each with an order of its sums)
+    assert all(torch.equal(t, t[:8].repeat(T // 8, *[1] * (t.dim() - 1))) for t in out)
 
 
 @pytest.mark.gpu
@@ -120,6 +127,23 @@ def test_masked_rows(dtype):
     out = dart.token_logprobs(leaf, tokens.to(DEV))
     grad = torch.autograd.grad(out.logprobs[keep].clamp_min(-100).sum() + out.entropy.sum(), leaf)[0]
     assert not grad[2].any() and bool(grad[keep].isfinite().all()) and not grad[1, 100:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [24, 2112])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_maxima_that_come_late(T, dtype):
+    """Rows that rise by far more than 2^z can hold between what a thread reads first and last, and rows that begin with
+    masked logits."""
+    import dartkv_amd as dart
+    x, tokens = rows(3, 30011, dtype, 20)
+    x[0] += torch.linspace(0, 200, 30011).to(dtype)
+    x[1, :20000] = -math.inf
+    x[2, 29000:] += 95
+    tokens = torch.tensor([30000, 25000, 29500])
+    out = dart.token_logprobs(x.repeat(T // 3, 1).to(DEV), tokens.repeat(T // 3).to(DEV), top=11)
+    check(dart.TokenLogprobs(*(t[:24] for t in out)), x.repeat(8, 1), tokens.repeat(8), 11)
+    assert all(torch.equal(t, t[:24].repeat(T // 24, *[1] * (t.dim() - 1))) for t in out)
 
 
 @pytest.mark.gpu
