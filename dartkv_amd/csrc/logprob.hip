@@ -2,11 +2,11 @@
 // of the logits (dkv_token_logprobs, dkv_token_logprobs_backward).
 //
 // With any m, z = (x - m) log2(e), s = sum 2^z and t = sum 2^z z:  log p(v) = (x_v - m) - ln s and
-// H = ln s - ln(2) t / s.  One pass: a thread keeps (m, s, t) of what it has read, m the maximum of its first chunks; only
-// when s leaves 2^16 is m raised, by d in units of z: s becomes 2^-d s and t becomes 2^-d (t - d s).  (Beyond, x - m and
-// ln s would cancel more digits than m itself has.)  x - m is taken before the factor, so a row at the type's lowest value
-// is a row of equals.  Masked logits are -inf, where 2^z z is NaN: steps with one, and those at a row's ends, are computed
-// again with z from -200 on.
+// H = ln s - ln(2) t / s.  One pass: a thread keeps (m, s, t) of what it has read; m is raised to the maximum after 1, 2,
+// 4, .. steps, and when s leaves 2^16, by d in units of z: s becomes 2^-d s and t becomes 2^-d (t - d s).  (Beyond, x - m
+// and ln s would cancel more digits than m itself has.)  x - m is taken before the factor, so a row at the type's lowest
+// value is a row of equals.  Masked logits are -inf, where 2^z z is NaN: steps with one, and those at a row's ends, are
+// computed with z from -200 on.
 //
 // Alternatives: a wave keeps the 64 largest keys it has seen sorted over its lanes (key: the value in an order of
 // integers, then the inverted index, so the lower index wins among equals).  Only what exceeds a bound goes on to a buffer
@@ -356,10 +356,11 @@ __global__ void __launch_bounds__(kThreads) logprob_rows(LogprobParams p) {
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) most = fmaxf(most, top[i]);
     }
-    // The first step, ends of rows, steps with a -inf and those that s grows too much in take the careful way, which raises
-    // m before.
+    // Steps 0, 1, 3, 7, .., ends of rows, steps with a -inf and those that s grows too much in take the careful way, which
+    // raises m before.  (With the first alone, 4,096 x 151,936 came out 5.6e-7 off in the entropy; with these 3.9e-7, the
+    // log probabilities 0.7e-7.)
     Sums sum = sums;
-    bool careful = steps == 0 || !group.whole;
+    bool careful = (steps & (steps + 1)) == 0 || !group.whole;
     if (!careful) {
       group.add(sum);
       careful = !__all(sum.s < 0x1p16f && sum.t == sum.t);
