@@ -65,8 +65,11 @@ def _check_shares(shares, free) -> None:
 
 def _tables_args(name, table, lengths, free, state, tokens, block_size, shares=None):
     """Checked arguments of a call on the tables' state, and the counts as an int32 vector."""
-    key = (name, block_size, tokens is None, shares is None,
-           _lib.layouts(table, lengths, free, state, *(t for t in (tokens, shares) if t is not None)))
+    if shares is None:
+        key = (name, block_size, _lib.layouts(table, lengths, free, state, *(() if tokens is None else (tokens,))))
+    else:
+        key = (name, block_size, tokens is None,
+               _lib.layouts(table, lengths, free, state, shares, *(() if tokens is None else (tokens,))))
     known = _lib.template(key)
     if known is None or (shares is not None and shares.data_ptr() % 16):
         device = _check_state(table, lengths, free, state, block_size)
@@ -170,7 +173,10 @@ def release_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tenso
     if tokens is not None and not isinstance(tokens, torch.Tensor):
         raise TypeError("tokens must be a one-dimensional int32 or int64 tensor")
     a, tokens = _tables_args("release", table, lengths, free, state, tokens, block_size, shares)
-    _launch_shared(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
+    if shares is None:
+        _lib.launch(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
+    else:
+        _launch_shared(_lib.load().dkv_release_blocks, a, table.device, "dkv_release_blocks")
 
 
 def fork_blocks(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, state: torch.Tensor,

@@ -13,9 +13,10 @@
 // in LDS; 64 of them are sorted and merged at once.  The bound is the k-th largest of the lanes' maxima after 1, 2, 4, ..
 // steps, or of the keys kept.  Lanes exchange by permutations within the vector unit, not through LDS.
 //
-// Bound by memory: 4,096 rows of 151,936 in bf16 213 us (5.9 TB/s), with five alternatives 240, with twenty 245; 4,096 of
-// 32,003 53 us (5.0 TB/s).  Before, by vector instructions: a maximum and a careful product for every element 326 us.  64 rows of 151,936
-// with twenty alternatives take 24 us in 16 parts each, a chain of sorting steps and a second launch that joins them.
+// Bound by memory: 4,096 rows of 151,936 in bf16 213 us (5.9 TB/s), with five alternatives 230 to 246, 8,192 with twenty
+// 485 (5.1 TB/s); 4,096 of 32,003 53 us (5.0 TB/s).  Before, by vector instructions: a maximum and a careful product for
+// every element 326 us.  64 rows of 151,936 with twenty alternatives take 24 us in 16 parts each, a chain of sorting steps
+// and a second launch that joins them.
 //
 // Backward, with g the gradient of the given token's log probability (and of the alternatives', each at its own index),
 // G their sum and h the entropy's: dx_v = sum of the g at v - p_v (G + h (log p_v + H)).  One read and one write: 97 us
@@ -162,7 +163,8 @@ struct Best {
     const bool wanted = key > bound;
     const uint64_t mask = __ballot(wanted);
     if (mask == 0) return;
-    if (wanted) buffer[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (wanted) buffer[waiting + before] = key;
     waiting += __builtin_popcountll(mask);
     if (waiting >= 64) flush(buffer, top, lane);
   }
@@ -571,9 +573,9 @@ constexpr int64_t kManyRows = 2048;
 
 // Parts of a row: enough workgroups for the card (four a CU) where there are few rows, none smaller than kPartChunks steps
 // of a thread (1,024 x 151,936: 58 us whole, 65 in two parts; 64 with twenty alternatives: 24 in 16 and in 19).
-int64_t parts_of(int64_t rows, int64_t V, int64_t dtype, int deep) {
+int64_t parts_of(int64_t rows, int64_t V, int64_t dtype, int least) {
   const int64_t E = dtype == kF32 ? 4 : 8, chunks = (V + 2 * E - 1) / E;
-  const int64_t most = (chunks + (int64_t)deep * kThreads - 1) / ((int64_t)deep * kThreads);
+  const int64_t most = (chunks + (int64_t)least * kThreads - 1) / ((int64_t)least * kThreads);
   const int64_t want = (1024 + rows - 1) / rows;
   return want < most ? want : most;
 }

@@ -212,7 +212,8 @@ def gradients(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weig
 class _RotateHeads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, keys, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        q_out, k_out, ctx.args, tensors, ctx.key = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+        q_out, k_out, ctx.args, tensors, ctx.key = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps,
+                                                            interleaved)
         ctx.save_for_backward(*tensors)
         return q_out, k_out
 
