@@ -141,18 +141,19 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
     """The outputs, and what a backward pass takes of the call: its arguments, its tensors with aligned rows, and what
     the arguments are kept by (None where rows had to be copied)."""
     given = (query, keys, cos, sin, positions, q_weight, k_weight)
-    key = ("rotate", eps, interleaved, tuple(t is None for t in given),
-           _lib.layouts(*(t for t in given if t is not None)))
+    key = ("rotate", eps, interleaved, positions is None, q_weight is None, k_weight is None,
+           _lib.layouts(*[t for t in given if t is not None]))
     known = _lib.template(key)
     if known is not None and not (query.data_ptr() | keys.data_ptr() | cos.data_ptr() | sin.data_ptr()
                                   | _lib.ptr(q_weight) | _lib.ptr(k_weight)) % 16:
         a, tensors = _lib.RotateHeadsArgs.from_buffer_copy(known), given
-        q_out, k_out = new_rows(query), new_rows(keys)
+        q_out, k_out = (torch.empty_like(query), torch.empty_like(keys)) if known.alike else (new_rows(query), new_rows(keys))
     else:
         a, *tensors = _checked(*given, eps, interleaved)
         q_out, k_out = new_rows(query), new_rows(keys)
         _strides(a, "qo", q_out), _strides(a, "ko", k_out)
         if all(x is y for x, y in zip(given, tensors)):
+            a.alike = all(x.stride() == torch.empty_like(y).stride() for x, y in ((q_out, query), (k_out, keys)))
             _lib.keep_template(key, a)
             a = _lib.RotateHeadsArgs.from_buffer_copy(a)
         else:
@@ -248,9 +249,9 @@ def rotate_heads(query: torch.Tensor, keys: torch.Tensor, cos: torch.Tensor, sin
     """
     if positions is not None and not isinstance(positions, torch.Tensor):
         raise TypeError("positions must be an int32 or int64 tensor")
-    followed_tensors = [t for t in (query, keys, q_weight, k_weight) if t is not None]
-    if followed(*followed_tensors, cos, sin):
-        no_tangents("rotate_heads", *followed_tensors, cos, sin)
+    given = [t for t in (query, keys, cos, sin, q_weight, k_weight) if t is not None]
+    if followed(*given):
+        no_tangents("rotate_heads", *given)
         if cos.requires_grad or sin.requires_grad:
             raise RuntimeError("rotate_heads has no gradients of cos and sin; detach them")
         return _RotateHeads.apply(query, keys, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
