@@ -11,7 +11,7 @@
 // new holders, a second one writes them and takes the old rows' off; an entry that stays the same (the common beginning
 // of beams) is not counted at all.  A third launch collects what is free and changes the lengths.  A thread has one column
 // of kRows rows, whose loads are all in flight, and counts equal blocks below each other (samples of one prompt) at once:
-// 256 rows of 1,000 blocks, 32 of a prompt, released in 5 us (12 with an atomic for each entry) and forked in 14 (21).
+// 256 rows of 1,000 blocks, 32 of a prompt, released in 10 us (18 with an atomic for each entry) and forked in 15 (21).
 // Where the table is small, one workgroup does all of it in one launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
