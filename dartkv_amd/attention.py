@@ -16,6 +16,8 @@ import collections
 import ctypes
 import math
 import os
+import threading
+import weakref
 from typing import Optional, Tuple
 
 import torch
@@ -87,31 +89,54 @@ def _fast_enabled() -> bool:
     return _FAST_ENABLED
 
 
-_workspaces: "collections.OrderedDict[tuple, torch.Tensor]" = collections.OrderedDict()
-_MAX_WORKSPACES = 8  # (device, stream) pairs whose workspace is kept; the least recently used goes first
+class _Buffers:
+    """A thread's workspaces, by (device, stream), the least recently used first."""
+
+    __slots__ = ("by_stream", "__weakref__")
+
+    def __init__(self) -> None:
+        self.by_stream: "collections.OrderedDict[tuple, torch.Tensor]" = collections.OrderedDict()
+
+
+class _ThreadBuffers(threading.local):
+    def __init__(self) -> None:
+        self.buffers = _Buffers()
+        with _buffers_lock:
+            _all_buffers.add(self.buffers)
+
+
+_buffers_lock = threading.Lock()
+_all_buffers: "weakref.WeakSet[_Buffers]" = weakref.WeakSet()
+_thread_buffers = _ThreadBuffers()
+_MAX_WORKSPACES = 8  # (device, stream) pairs whose workspace a thread keeps; the least recently used goes first
 
 
 def _workspace(device: torch.device, nbytes: int, stream: Optional[int] = None) -> torch.Tensor:
-    """A decode workspace for the split records: one per device and stream, kept and grown as needed (calls
-    on one stream run in order, so they can share it).  At most ``_MAX_WORKSPACES`` are kept (least recently
-    used dropped first; the caching allocator reuses a dropped one once the stream's work has run) and
-    ``release_workspaces`` drops them all.  Under graph capture a fresh one, which the graph keeps."""
+    """A workspace for what a call's launches leave for each other: one per thread, device and stream, kept and grown
+    as needed.  A thread's calls on one stream run in order, so they can share it; another thread's launches on that
+    stream may come between those of a call, so it has its own.  The caller holds it until its launches are made.  At
+    most ``_MAX_WORKSPACES`` of a thread are kept (least recently used dropped first; the caching allocator reuses a
+    dropped one, or one of a thread that ended, once the stream's work has run) and ``release_workspaces`` drops them
+    all.  Under graph capture a fresh one, which the graph keeps."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    kept = _thread_buffers.buffers.by_stream
     key = (device.index, _lib.stream_ptr(device) if stream is None else stream)
-    ws = _workspaces.get(key)
+    ws = kept.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        while len(_workspaces) > _MAX_WORKSPACES:
-            _workspaces.popitem(last=False)
-    _workspaces.move_to_end(key)
+        ws = kept[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        while len(kept) > _MAX_WORKSPACES:
+            kept.popitem(last=False)
+    kept.move_to_end(key)
     return ws
 
 
 def release_workspaces() -> None:
-    """Drop the kept decode workspaces (their memory returns to torch's caching allocator, so
+    """Drop the kept workspaces of all threads (their memory returns to torch's caching allocator, so
     ``torch.cuda.empty_cache`` can free it)."""
-    _workspaces.clear()
+    with _buffers_lock:
+        for buffers in list(_all_buffers):
+            buffers.by_stream = collections.OrderedDict()  # (its thread may be using the one it has)
 
 
 def _call_layout(plan, cache: DartKVCache, q3: torch.Tensor, kv_heads: int, head_dim: int, tail, use_fast: bool,

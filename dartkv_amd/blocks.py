@@ -97,7 +97,7 @@ def _tables_args(name, table, lengths, free, state, tokens, block_size, shares=N
 
 
 def _launch_shared(function, a, device, where) -> None:
-    """A call whose workspace is the calls' of its stream."""
+    """A call whose launches pass their records through a workspace."""
     stream = _lib.stream_ptr(device)
     if a.workspace_bytes:
         workspace = _workspace(device, a.workspace_bytes, stream)

@@ -142,7 +142,8 @@ def prompt_attention(query: torch.Tensor, keys: torch.Tensor, values: torch.Tens
         a.q_starts, a.k_starts = query_starts.data_ptr(), key_starts.data_ptr()
     stream = _lib.stream_ptr(query.device)
     if a.workspace_bytes:
-        a.workspace = _workspace(query.device, a.workspace_bytes, stream).data_ptr()
+        workspace = _workspace(query.device, a.workspace_bytes, stream)
+        a.workspace = workspace.data_ptr()
     _lib.launch(_lib.load().dkv_prompt_attention, a, query.device, "dkv_prompt_attention", stream)
     return out
 

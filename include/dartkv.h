@@ -6,7 +6,8 @@
  * (a hipStream_t passed as void*, NULL = default stream), returns immediately,
  * and returns DKV_OK (0) or an error code.  On error, dkv_last_error() returns a
  * thread-local message.  Nothing here allocates device memory: callers pass
- * outputs and workspace.
+ * outputs and workspace.  A call's launches pass records through its workspace, so
+ * one workspace serves the calls of one host thread on one stream.
  *
  * Element types (the *_dtype arguments) use DKV_DTYPE_*.  Sources, outputs,
  * caches and queries may be float64, float32, float16 or bfloat16 (the page
