@@ -141,7 +141,10 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, logprobs, entropy, top_logprobs, _):
-        return _backward(*ctx.saved_tensors, (logprobs, entropy, top_logprobs)), None, None
+        logits, tokens, *rest = ctx.saved_tensors
+        # (hooks of saved tensors, such as those that offload them, may give them back in another layout)
+        rest = [t.contiguous() for t in rest]
+        return _backward(*_rows(logits, tokens), *rest, (logprobs, entropy, top_logprobs)), None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:

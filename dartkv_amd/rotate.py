@@ -215,14 +215,19 @@ class _RotateHeads(torch.autograd.Function):
     def forward(ctx, query, keys, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         q_out, k_out, ctx.args, tensors, ctx.key = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps,
                                                             interleaved)
+        ctx.layouts = _lib.layouts(*(t for t in tensors if t is not None)) if ctx.key is None else ctx.key[-1]
         ctx.save_for_backward(*tensors)
         return q_out, k_out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, q_grad, k_grad):
-        need = ctx.needs_input_grad
-        dq, dk, dwq, dwk = _backward(ctx.args, ctx.saved_tensors, q_grad, k_grad, need[2:4], key=ctx.key)
+        need, args, key, tensors = ctx.needs_input_grad, ctx.args, ctx.key, ctx.saved_tensors
+        given, positions = [t for t in tensors if t is not None], tensors[4]
+        # (hooks of saved tensors, such as those that offload them, may give them back in another layout)
+        if _lib.layouts(*given) != ctx.layouts or any(t.data_ptr() % 16 for t in given if t is not positions):
+            (args, *tensors), key = _checked(*tensors, args.eps, bool(args.interleaved)), None
+        dq, dk, dwq, dwk = _backward(args, tensors, q_grad, k_grad, need[2:4], key=key)
         return dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None
 
 
