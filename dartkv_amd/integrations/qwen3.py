@@ -13,7 +13,8 @@ that the model's backend would run as plain causal attention without a mask
 
 ``attach_dart_fused_attention(model, rotate_heads=True)`` runs the norms of queries and
 keys and the rotary embedding on ``rotate_heads`` (one pass, one rounding, with
-gradients) in every call that does not run on the preparation kernel below.
+gradients) in every call that does not run on the preparation kernel below, unless
+the norms have hooks.
 
 The forward accepts the cache under both keyword names Transformers has used
 (``past_key_values`` in 5.x, ``past_key_value`` in 4.x).
@@ -151,19 +152,29 @@ def _can_run_prompt(attn: nn.Module, query: torch.Tensor, keys: torch.Tensor, va
             and not followed(query, keys, values))
 
 
+def _runs_as_its_class(module: nn.Module) -> bool:
+    """Whether a call of the module is its class's forward and nothing else: no hook, no forward of its own."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or "forward" in module.__dict__
+                or nn.modules.module._has_any_global_hook())
+
+
 def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tensor, cos: torch.Tensor,
                 sin: torch.Tensor) -> bool:
-    """Whether the norms and the rotation of these projections [B, T, H, D] are what ``rotate_heads`` computes."""
+    """Whether the norms and the rotation of these projections [B, T, H, D] are what ``rotate_heads`` computes, and
+    nothing sees or changes what the norms return."""
     norms = (attn.q_norm, attn.k_norm)
-    return (getattr(attn, "dart_rotate_heads", False) and query.device.type == "cuda"
-            and all(type(n) is modules.Qwen3RMSNorm for n in norms)
-            and norms[0].variance_epsilon == norms[1].variance_epsilon
+    if not (getattr(attn, "dart_rotate_heads", False) and query.device.type == "cuda"
+            and all(type(n) is modules.Qwen3RMSNorm and _runs_as_its_class(n) for n in norms)):
+        return False
+    weights = (norms[0].weight, norms[1].weight)
+    return (norms[0].variance_epsilon == norms[1].variance_epsilon
             and query.dtype == keys.dtype and query.dtype in DTYPES and cos.dtype in DTYPES and sin.dtype == cos.dtype
-            and norms[0].weight.dtype == norms[1].weight.dtype and norms[0].weight.dtype in DTYPES
+            and weights[0].dtype == weights[1].dtype and weights[0].dtype in DTYPES
             and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_ROTATE_HEAD_DIM
             and cos.dim() == 3 and cos.shape == sin.shape and cos.shape[0] in (1, query.shape[0])
             and cos.shape[1:] == (query.shape[1], attn.head_dim) and not followed(cos, sin)
-            and not _has_tangent(query, keys, norms[0].weight, norms[1].weight))
+            and not _has_tangent(query, keys, *weights))
 
 
 def _has_tangent(*tensors: torch.Tensor) -> bool:
