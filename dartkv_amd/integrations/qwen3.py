@@ -14,7 +14,7 @@ that the model's backend would run as plain causal attention without a mask
 ``attach_dart_fused_attention(model, rotate_heads=True)`` runs the norms of queries and
 keys and the rotary embedding on ``rotate_heads`` (one pass, one rounding, with
 gradients) in every call that does not run on the preparation kernel below, unless
-the norms have hooks.
+the norms have hooks or hold their weights elsewhere.
 
 The forward accepts the cache under both keyword names Transformers has used
 (``past_key_values`` in 5.x, ``past_key_value`` in 4.x).
@@ -169,6 +169,7 @@ def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tenso
         return False
     weights = (norms[0].weight, norms[1].weight)
     return (norms[0].variance_epsilon == norms[1].variance_epsilon
+            and all(w.device == query.device and tuple(w.shape) == (attn.head_dim,) for w in weights)
             and query.dtype == keys.dtype and query.dtype in DTYPES and cos.dtype in DTYPES and sin.dtype == cos.dtype
             and weights[0].dtype == weights[1].dtype and weights[0].dtype in DTYPES
             and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_ROTATE_HEAD_DIM

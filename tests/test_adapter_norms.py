@@ -66,6 +66,11 @@ def test_hooks_on_all_modules_keep_the_modules():
     assert _runs()
 
 
+def test_weights_elsewhere_keep_the_modules():
+    assert not _runs(_norm(device=types.SimpleNamespace(type="cpu")), _norm(device=types.SimpleNamespace(type="cpu")))
+    assert not _runs(k_norm=_norm(device=types.SimpleNamespace(type="meta")))
+
+
 def _model(**attach):
     torch.manual_seed(0)
     config = transformers.Qwen3Config(vocab_size=128, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
