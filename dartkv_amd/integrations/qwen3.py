@@ -14,7 +14,7 @@ that the model's backend would run as plain causal attention without a mask
 ``attach_dart_fused_attention(model, rotate_heads=True)`` runs the norms of queries and
 keys and the rotary embedding on ``rotate_heads`` (one pass, one rounding, with
 gradients) in every call that does not run on the preparation kernel below, unless
-the norms have hooks or hold their weights elsewhere.
+the norms have hooks, hold their weights elsewhere or would widen the type.
 
 The forward accepts the cache under both keyword names Transformers has used
 (``past_key_values`` in 5.x, ``past_key_value`` in 4.x).
@@ -161,8 +161,8 @@ def _runs_as_its_class(module: nn.Module) -> bool:
 
 def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tensor, cos: torch.Tensor,
                 sin: torch.Tensor) -> bool:
-    """Whether the norms and the rotation of these projections [B, T, H, D] are what ``rotate_heads`` computes, and
-    nothing sees or changes what the norms return."""
+    """Whether the norms and the rotation of these projections [B, T, H, D] are what ``rotate_heads`` computes, in the
+    type that the modules' products would have, and nothing sees or changes what the norms return."""
     norms = (attn.q_norm, attn.k_norm)
     if not (getattr(attn, "dart_rotate_heads", False) and query.device.type == "cuda"
             and all(type(n) is modules.Qwen3RMSNorm and _runs_as_its_class(n) for n in norms)):
@@ -172,6 +172,7 @@ def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tenso
             and all(w.device == query.device and tuple(w.shape) == (attn.head_dim,) for w in weights)
             and query.dtype == keys.dtype and query.dtype in DTYPES and cos.dtype in DTYPES and sin.dtype == cos.dtype
             and weights[0].dtype == weights[1].dtype and weights[0].dtype in DTYPES
+            and all(torch.promote_types(t.dtype, query.dtype) == query.dtype for t in (weights[0], cos))
             and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_ROTATE_HEAD_DIM
             and cos.dim() == 3 and cos.shape == sin.shape and cos.shape[0] in (1, query.shape[0])
             and cos.shape[1:] == (query.shape[1], attn.head_dim) and not followed(cos, sin)

@@ -71,6 +71,15 @@ def test_weights_elsewhere_keep_the_modules():
     assert not _runs(k_norm=_norm(device=types.SimpleNamespace(type="meta")))
 
 
+def test_types_that_the_modules_would_widen_keep_them():
+    """weight * x and x * cos have the wider type of the two."""
+    wide = dict(dtype=torch.float32)
+    assert not _runs(_norm(**wide), _norm(**wide))
+    assert not _runs(angles=torch.float32)
+    assert _runs(_norm(**wide), _norm(**wide), torch.float32, torch.float32)
+    assert _runs(dtype=torch.float32, angles=torch.float32)  # (16-bit weights under fp32 projections: fp32)
+
+
 def _model(**attach):
     torch.manual_seed(0)
     config = transformers.Qwen3Config(vocab_size=128, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
@@ -119,3 +128,14 @@ def test_a_tangent_keeps_the_modules(calls):
         tangent = forward_ad.unpack_dual(out).tangent
         assert tangent is not None and bool((tangent != 0).any())
     assert not calls
+
+
+@pytest.mark.gpu
+def test_fp32_weights_under_16_bit_projections(calls):
+    """As under autocast: the modules give fp32 queries and keys, and so does the attached module."""
+    results = []
+    for on in (False, True):
+        model = _model(rotate_heads=on)
+        with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+            results.append(model(torch.arange(9, device=DEV)[None], use_cache=False).logits)
+    assert not calls and torch.equal(*results)
