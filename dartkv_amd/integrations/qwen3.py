@@ -176,7 +176,16 @@ def _can_rotate(attn: nn.Module, modules, query: torch.Tensor, keys: torch.Tenso
             and attn.head_dim % 8 == 0 and attn.head_dim <= MAX_ROTATE_HEAD_DIM
             and cos.dim() == 3 and cos.shape == sin.shape and cos.shape[0] in (1, query.shape[0])
             and cos.shape[1:] == (query.shape[1], attn.head_dim) and not followed(cos, sin)
-            and not _has_tangent(query, keys, *weights))
+            and not _has_tangent(query, keys, *weights) and not torch.jit.is_tracing())
+
+
+def _rotated(*args, **kwargs):
+    """``rotate_heads``, as an operator where a compiler follows."""
+    if torch.compiler.is_compiling():
+        query, keys, cos, sin = args
+        return torch.ops.dartkv.rotate_heads(query, keys, cos, sin, None, kwargs["q_weight"], kwargs["k_weight"],
+                                             kwargs["eps"])
+    return rotate_heads(*args, **kwargs)
 
 
 def _has_tangent(*tensors: torch.Tensor) -> bool:
@@ -218,7 +227,7 @@ def build_dart_qwen3_attention_class():
             value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
             if _can_rotate(self, modules, query_states, key_states, cos, sin):
                 half = self.head_dim // 2  # (cos and sin hold the angles twice)
-                query_states, key_states = rotate_heads(
+                query_states, key_states = _rotated(
                     query_states.transpose(1, 2), key_states.transpose(1, 2), cos[..., :half], sin[..., :half],
                     q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.variance_epsilon,
                 )

@@ -80,6 +80,12 @@ def test_types_that_the_modules_would_widen_keep_them():
     assert _runs(dtype=torch.float32, angles=torch.float32)  # (16-bit weights under fp32 projections: fp32)
 
 
+def test_a_trace_records_the_modules(monkeypatch):
+    """torch.jit.trace would take what the kernel writes for a constant."""
+    monkeypatch.setattr(torch.jit, "is_tracing", lambda: True)
+    assert not _runs()
+
+
 def _model(**attach):
     torch.manual_seed(0)
     config = transformers.Qwen3Config(vocab_size=128, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
@@ -139,3 +145,21 @@ def test_fp32_weights_under_16_bit_projections(calls):
         with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
             results.append(model(torch.arange(9, device=DEV)[None], use_cache=False).logits)
     assert not calls and torch.equal(*results)
+
+
+@pytest.mark.gpu
+def test_a_compiled_module_has_the_operator_in_its_graph(calls):
+    attn = _model(rotate_heads=True).model.layers[0].self_attn
+    hidden, cos, sin = torch.randn(2, 9, 256, device=DEV), torch.rand(1, 9, 64, device=DEV), torch.rand(1, 9, 64, device=DEV)
+    graphs = []
+
+    def backend(graph, inputs):
+        graphs.append(graph)
+        return graph.forward
+
+    with torch.no_grad():
+        want, _ = attn(hidden, (cos, sin), None)
+        assert len(calls) == 1
+        got, _ = torch.compile(attn, backend=backend, fullgraph=True)(hidden, (cos, sin), None)
+    assert torch.equal(got, want)
+    assert any("rotate_heads" in str(node.target) for node in graphs[0].graph.nodes)
