@@ -104,7 +104,8 @@ def _rows(logits, tokens):
 
 
 def with_moments(logits, tokens, top):
-    """``TokenLogprobs``' four, and the rows' moments [.., 2], which ``gradient`` takes."""
+    """``TokenLogprobs``' four, and the rows' moments [.., 2], which ``gradient`` takes: a reference m and log2 of the sum
+    of e^(x - m)."""
     _checked(logits, tokens, top)
     shape = tokens.shape
     logprobs, entropy, top_logprobs, top_tokens, moments = _forward(*_rows(logits, tokens), top, True)

@@ -379,7 +379,8 @@ rotate_heads.register_autograd(_rotate_backward, setup_context=_rotate_setup)
 
 @torch.library.custom_op("dartkv::token_logprobs", mutates_args=())
 def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """``TokenLogprobs``' four, and each row's maximum and log2 of its sum, which the gradient needs."""
+    """``TokenLogprobs``' four, and what the gradient needs of each row: a reference m, which is not its maximum, and
+    log2 of the sum of e^(x - m)."""
     return _logprobs.with_moments(logits, tokens, top)
 
 

@@ -735,8 +735,9 @@ int dkv_append_rotated_blocks(const dkv_append_blocks_args* args, const dkv_rota
  * probabilities and entropy NaN; NaN logits are no alternatives (where too few others are,
  * top_tokens are -1).
  *
- * stats [rows][2] (optional): the row's maximum and log2 of its sum, which the backward
- * call needs.  workspace (16-byte aligned): dkv_token_logprobs_workspace_bytes.
+ * stats [rows][2] (optional): a reference m and log2 of the sum of e^(x - m) over the
+ * row, which the backward call needs.  m depends on how the row is read and is not its
+ * maximum; m + ln(2) log2(sum) is the logarithm of the sum of e^x.  workspace (16-byte aligned): dkv_token_logprobs_workspace_bytes.
  *
  * The backward call writes the gradient of the logits to grads.out (rows `stride` apart)
  * from those of logprobs, entropy and top_logprobs (NULL: 0); of args it reads logits,
