@@ -157,9 +157,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     NaN.  Logits of -inf have probability 0; a row of nothing else has log probabilities -inf, entropy 0 and no
     gradient.  A NaN or an infinity makes the row's results NaN; a NaN is no alternative (-1 where too few others are).
 
-    Rows may have any stride (a last dimension that is not contiguous is copied).  Gradients of ``logits`` through the
-    log probabilities, the entropy and the alternatives' log probabilities, not twice; a captured backward pass as for
-    ``rotate_heads``.
+    Rows of [rows, V] logits may have any stride and are read in place.  A last dimension that is not contiguous is
+    copied, and so are more leading dimensions that do not fold into one, as ``logits[:, :-1]`` of a batch: the whole of
+    the logits, kept for the backward pass.  Gradients of ``logits`` through the log probabilities, the entropy and the
+    alternatives' log probabilities, not twice; a captured backward pass as for ``rotate_heads``.
     """
     top = int(top)
     _checked(logits, tokens, top)
