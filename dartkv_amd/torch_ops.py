@@ -363,6 +363,8 @@ def _(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weight, eps,
 
 
 def _rotate_setup(ctx, inputs, output):
+    if any(ctx.needs_input_grad[2:4]):
+        raise RuntimeError("rotate_heads has no gradients of cos and sin; detach them")
     query, keys, cos, sin, positions, q_weight, k_weight, ctx.eps, ctx.interleaved = inputs
     ctx.save_for_backward(query, keys, cos, sin, positions, q_weight, k_weight)
 
