@@ -80,6 +80,7 @@ def _forward(logits, tokens, top, stats):
 
 def _backward(logits, tokens, moments, entropy, top_tokens, grads):
     """The gradient of [rows, V] logits from those of logprobs, entropy and top_logprobs (None: 0)."""
+    no_tangents("the gradient of token_logprobs", logits, *grads)
     device, (rows, V) = logits.device, logits.shape
     out = torch.empty(rows, V, dtype=logits.dtype, device=device)
     if rows == 0:
@@ -107,6 +108,7 @@ def with_moments(logits, tokens, top):
     """``TokenLogprobs``' four, and the rows' moments [.., 2], which ``gradient`` takes: a reference m and log2 of the sum
     of e^(x - m)."""
     _checked(logits, tokens, top)
+    no_tangents("token_logprobs", logits)
     shape = tokens.shape
     logprobs, entropy, top_logprobs, top_tokens, moments = _forward(*_rows(logits, tokens), top, True)
     return (logprobs.view(shape), entropy.view(shape), top_logprobs.view(*shape, top), top_tokens.view(*shape, top),

@@ -24,7 +24,7 @@ DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def no_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Operators with a backward pass alone refuse forward-mode tangents."""
+    """Operators with a backward pass alone, and their backward passes, refuse forward-mode tangents."""
     if getattr(forward_ad, "_current_level", 0) >= 0 and any(
             t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{name} has no forward-mode derivative; unpack its inputs")
@@ -169,6 +169,7 @@ def _backward(a, tensors, q_grad, k_grad, wanted, like=None, key=None):
     """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no).  ``key``: what the
     arguments are kept by, beside the gradients' layouts."""
     query, keys, cos, sin, positions, q_weight, k_weight = tensors
+    no_tangents("the gradient of rotate_heads", q_grad, k_grad, query, keys, cos, sin, q_weight, k_weight)
     dq, dk = (new_rows(t) for t in like or (query, keys))
     weights = [w.new_empty(w.shape) if w is not None and want else None
                for w, want in zip((q_weight, k_weight), wanted)]
