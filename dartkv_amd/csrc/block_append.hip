@@ -393,7 +393,7 @@ int append_params(const dkv_append_blocks_args& a, const char* where, AppendPara
   p.span = a.tokens * a.H <= 16384 ? 1 : 64;
   const int64_t units = (a.tokens + p.span - 1) / p.span * 2 * a.H;
   const int64_t grid = (units + kThreads / 64 - 1) / (kThreads / 64);
-  DKV_CHECK(grid < (1ll << 31), DKV_ERR_INVALID, "%s: too many tokens", where);
+  DKV_CHECK(grid < kGridLimit, DKV_ERR_INVALID, "%s: too many tokens", where);
   p.groups = (uint32_t)grid;
   return DKV_OK;
 }
@@ -441,7 +441,7 @@ extern "C" int dkv_append_rotated_blocks(const dkv_append_blocks_args* args, con
   if (p.T == 0) return DKV_OK;
   DKV_CHECK(a.query && a.q_out && a.positions && (a.half == 0 || (a.cos && a.sin)), DKV_ERR_INVALID, "%s: NULL pointer",
             where);
-  DKV_CHECK((uint64_t)p.groups + r.side[0].groups < (1ull << 31), DKV_ERR_INVALID, "%s: too many tokens", where);
+  DKV_CHECK((int64_t)p.groups + r.side[0].groups < kGridLimit, DKV_ERR_INVALID, "%s: too many tokens", where);
   // Queries of many rows have a launch of their own: beside the append's 168 registers too few of them are in flight.
   if (r.steps > 1) {
     RotateParams queries = r;

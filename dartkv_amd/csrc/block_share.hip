@@ -614,6 +614,7 @@ extern "C" int dkv_copy_blocks(const dkv_copy_blocks_args* args, void* stream) {
   const int64_t y = 2 * a.layers * ((a.H + p.heads - 1) / p.heads);
   int64_t x = 65536 / y < 1 ? 1 : 65536 / y;
   x = x > a.count ? a.count : x;
+  DKV_CHECK(x * y < kGridLimit, DKV_ERR_INVALID, "dkv_copy_blocks: too many layers and heads");
   p.across = (uint32_t)x;
   hipLaunchKernelGGL(block_copy, dim3((unsigned)(x * y)), dim3(kThreads), 0, (hipStream_t)stream, p);
   return dkv_check_launch("dkv_copy_blocks");

@@ -8,6 +8,9 @@
 namespace dkv {
 // Defined in capi.hip.
 void set_error(const char* fmt, ...);
+
+// A launch holds fewer than 2^32 threads: fewer than this many workgroups of 256.
+constexpr int64_t kGridLimit = 1ll << 24;
 }  // namespace dkv
 
 #define DKV_CHECK(cond, code, ...)   \

@@ -217,6 +217,8 @@ int run_rotate(const dkv_rotate_heads_args& a, bool backward, const char* where,
                 (!backward || (a.q_grad && a.k_grad)),
             DKV_ERR_INVALID, "%s: NULL pointer", where);
   const RotateShape s = rotate_shape(a.D, a.half);
+  DKV_CHECK(backward || (int64_t)p.side[0].groups + p.side[1].groups < kGridLimit, DKV_ERR_INVALID,
+            "%s: more rows than a launch holds", where);
   if (backward) {
     p.steps = 1;
     for (int i = 0; i < 2; ++i) {
