@@ -591,6 +591,30 @@ int64_t chunks_of(int64_t V, int64_t dtype, int64_t parts) {
   return (each + kThreads - 1) / kThreads * kThreads;
 }
 
+// Rows of a launch.
+constexpr int64_t kMaxRows = kGridLimit / 2;
+
+// Rows in several calls of about as many, none of so few that they would be read in parts.
+template <typename Call>
+int in_turns(const dkv_token_logprobs_args& a, Call call) {
+  const int64_t turns = (a.rows + kMaxRows - 1) / kMaxRows, each = (a.rows + turns - 1) / turns;
+  const int64_t esize = a.dtype == kF32 ? 4 : 2;
+  for (int64_t first = 0; first < a.rows; first += each) {
+    dkv_token_logprobs_args part = a;
+    part.rows = a.rows - first < each ? a.rows - first : each;
+    part.logits = (const char*)a.logits + first * a.stride * esize;
+    part.tokens = (const char*)a.tokens + first * (a.wide_tokens ? 8 : 4);
+    if (a.logprobs) part.logprobs = a.logprobs + first;
+    if (a.entropy) part.entropy = a.entropy + first;
+    if (a.stats) part.stats = a.stats + 2 * first;
+    if (a.top_logprobs) part.top_logprobs = a.top_logprobs + first * a.top;
+    if (a.top_tokens) part.top_tokens = a.top_tokens + first * a.top;
+    const int rc = call(part, first);
+    if (rc != DKV_OK) return rc;
+  }
+  return DKV_OK;
+}
+
 int check_logprobs(const dkv_token_logprobs_args& a, const char* where) {
   DKV_CHECK(a.dtype == kF32 || a.dtype == kF16 || a.dtype == kBF16, DKV_ERR_DTYPE,
             "%s: logits must be bf16, fp16 or fp32", where);
@@ -620,6 +644,8 @@ extern "C" int dkv_token_logprobs(const dkv_token_logprobs_args* args, void* str
             DKV_ERR_INVALID, "%s: NULL pointer", where);
   const int64_t esize = a.dtype == kF32 ? 4 : 2;
   DKV_CHECK(((uintptr_t)a.logits & (esize - 1)) == 0 && a.stride >= 0, DKV_ERR_INVALID, "%s: bad rows", where);
+  if (a.rows > kMaxRows)
+    return in_turns(a, [&](const dkv_token_logprobs_args& part, int64_t) { return dkv_token_logprobs(&part, stream); });
   LogprobParams p = {};
   p.logits = (const char*)a.logits, p.tokens = a.tokens;
   p.logprobs = a.logprobs, p.entropy = a.entropy, p.stats = a.stats;
@@ -635,7 +661,6 @@ extern "C" int dkv_token_logprobs(const dkv_token_logprobs_args* args, void* str
     p.records = (float*)a.workspace;
     p.lists = (uint64_t*)(p.records + 4 * a.rows * parts);
   }
-  DKV_CHECK(a.rows * parts < (1ll << 31), DKV_ERR_INVALID, "%s: too many rows", where);
   const dim3 grid((unsigned)(a.rows * parts)), block(kThreads);
   const hipStream_t s = (hipStream_t)stream;
   const bool alone = parts == 1 && a.rows >= kManyRows;
@@ -676,6 +701,15 @@ extern "C" int dkv_token_logprobs_backward(const dkv_token_logprobs_args* args, 
   DKV_CHECK((((uintptr_t)a.logits | (uintptr_t)grads->out) & (esize - 1)) == 0 && a.stride >= 0 &&
                 grads->stride >= a.vocab,
             DKV_ERR_INVALID, "%s: bad rows", where);
+  if (a.rows > kMaxRows)
+    return in_turns(a, [&](const dkv_token_logprobs_args& part, int64_t first) {
+      dkv_token_logprobs_grads g = *grads;
+      if (g.logprobs) g.logprobs += first;
+      if (g.entropy) g.entropy += first;
+      if (g.top_logprobs) g.top_logprobs += first * a.top;
+      g.out = (char*)g.out + first * g.stride * esize;
+      return dkv_token_logprobs_backward(&part, &g, stream);
+    });
   GradParams p = {};
   p.logits = (const char*)a.logits, p.out = (char*)grads->out, p.tokens = a.tokens;
   p.stats = a.stats, p.entropy = a.entropy;
@@ -685,7 +719,6 @@ extern "C" int dkv_token_logprobs_backward(const dkv_token_logprobs_args* args, 
   p.V = (int32_t)a.vocab, p.wide = a.wide_tokens != 0;
   const int64_t parts = parts_of(a.rows, a.vocab, a.dtype, 1);
   p.splits = (int32_t)parts, p.chunks = chunks_of(a.vocab, a.dtype, parts);
-  DKV_CHECK(a.rows * parts < (1ll << 31), DKV_ERR_INVALID, "%s: too many rows", where);
   const dim3 grid((unsigned)(a.rows * parts)), block(kThreads);
   if (a.dtype == kF32)
     hipLaunchKernelGGL(logprob_backward<kF32>, grid, block, 0, (hipStream_t)stream, p);
