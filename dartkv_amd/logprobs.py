@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -80,12 +81,14 @@ def _forward(logits, tokens, top, stats):
 
 def _backward(logits, tokens, moments, entropy, top_tokens, grads):
     """The gradient of [rows, V] logits from those of logprobs, entropy and top_logprobs (None: 0)."""
-    no_tangents("the gradient of token_logprobs", logits, *grads)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        no_tangents("the gradient of token_logprobs", logits, *grads)
     device, (rows, V) = logits.device, logits.shape
     out = torch.empty(rows, V, dtype=logits.dtype, device=device)
     if rows == 0:
         return out
-    grads = [g if g is None else g.to(torch.float32).contiguous() for g in grads]
+    grads = [g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+             for g in grads]
     a, g = _lib.TokenLogprobsArgs(), _lib.TokenLogprobsGrads()
     a.logits, a.tokens, a.stats, a.entropy = logits.data_ptr(), tokens.data_ptr(), moments.data_ptr(), entropy.data_ptr()
     a.top_tokens = top_tokens.data_ptr()
@@ -144,10 +147,13 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, logprobs, entropy, top_logprobs, _):
-        logits, tokens, *rest = ctx.saved_tensors
+        logits, *rest = ctx.saved_tensors
         # (hooks of saved tensors, such as those that offload them, may give them back in another layout)
-        rest = [t.contiguous() for t in rest]
-        return _backward(*_rows(logits, tokens), *rest, (logprobs, entropy, top_logprobs)), None, None
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        if not all([t.is_contiguous() for t in rest]):
+            rest = [t.contiguous() for t in rest]
+        return _backward(logits, *rest, (logprobs, entropy, top_logprobs)), None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:

@@ -21,6 +21,7 @@ from .prompt import aligned_rows, followed
 
 MAX_ROTATE_HEAD_DIM = 256
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+_MAX_BACKWARD = 32  # arguments of backward passes that are kept for a layout of the forward
 
 
 def no_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -138,8 +139,8 @@ def _point(a, query, keys, cos, sin, positions, q_weight, k_weight) -> None:
 
 
 def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interleaved):
-    """The outputs, and what a backward pass takes of the call: its arguments, its tensors with aligned rows, and what
-    the arguments are kept by (None where rows had to be copied)."""
+    """The outputs, and what a backward pass takes of the call: its arguments, its tensors with aligned rows, and the
+    arguments that are kept for its layouts (None where rows had to be copied)."""
     given = (query, keys, cos, sin, positions, q_weight, k_weight)
     key = ("rotate", eps, interleaved, positions is None, q_weight is None, k_weight is None,
            _lib.layouts(*[t for t in given if t is not None]))
@@ -154,30 +155,31 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
         _strides(a, "qo", q_out), _strides(a, "ko", k_out)
         if all(x is y for x, y in zip(given, tensors)):
             a.alike = all(x.stride() == torch.empty_like(y).stride() for x, y in ((q_out, query), (k_out, keys)))
+            a.backward = {}  # (of backward passes, by the gradients' layouts)
             _lib.keep_template(key, a)
-            a = _lib.RotateHeadsArgs.from_buffer_copy(a)
+            known, a = a, _lib.RotateHeadsArgs.from_buffer_copy(a)
         else:
-            key = None
+            known = None
     if a.tokens and a.batch:
         _point(a, *tensors)
         a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
         _lib.launch(_lib.load().dkv_rotate_heads, a, query.device, "dkv_rotate_heads")
-    return q_out, k_out, a, tensors, key
+    return q_out, k_out, a, tensors, known
 
 
-def _backward(a, tensors, q_grad, k_grad, wanted, like=None, key=None):
-    """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no).  ``key``: what the
-    arguments are kept by, beside the gradients' layouts."""
+def _backward(a, tensors, q_grad, k_grad, wanted, like=None, kept=None):
+    """Gradients of query, keys and the weights (None where there is none, or ``wanted`` says no).  ``kept``: the arguments
+    that are kept for the forward's layouts, with those of its backward passes."""
     query, keys, cos, sin, positions, q_weight, k_weight = tensors
-    no_tangents("the gradient of rotate_heads", q_grad, k_grad, query, keys, cos, sin, q_weight, k_weight)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        no_tangents("the gradient of rotate_heads", q_grad, k_grad, query, keys, cos, sin, q_weight, k_weight)
     dq, dk = (new_rows(t) for t in like or (query, keys))
     weights = [w.new_empty(w.shape) if w is not None and want else None
                for w, want in zip((q_weight, k_weight), wanted)]
     if not a.tokens or not a.batch:
         return dq, dk, *(w if w is None else w.zero_() for w in weights)
-    if key is not None:
-        key = ("rotate_backward", key, wanted, _lib.layouts(q_grad, k_grad))
-    known = None if key is None else _lib.template(key)
+    key = None if kept is None else (wanted, _lib.layouts(q_grad, k_grad))
+    known = None if kept is None else kept.backward.get(key)
     if known is None or (q_grad.data_ptr() | k_grad.data_ptr()) % 16:
         t_axis = 0 if query.dim() == 3 else 2
         given = q_grad, k_grad
@@ -188,8 +190,10 @@ def _backward(a, tensors, q_grad, k_grad, wanted, like=None, key=None):
         known.workspace_bytes = 0
         if any(w is not None for w in weights):
             known.workspace_bytes = _lib.load().dkv_rotate_heads_backward_workspace_bytes(known)
-        if key is not None and q_grad is given[0] and k_grad is given[1]:
-            _lib.keep_template(key, known)
+        if kept is not None and q_grad is given[0] and k_grad is given[1]:
+            if len(kept.backward) >= _MAX_BACKWARD:
+                kept.backward.clear()
+            kept.backward[key] = known
     a = _lib.RotateHeadsArgs.from_buffer_copy(known)
     _point(a, *tensors)
     a.q_grad, a.k_grad, a.q_out, a.k_out = q_grad.data_ptr(), k_grad.data_ptr(), dq.data_ptr(), dk.data_ptr()
@@ -211,24 +215,31 @@ def gradients(q_grad, k_grad, query, keys, cos, sin, positions, q_weight, k_weig
     return _backward(a, tensors, q_grad, k_grad, (True, True), (query, keys))
 
 
+def _rows_of(query, keys, cos, sin) -> tuple:
+    """What a call's arguments hold of its tensors' layouts, but for their sizes."""
+    return query.stride(), keys.stride(), cos.stride(), sin.stride(), query.dtype, cos.dtype
+
+
 class _RotateHeads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, keys, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        q_out, k_out, ctx.args, tensors, ctx.key = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps,
-                                                            interleaved)
-        ctx.layouts = _lib.layouts(*(t for t in tensors if t is not None)) if ctx.key is None else ctx.key[-1]
+        q_out, k_out, ctx.args, tensors, ctx.kept = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps,
+                                                             interleaved)
+        ctx.rows = _rows_of(*tensors[:4])
         ctx.save_for_backward(*tensors)
         return q_out, k_out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, q_grad, k_grad):
-        need, args, key, tensors = ctx.needs_input_grad, ctx.args, ctx.key, ctx.saved_tensors
-        given, positions = [t for t in tensors if t is not None], tensors[4]
+        need, args, kept, tensors = ctx.needs_input_grad, ctx.args, ctx.kept, ctx.saved_tensors
+        query, keys, cos, sin, *vectors = tensors  # (vectors: positions and weights)
         # (hooks of saved tensors, such as those that offload them, may give them back in another layout)
-        if _lib.layouts(*given) != ctx.layouts or any(t.data_ptr() % 16 for t in given if t is not positions):
-            (args, *tensors), key = _checked(*tensors, args.eps, bool(args.interleaved)), None
-        dq, dk, dwq, dwk = _backward(args, tensors, q_grad, k_grad, need[2:4], key=key)
+        if _rows_of(query, keys, cos, sin) != ctx.rows or not all([t is None or t.is_contiguous() for t in vectors]) \
+                or (query.data_ptr() | keys.data_ptr() | cos.data_ptr() | sin.data_ptr()
+                    | _lib.ptr(vectors[1]) | _lib.ptr(vectors[2])) % 16:
+            (args, *tensors), kept = _checked(*tensors, args.eps, bool(args.interleaved)), None
+        dq, dk, dwq, dwk = _backward(args, tensors, q_grad, k_grad, need[2:4], kept=kept)
         return dq if need[0] else None, dk if need[1] else None, dwq, dwk, None, None, None, None, None
 
 
