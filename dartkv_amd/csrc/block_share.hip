@@ -523,7 +523,7 @@ dim3 row_grid(const ShareParams& p) {
 }
 
 // One workgroup does everything where tables and pool are few, as the launches then cost more than their work: a step of
-// 64 beams of 63 blocks (release, fork, reserve, copy) 36 us, with three launches in place of one 42 (host path).
+// 64 beams of 63 blocks (release, fork, reserve, copy) 36 us, 28 of them kernels, and 42 with three launches in place of one.
 bool small(const ShareParams& p) { return (int64_t)p.R * p.max_blocks <= kSmallTable && p.groups == 1; }
 
 template <bool FORK>

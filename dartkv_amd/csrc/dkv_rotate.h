@@ -285,7 +285,8 @@ __device__ __forceinline__ void rotate_rows(const RotateParams& p, const RotateS
 // 155 us, two 149, four 201, whose registers leave two waves a SIMD).
 constexpr int kRotateSteps = 2;
 
-// How a row lies over lanes.
+// How a row lies over lanes.  (32,768 tokens of 32 + 8 heads in bf16, forward: 128 channels in halves 133 us, 5.1 TB/s; 72
+// in halves, so that 36 angles go two at a time, 200, 1.9 TB/s; 96 with 12 angles 215; 80 with 15, one at a time, 520.)
 struct RotateShape {
   int vec, lanes, rows_shift;
 };

@@ -4,23 +4,26 @@
 // With any m, z = (x - m) log2(e), s = sum 2^z and t = sum 2^z z:  log p(v) = (x_v - m) - ln s and
 // H = ln s - ln(2) t / s.  One pass: a thread keeps (m, s, t) of what it has read; m is raised to the maximum after 1, 2,
 // 4, .. steps, and when s leaves 2^16, by d in units of z: s becomes 2^-d s and t becomes 2^-d (t - d s).  (Beyond, x - m
-// and ln s would cancel more digits than m itself has.)  x - m is taken before the factor, so a row at the type's lowest
-// value is a row of equals.  Masked logits are -inf, where 2^z z is NaN: steps with one, and those at a row's ends, are
-// computed with z from -200 on.
+// and ln s would cancel more digits than m itself has.  So m is not the row's maximum.)  x - m is taken before the factor,
+// so a row at the type's lowest value is a row of equals.  Masked logits are -inf, where 2^z z is NaN: steps with one, once
+// that shows, and those at a row's ends are computed with z from -200 on.
 //
 // Alternatives: a wave keeps the 64 largest keys it has seen sorted over its lanes (key: the value in an order of
 // integers, then the inverted index, so the lower index wins among equals).  Only what exceeds a bound goes on to a buffer
 // in LDS; 64 of them are sorted and merged at once.  The bound is the k-th largest of the lanes' maxima after 1, 2, 4, ..
 // steps, or of the keys kept.  Lanes exchange by permutations within the vector unit, not through LDS.
 //
-// Bound by memory: 4,096 rows of 151,936 in bf16 213 us (5.9 TB/s), with five alternatives 230 to 246, 8,192 with twenty
+// Bound by memory: 4,096 rows of 151,936 in bf16 213 to 218 us (5.7 TB/s), with five alternatives 227 to 246, 8,192 with twenty
 // 485 (5.1 TB/s); 4,096 of 32,003 53 us (5.0 TB/s).  Before, by vector instructions: a maximum and a careful product for
 // every element 326 us.  64 rows of 151,936 with twenty alternatives take 24 us in 16 parts each, a chain of sorting steps
-// and a second launch that joins them.
+// and a second launch that joins them.  Nine tenths of 4,096 x 151,936 masked: 293 us in place of 218, with five
+// alternatives 329 in place of 227, and 575 where rows begin with the mask: every -inf is a candidate until there are five
+// others.
 //
 // Backward, with g the gradient of the given token's log probability (and of the alternatives', each at its own index),
 // G their sum and h the entropy's: dx_v = sum of the g at v - p_v (G + h (log p_v + H)).  One read and one write: 97 us
-// for 4,096 rows of 32,003 in bf16 (5.4 TB/s).
+// for 4,096 rows of 32,003 in bf16 (5.4 TB/s).  Logits that do not begin as their gradient within 16 bytes are read one by
+// one (rows cut out of 32,016: 80 us more).
 #include <hip/hip_runtime.h>
 #include <float.h>
 #include <stdint.h>

@@ -679,6 +679,7 @@ int dkv_block_attention(const dkv_block_attention_args* args, void* stream);
  * The backward call takes the gradients of the outputs as q_grad, k_grad, and writes
  * those of the inputs to q_out, k_out, and of the weights to q_weight_grad, k_weight_grad
  * (weight_dtype; NULL: not wanted).  Sums are made in one order, whatever runs beside.
+ * Calls of no tokens launch nothing and write nothing, no weights' gradients either.
  * workspace (16-byte aligned): dkv_rotate_heads_backward_workspace_bytes, where a
  * weight's gradient is wanted.
  *
