@@ -155,7 +155,7 @@ def _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps, interlea
         _strides(a, "qo", q_out), _strides(a, "ko", k_out)
         if all(x is y for x, y in zip(given, tensors)):
             a.alike = all(x.stride() == torch.empty_like(y).stride() for x, y in ((q_out, query), (k_out, keys)))
-            a.backward = {}  # (of backward passes, by the gradients' layouts)
+            a.rows, a.backward = _rows_of(*tensors[:4]), {}  # (of backward passes, by the gradients' layouts)
             _lib.keep_template(key, a)
             known, a = a, _lib.RotateHeadsArgs.from_buffer_copy(a)
         else:
@@ -173,7 +173,10 @@ def _backward(a, tensors, q_grad, k_grad, wanted, like=None, kept=None):
     query, keys, cos, sin, positions, q_weight, k_weight = tensors
     if getattr(forward_ad, "_current_level", 0) >= 0:
         no_tangents("the gradient of rotate_heads", q_grad, k_grad, query, keys, cos, sin, q_weight, k_weight)
-    dq, dk = (new_rows(t) for t in like or (query, keys))
+    if kept is not None and kept.alike:
+        dq, dk = torch.empty_like(query), torch.empty_like(keys)
+    else:
+        dq, dk = (new_rows(t) for t in like or (query, keys))
     weights = [w.new_empty(w.shape) if w is not None and want else None
                for w, want in zip((q_weight, k_weight), wanted)]
     if not a.tokens or not a.batch:
@@ -225,7 +228,7 @@ class _RotateHeads(torch.autograd.Function):
     def forward(ctx, query, keys, q_weight, k_weight, cos, sin, positions, eps, interleaved):
         q_out, k_out, ctx.args, tensors, ctx.kept = _forward(query, keys, cos, sin, positions, q_weight, k_weight, eps,
                                                              interleaved)
-        ctx.rows = _rows_of(*tensors[:4])
+        ctx.rows = _rows_of(*tensors[:4]) if ctx.kept is None else ctx.kept.rows
         ctx.save_for_backward(*tensors)
         return q_out, k_out
 
